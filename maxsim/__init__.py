@@ -14,13 +14,19 @@ from __future__ import annotations
 
 import maxsim_amd as _impl
 from maxsim_amd import (  # noqa: F401  (re-exported)
+    AdamW,
     __all__,
     __version__,
     _pack_padded,
+    adamw_state_values,
+    adamw_step,
     host_checks,
+    layer_norm,
     maxsim_reference,
     maxsim_reference_with_argmax,
+    normalize_embeddings,
     pack_documents,
+    pack_normalized_documents,
     score_candidates_padded,
     score_candidates_padded_backward_reference,
     score_candidates_padded_reference,

@@ -18,6 +18,11 @@ gradients are summed in fp32.  ``.grad`` has the input dtype: the kernels
 round the fp32 sums to nearest even on the way out, the bits autograd's cast
 of fp32 gradients would give, without the separate cast pass.
 
+Not in ``__all__``, which stays the reference's list: the training loss
+(:func:`score_contrastive_cross_entropy`), :func:`pack_documents`, and the
+operators around the scores (:mod:`maxsim_amd.training`: layer norm, unit
+embeddings, AdamW).
+
 The pure-PyTorch ``*_reference`` functions of the reference package are
 exported too (:mod:`maxsim_amd.reference`) for benchmarks and comparisons;
 they are never used by the operators.
@@ -45,6 +50,14 @@ from .reference import (
     score_pairs_packed_backward_reference,
     score_pairs_packed_reference,
     score_pairs_packed_with_argmax_reference,
+)
+from .training import (
+    AdamW,
+    adamw_state_values,
+    adamw_step,
+    layer_norm,
+    normalize_embeddings,
+    pack_normalized_documents,
 )
 
 __version__ = "0.1.0"

@@ -3,9 +3,11 @@
 Produces, next to this file:
 
 * ``libmaxsim_amd.so`` -- the HIP kernels and the C ABI of
-  ``include/maxsim_amd.h`` (hipcc, gfx950; no torch dependency);
+  ``include/maxsim_amd.h`` and ``include/maxsim_amd_training.h`` (hipcc,
+  gfx950; no torch dependency);
 * ``_maxsim_amd_torch.so`` -- the torch operator registrations
-  (``torch_binding.cpp``), linked against ``libmaxsim_amd.so``.
+  (``torch_binding.cpp``, ``torch_training.cpp``), linked against
+  ``libmaxsim_amd.so``.
 
 Run ``python maxsim_amd/_build.py`` (or ``__graft_entry__.build()``); not as
 ``python -m``, which would import the package and its previous build first.  The HIP
@@ -27,7 +29,9 @@ ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = os.environ.get("MAXSIM_AMD_ARCH", "gfx950")
 
 HIP_SOURCES = ["maxsim_fwd.hip", "maxsim_kloop.hip", "maxsim_bwd.hip", "maxsim_pack.hip",
-               "maxsim_ce.hip", "maxsim_check.hip", "maxsim_capi.hip"]
+               "maxsim_ce.hip", "maxsim_check.hip", "maxsim_norm.hip", "maxsim_unit.hip",
+               "maxsim_adamw.hip", "maxsim_capi.hip"]
+TORCH_SOURCES = ["torch_binding.cpp", "torch_training.cpp"]
 LIB = PKG / "libmaxsim_amd.so"
 TORCH_LIB = PKG / "_maxsim_amd_torch.so"
 
@@ -88,15 +92,19 @@ def build_torch_binding() -> Path:
     tdir = Path(torch.__file__).resolve().parent
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     tmp = TORCH_LIB.with_suffix(".so.tmp")
-    cmd = [
-        "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+    objdir = PKG / "_objs"
+    objs = [objdir / (Path(src).stem + ".o") for src in TORCH_SOURCES]
+    _run([[
+        "g++", "-O2", "-std=c++17", "-fPIC",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         "-I", str(tdir / "include"),
         "-I", str(tdir / "include" / "torch" / "csrc" / "api" / "include"),
         "-I", str(ROCM / "include"),
-        str(CSRC / "torch_binding.cpp"),
-        "-o", str(tmp),
+        "-c", str(CSRC / src), "-o", str(obj),
+    ] for src, obj in zip(TORCH_SOURCES, objs)])
+    cmd = [
+        "g++", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs),
         "-L", str(PKG), "-lmaxsim_amd",
         "-L", str(tdir / "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip",
         "-Wl,-rpath,$ORIGIN",

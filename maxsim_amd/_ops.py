@@ -14,7 +14,10 @@ are the fused training loss behind
 :func:`maxsim_amd.score_contrastive_cross_entropy`.  ``maxsim_check_padded``,
 ``maxsim_check_packed`` and ``maxsim_check_contrastive`` queue a device-side
 check of a call's offsets, ids or lengths and return the words that
-``maxsim_check_wait`` waits for.
+``maxsim_check_wait`` waits for.  ``maxsim_layer_norm``,
+``maxsim_normalize_embeddings``, ``maxsim_pack_normalized`` (differentiable in
+C++), ``maxsim_adamw_step`` and their parts are behind
+:mod:`maxsim_amd.training`.
 
 Importing this module loads ``_maxsim_amd_torch.so`` (which pulls in
 ``libmaxsim_amd.so``).  There is no fallback: if the native build is missing
@@ -142,6 +145,57 @@ def _(scores, targets, inv_temperature, reduction):
 def _(grad_loss, scores, lse, targets, inv_temperature, reduction, queries, documents,
       document_offsets, argmax):
     return queries.new_empty(queries.shape), documents.new_empty(documents.shape)
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_layer_norm")
+def _(x, weight, bias, eps):
+    return x.new_empty(x.shape)
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_layer_norm_forward")
+def _(x, weight, bias, eps):
+    rows = (x.numel() // x.shape[-1],)
+    return x.new_empty(x.shape), _f32(x, rows), _f32(x, rows)
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_layer_norm_backward")
+def _(dy, x, mean, rstd, weight, want_dx, want_dweight, want_dbias, weight_dtype):
+    dim = x.shape[-1]
+    return (x.new_empty(x.shape if want_dx else (0,)),
+            x.new_empty((dim if want_dweight else 0,), dtype=weight_dtype),
+            x.new_empty((dim if want_dbias else 0,), dtype=weight_dtype))
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_normalize_embeddings")
+def _(x, lengths, eps):
+    return x.new_empty(x.shape)
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_normalize_embeddings_backward")
+def _(dy, x, lengths, eps):
+    return x.new_empty(x.shape)
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_pack_normalized")
+def _(x, lengths, offsets, packed_rows, eps):
+    return x.new_empty((packed_rows, x.shape[2]))
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_pack_normalized_backward")
+def _(dy, x, lengths, offsets, eps):
+    return x.new_empty(x.shape)
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_adamw_step")
+def _(params, grads, exp_avgs, exp_avg_sqs, scales, masters, lr, lr_tensor, beta1, beta2, eps,
+      weight_decay, step, step_tensor, seed):
+    return None
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_adamw_state_values")
+def _(exp_avg, exp_avg_sq, scales):
+    return (torch.empty_like(exp_avg, dtype=torch.bfloat16),
+            torch.empty_like(exp_avg, dtype=torch.bfloat16))
 
 
 __all__ = ["ops", "NATIVE_LIB", "TORCH_BINDING"]

@@ -1,0 +1,373 @@
+// Layer norm over the last axis, forward and backward.
+//
+//   mu = mean(x), s = 1 / sqrt(mean((x - mu)^2) + eps), xh = (x - mu) s
+//   y  = xh w + b
+//   g  = dy w
+//   dx = s (g - mean(g) - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
+//
+// Memory-bound: the forward reads and writes each element once, the backward
+// reads x and dy and writes dx, at under 20 operations per element.  A row
+// stays in the registers of one group of lanes (maxsim_rows.h), so the mean
+// and then the squared distances from it are taken from the one read: no
+// difference of large sums.  Statistics, sums and the weights' gradients are
+// fp32; y, dx, dw and db are rounded once, to nearest even.
+#include <algorithm>
+
+#include "maxsim_host.h"
+#include "maxsim_rows.h"
+#include "../../include/maxsim_amd_training.h"
+
+namespace maxsim {
+
+struct LnForward {
+  const void* x;
+  int64_t rows, stride;  // stride: elements from row to row of x
+  int dim;
+  const void* weight;
+  const void* bias;
+  float eps;
+  void* y;
+  float* mean;  // both or neither
+  float* rstd;
+};
+
+// Workgroups that take the rows in turn, each group of lanes with its weights
+// in registers for all its rows and the next row's loads in flight.
+template <typename T, typename W, int G, int K>
+__global__ __launch_bounds__(row_threads(G)) void ln_forward_kernel(LnForward a) {
+  using S = typename T::storage;
+  constexpr int V = kVec<T>, GROUPS = row_threads(G) / G;
+  __shared__ float part[2][G > 64 ? G / 64 : 1];
+  const int j = threadIdx.x % G, group = threadIdx.x / G;
+  const int dim = a.dim;
+  const S* x = static_cast<const S*>(a.x);
+  S* y = static_cast<S*>(a.y);
+  const float inv_dim = 1.0f / (float)dim;
+
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  int64_t row = (int64_t)blockIdx.x * GROUPS + group;
+  uint4 next[K] = {};
+  if (row < a.rows) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) next[k] = load_chunk<T>(x + row * a.stride, (j + k * G) * V, dim);
+  }
+  float w[K][V], b[K][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    load_param<W, V>(a.weight, (j + k * G) * V, dim, 1.0f, w[k]);
+    load_param<W, V>(a.bias, (j + k * G) * V, dim, 0.0f, b[k]);
+  }
+  // the workgroup's groups stay together: the reductions need every lane
+  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < a.rows; base += step, row += step) {
+    float f[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) unpack16<T>(next[k], f[k]);
+    if (row + step < a.rows) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        next[k] = load_chunk<T>(x + (row + step) * a.stride, (j + k * G) * V, dim);
+    }
+    float sum[1] = {0.0f};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[0] += f[k][e];
+    group_sums<G>(sum, part[0]);
+    const float mean = sum[0] * inv_dim;
+    float sq[1] = {0.0f};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[k][e] -= mean;
+        sq[0] += (j + k * G) * V + e < dim ? f[k][e] * f[k][e] : 0.0f;
+      }
+    group_sums<G>(sq, part[1]);
+    const float rstd = 1.0f / sqrtf(sq[0] * inv_dim + a.eps);
+    if (row < a.rows) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[k][e] = f[k][e] * rstd * w[k][e] + b[k][e];
+        store_chunk<T>(y + row * dim, (j + k * G) * V, dim, f[k]);
+      }
+      if (a.mean && j == 0) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+      }
+    }
+  }
+}
+
+struct LnBackward {
+  const void* dy;
+  const void* x;
+  int64_t rows, dy_stride, x_stride;
+  int dim;
+  const float* mean;
+  const float* rstd;
+  const void* weight;
+  void* dx;        // NULL: not wanted
+  float* partial;  // [gridDim.x][2][dim] sums of dy xh and dy; NULL: not wanted
+};
+
+// The rows in turn as in the forward; each lane adds up its columns' share of
+// dw and db over its rows, the workgroup joins its groups' (in one order) and
+// writes one partial row, which ln_weight_grad_kernel adds up.
+template <typename T, typename W, int G, int K>
+__global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward a) {
+  using S = typename T::storage;
+  constexpr int V = kVec<T>, GROUPS = row_threads(G) / G;
+  constexpr int COLS = G * K * V;
+  // two chunks per lane of 1024 threads leave no registers for the next row
+  // and the weights (128 per lane): both are loaded where they are used
+  constexpr bool AHEAD = G < 1024 || K == 1;
+  __shared__ float part[2][G > 64 ? 2 * G / 64 : 1];
+  __shared__ float cols[G < 256 ? COLS : 1];
+  const int j = threadIdx.x % G, group = threadIdx.x / G;
+  const int dim = a.dim;
+  const S* x = static_cast<const S*>(a.x);
+  const S* dy = static_cast<const S*>(a.dy);
+  S* dx = static_cast<S*>(a.dx);
+  const float inv_dim = 1.0f / (float)dim;
+
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  int64_t row = (int64_t)blockIdx.x * GROUPS + group;
+  uint4 next_x[K] = {}, next_d[K] = {};
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto load = [&](int64_t r) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      next_x[k] = load_chunk<T>(x + r * a.x_stride, (j + k * G) * V, dim);
+      next_d[k] = load_chunk<T>(dy + r * a.dy_stride, (j + k * G) * V, dim);
+    }
+    next_mean = a.mean[r];
+    next_rstd = a.rstd[r];
+  };
+  if (AHEAD && row < a.rows) load(row);
+  float w[AHEAD ? K : 1][V], dw[K][V], db[K][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if constexpr (AHEAD) load_param<W, V>(a.weight, (j + k * G) * V, dim, 1.0f, w[k]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[k][e] = db[k][e] = 0.0f;
+  }
+  int turn = 0;
+  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < a.rows; base += step, row += step) {
+    float f[K][V], d[K][V];
+    if constexpr (!AHEAD) {
+      asm volatile("" ::: "memory");  // the weights are not kept over the rows
+      load(row);
+    }
+    const float mean = next_mean, rstd = next_rstd;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      unpack16<T>(next_x[k], f[k]);
+      unpack16<T>(next_d[k], d[k]);
+    }
+    const bool here = row < a.rows;
+    if (AHEAD && row + step < a.rows) load(row + step);
+    float sums[2] = {0.0f, 0.0f};
+    // past the row's end dy and w are 0; a group without a row adds nothing
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float(&wk)[V] = w[AHEAD ? k : 0];
+      if constexpr (!AHEAD) load_param<W, V>(a.weight, (j + k * G) * V, dim, 1.0f, wk);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[k][e] = (f[k][e] - mean) * rstd;
+        if (here) {
+          dw[k][e] += d[k][e] * f[k][e];
+          db[k][e] += d[k][e];
+        }
+        d[k][e] *= wk[e];
+        sums[0] += d[k][e];
+        sums[1] += d[k][e] * f[k][e];
+      }
+    }
+    if (dx) {
+      group_sums<G>(sums, part[turn]);
+      turn ^= 1;
+      if (here) {
+        const float c1 = sums[0] * inv_dim, c2 = sums[1] * inv_dim;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) f[k][e] = rstd * (d[k][e] - c1 - f[k][e] * c2);
+          store_chunk<T>(dx + row * dim, (j + k * G) * V, dim, f[k]);
+        }
+      }
+    }
+  }
+  if (!a.partial) return;
+  float* out = a.partial + (int64_t)blockIdx.x * 2 * dim;
+  auto write = [&](float (&v)[K][V], float* to) {
+    if constexpr (G < 256) {
+      // a wave's groups in registers, then one wave after the other
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[k][e] = groups_sum<G>(v[k][e]);
+      for (int wave = 0; wave < row_threads(G) / 64; ++wave) {
+        if ((int)threadIdx.x >> 6 == wave && (threadIdx.x & 63) < G) {
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const int c = (j + k * G) * V + e;
+              cols[c] = wave == 0 ? v[k][e] : cols[c] + v[k][e];
+            }
+        }
+        __syncthreads();
+      }
+      for (int c = threadIdx.x; c < dim; c += row_threads(G)) to[c] = cols[c];
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const int c = (j + k * G) * V + e;
+          if (c < dim) to[c] = v[k][e];
+        }
+    }
+  };
+  write(dw, out);
+  write(db, out + dim);
+}
+
+// dw and db from the partial rows: a workgroup takes 64 columns of one of the
+// two, its 16 waves every sixteenth partial row each, joined in LDS in one
+// order.
+constexpr int kGradWaves = 16;
+template <typename W>
+__global__ __launch_bounds__(64 * kGradWaves) void ln_weight_grad_kernel(
+    const float* __restrict__ partial, int count, int dim, void* dweight, void* dbias) {
+  __shared__ float part[kGradWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane, which = blockIdx.y;
+  float s = 0.0f;
+  if (c < dim) {
+    const float* p = partial + (int64_t)which * dim + c;
+#pragma unroll 8
+    for (int i = wave; i < count; i += kGradWaves) s += p[(int64_t)i * 2 * dim];
+  }
+  part[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || c >= dim) return;
+#pragma unroll
+  for (int w = 1; w < kGradWaves; ++w) s += part[w][lane];
+  auto* out = static_cast<typename W::storage*>(which ? dbias : dweight);
+  if (out) out[c] = from_float<W>(s);
+}
+
+template <typename F>
+static void with_types(maxsim_dtype t, maxsim_dtype w, F&& f) {
+  if (t == MAXSIM_FLOAT32) f(F32{}, F32{});
+  else if (t == MAXSIM_FLOAT16 && w == MAXSIM_FLOAT16) f(F16{}, F16{});
+  else if (t == MAXSIM_FLOAT16) f(F16{}, F32{});
+  else if (w == MAXSIM_BFLOAT16) f(BF16{}, BF16{});
+  else f(BF16{}, F32{});
+}
+
+static int check_layer_norm(maxsim_dtype dtype, maxsim_dtype weight_dtype, int64_t rows,
+                            int64_t dim) {
+  if (int e = check_dtype(dtype)) return e;
+  if (int e = check_dtype(weight_dtype)) return e;
+  if (weight_dtype != dtype && weight_dtype != MAXSIM_FLOAT32)
+    return fail(MAXSIM_ERR_INVALID, "weight_dtype must be the rows' dtype or float32");
+  if (rows < 0) return fail(MAXSIM_ERR_INVALID, "negative size");
+  return check_dim(dim);
+}
+
+// Workgroups of the backward: at most four per CU, and at least eight passes
+// each where there are rows for that, since every workgroup costs a partial
+// row of 8 dim bytes, written and read again.
+static int64_t backward_blocks(maxsim_dtype dtype, int64_t rows, int64_t dim) {
+  int groups = 1;
+  auto take = [&](auto s) { groups = row_threads(s.G) / s.G; };
+  if (dtype == MAXSIM_FLOAT32) with_shape<F32>(dim, take);
+  else with_shape<BF16>(dim, take);
+  const int64_t turns = (rows + groups - 1) / groups;
+  return std::max<int64_t>(1, std::min<int64_t>({turns, 1024, std::max<int64_t>(256, turns / 8)}));
+}
+
+}  // namespace maxsim
+
+using namespace maxsim;
+
+extern "C" {
+
+int maxsim_amd_layer_norm_forward(maxsim_dtype dtype, maxsim_dtype weight_dtype, const void* x,
+                                  int64_t rows, int64_t dim, int64_t row_stride,
+                                  const void* weight, const void* bias, float eps, void* y,
+                                  float* mean, float* rstd, void* stream) {
+  clear_error();
+  if (int e = check_layer_norm(dtype, weight_dtype, rows, dim)) return e;
+  if (!(eps >= 0.0f)) return fail(MAXSIM_ERR_INVALID, "eps must be >= 0");
+  if (row_stride < 0) return fail(MAXSIM_ERR_INVALID, "negative row stride");
+  if (rows == 0) return MAXSIM_OK;
+  if (!x || !y || !mean != !rstd) return fail(MAXSIM_ERR_INVALID, "null pointer argument");
+  const LnForward a{x, rows, row_stride, (int)dim, weight, bias, eps, y, mean, rstd};
+  with_types(dtype, weight_dtype, [&](auto t, auto w) {
+    using T = decltype(t);
+    with_shape<T>(dim, [&](auto s) {
+      constexpr int G = decltype(s)::G, K = decltype(s)::K, threads = row_threads(G);
+      const int64_t need = (rows + threads / G - 1) / (threads / G);
+      const int64_t blocks = std::min<int64_t>(need, (int64_t)device_cus() * (2048 / threads));
+      hipLaunchKernelGGL((ln_forward_kernel<T, decltype(w), G, K>), dim3((unsigned)blocks),
+                         dim3(threads), 0, static_cast<hipStream_t>(stream), a);
+    });
+  });
+  return check_launch("ln_forward_kernel");
+}
+
+size_t maxsim_amd_layer_norm_backward_workspace_size(maxsim_dtype dtype, int64_t rows,
+                                                     int64_t dim) {
+  if (rows <= 0 || dim <= 0 || dim > MAXSIM_AMD_MAX_DIM) return 0;
+  return (size_t)backward_blocks(dtype, rows, dim) * 2 * dim * sizeof(float);
+}
+
+int maxsim_amd_layer_norm_backward(maxsim_dtype dtype, maxsim_dtype weight_dtype, const void* dy,
+                                   int64_t dy_stride, const void* x, int64_t x_stride,
+                                   const float* mean, const float* rstd, const void* weight,
+                                   int64_t rows, int64_t dim, void* dx, void* dweight,
+                                   void* dbias, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  clear_error();
+  if (int e = check_layer_norm(dtype, weight_dtype, rows, dim)) return e;
+  if (dy_stride < 0 || x_stride < 0) return fail(MAXSIM_ERR_INVALID, "negative row stride");
+  if (rows > 0 && (!dy || !x || !mean || !rstd))
+    return fail(MAXSIM_ERR_INVALID, "null pointer argument");
+  const bool weights = dweight || dbias;
+  if (!dx && !weights) return MAXSIM_OK;
+  const int64_t blocks = rows > 0 ? backward_blocks(dtype, rows, dim) : 0;
+  if (weights && rows > 0 &&
+      (!workspace || workspace_bytes < (size_t)blocks * 2 * dim * sizeof(float)))
+    return fail(MAXSIM_ERR_INVALID,
+                "the weights' gradients need a workspace of "
+                "maxsim_amd_layer_norm_backward_workspace_size() bytes");
+  float* partial = weights ? static_cast<float*>(workspace) : nullptr;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (rows > 0) {
+    const LnBackward a{dy, x, rows, dy_stride, x_stride, (int)dim, mean, rstd, weight, dx, partial};
+    with_types(dtype, weight_dtype, [&](auto t, auto w) {
+      using T = decltype(t);
+      with_shape<T>(dim, [&](auto s) {
+        constexpr int G = decltype(s)::G, K = decltype(s)::K;
+        hipLaunchKernelGGL((ln_backward_kernel<T, decltype(w), G, K>), dim3((unsigned)blocks),
+                           dim3(row_threads(G)), 0, st, a);
+      });
+    });
+    if (int e = check_launch("ln_backward_kernel")) return e;
+  }
+  if (!weights) return MAXSIM_OK;
+  with_types(dtype, weight_dtype, [&](auto, auto w) {
+    hipLaunchKernelGGL((ln_weight_grad_kernel<decltype(w)>), dim3((unsigned)((dim + 63) / 64), 2),
+                       dim3(64 * kGradWaves), 0, st, partial, (int)blocks, (int)dim, dweight,
+                       dbias);
+  });
+  return check_launch("ln_weight_grad_kernel");
+}
+
+}  // extern "C"

@@ -7,10 +7,7 @@
 // RuntimeError), makes inputs contiguous and int32, allocates the outputs
 // with the caching allocator and calls the C ABI on the current HIP stream.
 // The C ABI itself never allocates.
-#include <ATen/ATen.h>
 #include <ATen/core/CachingHostAllocator.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
 
 #include <chrono>
@@ -19,10 +16,12 @@
 #include <vector>
 
 #include "maxsim_internal.h"
+#include "torch_common.h"
 
 namespace {
 
 using at::Tensor;
+using namespace maxsim_torch;
 
 maxsim_dtype to_dtype(const Tensor& t) {
   switch (t.scalar_type()) {
@@ -35,15 +34,6 @@ maxsim_dtype to_dtype(const Tensor& t) {
                   t.scalar_type());
   }
   return MAXSIM_FLOAT32;
-}
-
-void check_status(int rc) {
-  TORCH_CHECK(rc == MAXSIM_OK, "maxsim_amd: ", maxsim_amd_last_error());
-}
-
-void* current_stream(const Tensor& t) {
-  return reinterpret_cast<void*>(
-      c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream());
 }
 
 Tensor as_i32(const Tensor& t) {
@@ -63,13 +53,6 @@ void check_embeddings(const Tensor& q, const Tensor& d) {
 void check_on(const Tensor& t, const Tensor& q, const char* name) {
   TORCH_CHECK(t.device() == q.device(), name,
               " must be on the same device as queries");
-}
-
-at::TensorOptions f32_opts(const Tensor& q) {
-  return at::TensorOptions().dtype(at::kFloat).device(q.device());
-}
-at::TensorOptions i32_opts(const Tensor& q) {
-  return at::TensorOptions().dtype(at::kInt).device(q.device());
 }
 
 // ---- layout checks ---------------------------------------------------------

@@ -1,0 +1,250 @@
+"""What lies around the scores in training and indexing: from an encoder's
+hidden states to scored token embeddings, and the step that trains both.
+
+* :func:`layer_norm` -- layer norm over the last axis, differentiable.
+* :func:`normalize_embeddings` -- token embeddings of unit length, those of
+  padding 0; :func:`pack_normalized_documents` -- the same, packed into the
+  inputs of the contrastive functions.  Differentiable.
+* :func:`adamw_step` and :class:`AdamW` -- the AdamW step over many tensors in
+  a few launches, with states in 32 or 8 bits.
+
+The reference leaves these to torch (its training example, README.md:160-205).
+Here they are hand-written HIP kernels behind ``include/maxsim_amd_training.h``:
+one pass over memory each, sums in fp32, 16-bit results rounded once.  All are
+exported from :mod:`maxsim_amd`.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Tuple
+
+import torch
+
+from ._ops import ops
+
+#: Elements of a parameter that share the scales of their 8-bit states.
+STATE_BLOCK = 256
+
+
+def _require_hip(name: str, t: torch.Tensor) -> None:
+    # the operators are registered for HIP tensors alone, and without one the
+    # dispatcher's error names no argument
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a HIP (torch 'cuda') tensor; got {t.device}")
+
+
+# ---------------------------------------------------------------------------
+# Layer norm
+# ---------------------------------------------------------------------------
+def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean) / sqrt(variance + eps) * weight + bias`` over the last axis.
+
+    Args:
+        x: ``[..., dim]`` fp32 / fp16 / bf16, dim up to 16384.  Leading axes
+            that are not one run of rows are copied first.
+        weight, bias: ``[dim]`` in x's dtype or fp32 (both alike); None: 1, 0.
+        eps: added to the variance (over ``dim``), >= 0.
+
+    Returns:
+        ``x.shape`` in x's dtype.  Differentiable with respect to x, weight
+        and bias, each gradient in its tensor's dtype (fp32 sums rounded
+        once, in an order that the sizes alone decide).
+    """
+    _require_hip("x", x)
+    return ops.maxsim_layer_norm(x, weight, bias, eps)
+
+
+# ---------------------------------------------------------------------------
+# Token embeddings of unit length
+# ---------------------------------------------------------------------------
+def normalize_embeddings(x, lengths=None, *, eps: float = 1e-12) -> torch.Tensor:
+    """``x / max(|x|, eps)`` for each token embedding.
+
+    Args:
+        x: ``[..., dim]`` fp32 / fp16 / bf16, dim up to 16384.
+        lengths: ``[N]`` int32/int64 for x ``[N, L, dim]``: tokens at or past
+            a sequence's length become 0 and are never read (they may hold
+            NaN).  A length of 0 leaves the sequence without a token; lengths
+            outside ``[0, L]`` are clamped.
+        eps: > 0; a token no longer than it is divided by it.
+
+    Returns:
+        ``x.shape`` in x's dtype, differentiable with respect to x (padding
+        gets a gradient of 0, whatever comes down for it).
+    """
+    _require_hip("x", x)
+    return ops.maxsim_normalize_embeddings(x, lengths, eps)
+
+
+def pack_normalized_documents(doc_emb, doc_lengths, *,
+                              eps: float = 1e-12) -> Tuple[torch.Tensor, torch.Tensor]:
+    """:func:`maxsim_amd.pack_documents` of :func:`normalize_embeddings` in one
+    pass, differentiable: padded documents ``[Nb, Ld, D]`` with lengths
+    ``[Nb]`` become ``(documents [total, D], document_offsets [Nb + 1] int32)``
+    for the contrastive functions, with every row at unit length.
+
+    Lengths are clamped to ``[0, Ld]``; the host waits for the total row count
+    (the output's size).  Padding is never read and gets a gradient of 0."""
+    if doc_emb.dim() != 3:
+        raise ValueError(f"doc_emb must be 3-D [Nb, Ld, D]; got shape {tuple(doc_emb.shape)}")
+    Nb, Ld, _ = doc_emb.shape
+    if tuple(doc_lengths.shape) != (Nb,):
+        raise ValueError(
+            f"doc_lengths must have shape [Nb={Nb}]; got {tuple(doc_lengths.shape)}")
+    _require_hip("doc_emb", doc_emb)
+    lengths, offsets, total = ops.maxsim_length_offsets(
+        doc_lengths.to(doc_emb.device, non_blocking=True), Ld)
+    return ops.maxsim_pack_normalized(doc_emb, lengths, offsets, total, eps), offsets
+
+
+# ---------------------------------------------------------------------------
+# AdamW
+# ---------------------------------------------------------------------------
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.9, 0.999),
+               eps: float = 1e-8, weight_decay: float = 1e-2, scales=None, masters=None,
+               seed: int = 0) -> None:
+    """One AdamW step (decoupled weight decay) over lists of tensors, in place::
+
+        m = beta1 m + (1 - beta1) g        v = beta2 v + (1 - beta2) g^2
+        p = p (1 - lr weight_decay)
+            - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+
+    Args:
+        params: fp32 / fp16 / bf16 tensors on one device, each dense in memory
+            in any order of its axes; no tensor twice.
+        grads: their gradients, in the parameter's dtype or fp32.
+        exp_avgs, exp_avg_sqs: the states, in the parameters' order in memory:
+            fp32, or uint8 codes with ``scales``.
+        step: number of this step, from 1; or an int64 tensor of one element
+            on the device, read when the kernels run (for a captured graph).
+        lr: a number, or an fp32 tensor of one element on the device.
+        scales: for 8-bit states, a uint8 ``[ceil(numel / 256), 2]`` per
+            parameter.  All states start as zeros.
+        masters: fp32 tensors that 16-bit parameters are the rounding of; the
+            step is taken on them.  Without them a 16-bit parameter is read,
+            moved in fp32 and rounded to nearest, which loses steps smaller
+            than half its spacing.
+        seed: of the random rounding of 8-bit states, which depends on
+            (seed, step, position of the element in the lists) alone.
+
+    8-bit states keep 4 significant bits per element and a power-of-two scale
+    per 256; they are rounded up or down at random in proportion, so that the
+    moving averages keep moving by less than their spacing.  The step itself
+    uses them unrounded.  A value that is not finite makes its block NaN."""
+    params = list(params)
+    lr_tensor = lr if isinstance(lr, torch.Tensor) else None
+    step_tensor = step if isinstance(step, torch.Tensor) else None
+    if not params:
+        return
+    _require_hip("params", params[0])
+    ops.maxsim_adamw_step(
+        params, list(grads), list(exp_avgs), list(exp_avg_sqs), list(scales or ()),
+        list(masters or ()), 0.0 if lr_tensor is not None else lr, lr_tensor, betas[0], betas[1],
+        eps, weight_decay, 1 if step_tensor is not None else step, step_tensor, seed)
+
+
+def adamw_state_values(exp_avg, exp_avg_sq, scales) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What the 8-bit states of a parameter stand for: the first and second
+    moment in bf16, which holds them exactly."""
+    _require_hip("exp_avg", exp_avg)
+    return ops.maxsim_adamw_state_values(exp_avg, exp_avg_sq, scales)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW on :func:`adamw_step`: every parameter of a group in a few
+    launches, states in 32 or 8 bits.
+
+    Args:
+        params, lr, betas, eps, weight_decay: as ``torch.optim.AdamW``; lr may
+            be an fp32 tensor of one element on the parameters' device.
+        state_bits: 32, or 8 for parameters of at least ``min_8bit_size``
+            elements (below it 8 bits save nothing that counts).
+        master_weights: keep an fp32 copy of each 16-bit parameter and step on
+            that (made at the parameter's first step; the parameter itself is
+            then only written).
+        seed: of the random rounding of 8-bit states.
+
+    State of a parameter: ``step`` (an int), ``exp_avg``, ``exp_avg_sq``, and
+    ``scales`` / ``master`` where they apply.  ``state_dict`` round trips keep
+    the states' own dtypes.  The step count lives on the host: a captured graph
+    would replay one step's, so ``step()`` refuses to be captured
+    (:func:`adamw_step` takes it as a tensor)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, min_8bit_size: int = 4096,
+                 master_weights: bool = False, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32; got {state_bits}")
+        if not isinstance(lr, torch.Tensor) and not (lr >= 0.0 and math.isfinite(lr)):
+            raise ValueError(f"lr must be finite and >= 0; got {lr}")
+        for name, value in (("eps", eps), ("weight_decay", weight_decay)):
+            if not (value >= 0.0 and math.isfinite(value)):
+                raise ValueError(f"{name} must be finite and >= 0; got {value}")
+        if not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"betas must be in [0, 1); got {tuple(betas)}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
+                                      weight_decay=weight_decay, state_bits=state_bits,
+                                      min_8bit_size=min_8bit_size,
+                                      master_weights=master_weights, seed=seed))
+
+    def _new_state(self, p, group) -> dict:
+        eight = group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]
+        dtype = torch.uint8 if eight else torch.float32
+        state = {"step": 0, "exp_avg": torch.zeros_like(p, dtype=dtype),
+                 "exp_avg_sq": torch.zeros_like(p, dtype=dtype)}
+        if eight:
+            blocks = (p.numel() + STATE_BLOCK - 1) // STATE_BLOCK
+            state["scales"] = torch.zeros(blocks, 2, dtype=torch.uint8, device=p.device)
+        if group["master_weights"] and p.dtype != torch.float32:
+            state["master"] = p.detach().to(torch.float32)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """Step every parameter that has a gradient; returns the closure's loss."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step() counts its steps on the host and cannot be captured; "
+                               "use adamw_step with a step tensor")
+        for at, group in enumerate(self.param_groups):
+            # one call per device, step count and kind of state
+            calls: dict = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not support sparse gradients")
+                state = self.state[p]
+                if not state:
+                    state.update(self._new_state(p, group))
+                key = (p.device, state["step"], "scales" in state, "master" in state)
+                calls.setdefault(key, []).append((p, state))
+            for (_, step, eight, master), found in calls.items():
+                states = [s for _, s in found]
+                adamw_step([p for p, _ in found], [p.grad for p, _ in found],
+                           [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+                           step=step + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                           weight_decay=group["weight_decay"],
+                           scales=[s["scales"] for s in states] if eight else None,
+                           masters=[s["master"] for s in states] if master else None,
+                           seed=group["seed"] + at)
+                for s in states:
+                    s["step"] = step + 1
+        return loss
+
+    def load_state_dict(self, state_dict) -> None:
+        """As torch's, which casts a state to its parameter's dtype; here each
+        keeps its own (8-bit codes, fp32 moments and masters)."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, params):
+            for name, value in state_dict["state"].get(i, {}).items():
+                if isinstance(value, torch.Tensor):
+                    value = value.to(device=p.device, copy=True)
+                self.state[p][name] = value
