@@ -32,27 +32,29 @@
 namespace maxsim {
 
 constexpr int kAdamThreads = 256;
-constexpr int kLaneElems = 8;  // elements of a lane at a time: 32 lanes are a block
+constexpr int kLaneElems = 8;  // elements of a lane: 32 lanes are a block
 constexpr int kBlock = MAXSIM_AMD_STATE_BLOCK;
 static_assert(kBlock == 32 * kLaneElems, "half a wave holds a block");
-constexpr int kTurns = 2;  // blocks of a lane per workgroup
-constexpr int kChunkElems = kAdamThreads * kLaneElems * kTurns;
-constexpr int kTensors = 48;  // of one launch: 3.5 KB of its 4 KB of arguments
+// One turn per workgroup: with two (and their loads together) the registers
+// halve the waves, 384 against 364 us for 66 M fp32 parameters.
+constexpr int kChunkElems = kAdamThreads * kLaneElems;
+constexpr int64_t kMaxElems = (int64_t)1 << 40;  // of a step: 32-bit block numbers
+constexpr int64_t kMaxChunks = UINT32_MAX / kAdamThreads;  // of a launch: threads in 32 bits
 
-struct AdamTensor {
-  void* p;
-  const void* g;
-  void* m;
-  void* v;
-  uint8_t* scales;
-  float* master;
-  int64_t n;
-  uint64_t position;  // of element 0, for the random bits
-};
-
-struct AdamArgs {
-  AdamTensor t[kTensors];
-  uint32_t first[kTensors + 1];  // chunk numbers
+// The tensors of a launch, as many as 4 KB of kernel arguments hold (88 in
+// the plain 32-bit step, 61 with 8-bit states and masters).
+template <int BITS, bool MASTER> struct AdamArgs {
+  static constexpr int kTensors =
+      (4096 - 128) / (5 * 8 + 4 + (BITS == 8 ? 8 + 4 : 0) + (MASTER ? 8 : 0));
+  void* p[kTensors];
+  const void* g[kTensors];
+  void* m[kTensors];
+  void* v[kTensors];
+  int64_t n[kTensors];
+  uint8_t* scales[BITS == 8 ? kTensors : 1];
+  float* master[MASTER ? kTensors : 1];
+  uint32_t block[BITS == 8 ? kTensors : 1];  // position of element 0, in blocks
+  uint32_t first[kTensors];                  // chunk number of element 0
   int count;
   float lr, decay, b1, r1, b2, r2, eps;  // r: 1 - b
   float c1, c2;                          // 1 - b^t
@@ -63,11 +65,16 @@ struct AdamArgs {
   double beta1, beta2;
   uint64_t seed;
 };
-static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
+static_assert(sizeof(AdamArgs<32, false>) <= 4096 && sizeof(AdamArgs<32, true>) <= 4096 &&
+                  sizeof(AdamArgs<8, false>) <= 4096 && sizeof(AdamArgs<8, true>) <= 4096,
+              "kernel arguments");
 
 __host__ __device__ inline uint32_t dither_key(uint64_t seed, uint64_t step) {
   return (uint32_t)seed * 0x9e3779b1u + (uint32_t)step * 0x3c6ef373u;
 }
+
+constexpr uint32_t kDitherStep = 0x9e3779b1u;
+constexpr uint32_t kNan = 0x7fc00000u;
 
 // 32 random bits of one element: multiplications by odd constants (from the
 // golden ratio and the roots of 2, 3, 5 and 7) between shifts that bring the
@@ -85,31 +92,36 @@ template <bool SIGNED> struct Code {
   static constexpr int lowest = SIGNED ? 32 : 48;  // E below this count as it
 };
 
-__device__ __forceinline__ float pow2f(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
+// The exponent that moves codes to values (and, negated, back): E - top.
+template <bool SIGNED>
+__device__ __forceinline__ int code_shift(int e) {
+  return min(max(e, Code<SIGNED>::lowest), 254) - Code<SIGNED>::top;
+}
 
-// Both directions go by two exact factors, of which 2^126 has no place in one
-// (E - top spans more than fp32's exponents).
+// Byte k of a word of four codes; nan: a NaN's bits where the block stands for
+// NaN, else 0.  The low codes are subnormal as fp32 patterns, and exact.
 template <bool SIGNED>
-__device__ __forceinline__ float decode_factor(int e) {
-  return e == 255 ? NAN : pow2f(min(max(e, Code<SIGNED>::lowest), 254) - Code<SIGNED>::top - 126);
+__device__ __forceinline__ float decode(uint32_t word, int k, int shift, uint32_t nan) {
+  const uint32_t code = word >> (8 * k);
+  const float x =
+      __builtin_amdgcn_ldexpf(__uint_as_float((code & (SIGNED ? 127u : 255u)) << 20 | nan), shift);
+  return SIGNED ? __uint_as_float(__float_as_uint(x) | (code & 128u) << 24) : x;
 }
+// The code of x in the top byte.
 template <bool SIGNED>
-__device__ __forceinline__ float decode(uint32_t code, float factor) {
-  const float u = __uint_as_float((SIGNED ? code & 127u : code) << 20);
-  const float x = u * 0x1p126f * factor;
-  return SIGNED && (code & 128u) ? -x : x;
+__device__ __forceinline__ uint32_t encode(float x, int shift, uint32_t dither20) {
+  const float u = __builtin_amdgcn_ldexpf(fabsf(x), -shift);
+  const uint32_t q = (__float_as_uint(u) + dither20) << 4;
+  if constexpr (SIGNED) return (q & 0x7fffffffu) | (__float_as_uint(x) & 0x80000000u);
+  else return max(q, min(__float_as_uint(x), 1u) << 24);
 }
-template <bool SIGNED>
-__device__ __forceinline__ float encode_factor(int e) {
-  return pow2f(Code<SIGNED>::top + 126 - min(max(e, Code<SIGNED>::lowest), 254));
-}
-template <bool SIGNED>
-__device__ __forceinline__ uint32_t encode(float x, float factor, uint32_t dither20) {
-  const float u = fabsf(x) * factor * 0x1p-126f;
-  uint32_t q = (__float_as_uint(u) + dither20) >> 20;
-  if constexpr (SIGNED) q |= (__float_as_uint(x) >> 31) << 7;
-  else if (q == 0 && x > 0.0f) q = 1;
-  return q;
+
+// sqrt by the hardware's instruction (1 ulp), whose operand must not be
+// subnormal: small ones are moved by an even power of two.
+__device__ __forceinline__ float root_of(float v) {
+  const bool small = v < 0x1p-96f;
+  const float r = __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v);
+  return small ? r * 0x1p-32f : r;
 }
 
 // Largest over the 32 lanes of a half wave, in each of them.
@@ -187,103 +199,105 @@ __device__ __forceinline__ void store_codes(void* p, int64_t i, int64_t n, uint2
   }
 }
 
+// The top bytes of eight words, in order.
+__device__ __forceinline__ uint2 top_bytes(const uint32_t (&q)[8]) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    // v_perm_b32 takes bytes 0-3 from its second operand, 4-7 from its first
+    const uint32_t lo = __builtin_amdgcn_perm(q[4 * i + 1], q[4 * i], 0x0c0c0703u);
+    const uint32_t hi = __builtin_amdgcn_perm(q[4 * i + 3], q[4 * i + 2], 0x07030c0cu);
+    w[i] = lo | hi;
+  }
+  return make_uint2(w[0], w[1]);
+}
+
 struct AdamStep {
-  float keep, size, root;  // 1 - lr decay, lr / c1, sqrt(c2)
+  float keep, size, root;  // 1 - lr decay, lr / c1, 1 / sqrt(c2)
   uint32_t key;
 };
 
-// The states of each turn are loaded before any of them is used.
+// Tensor k's elements from base on.  The quotient is a product with the
+// hardware's reciprocal (1 ulp): the update is off by a few 1e-7 of itself,
+// and exact roots and quotients made the step bound by arithmetic (bf16 with
+// 8-bit states, 66 M parameters: 190 us against 155).
 template <typename P, typename Gr, int BITS, bool MASTER, bool FULL>
-__device__ __forceinline__ void adam_chunk(const AdamArgs& a, const AdamTensor& t,
+__device__ __forceinline__ void adam_chunk(const AdamArgs<BITS, MASTER>& a, int k,
                                            const AdamStep& h, int64_t base) {
 #pragma clang fp contract(off)
-  const int64_t n = t.n;
-  float p[kTurns][8], g[kTurns][8], m[kTurns][8], v[kTurns][8];
-  uint2 mc[kTurns], vc[kTurns];
-  uint16_t sc[kTurns];
-#pragma unroll
-  for (int u = 0; u < kTurns; ++u) {
-    const int64_t i = base + (int64_t)(u * kAdamThreads + threadIdx.x) * kLaneElems;
-    load8<Gr, FULL>(t.g, i, n, g[u]);
-    if constexpr (MASTER) load8<F32, FULL>(t.master, i, n, p[u]);
-    else load8<P, FULL>(t.p, i, n, p[u]);
-    if constexpr (BITS == 8) {
-      mc[u] = load_codes<FULL>(t.m, i, n);
-      vc[u] = load_codes<FULL>(t.v, i, n);
-      sc[u] = 0;
-      if (FULL || i < n) __builtin_memcpy(&sc[u], t.scales + 2 * (i / kBlock), 2);
-    } else {
-      load8<F32, FULL>(t.m, i, n, m[u]);
-      load8<F32, FULL>(t.v, i, n, v[u]);
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < kTurns; ++u) {
-    const int64_t i = base + (int64_t)(u * kAdamThreads + threadIdx.x) * kLaneElems;
-    if constexpr (BITS == 8) {
-      const float fm = decode_factor<true>(sc[u] & 255), fv = decode_factor<false>(sc[u] >> 8);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        m[u][e] = decode<true>((e < 4 ? mc[u].x : mc[u].y) >> (8 * (e & 3)) & 255u, fm);
-        v[u][e] = decode<false>((e < 4 ? vc[u].x : vc[u].y) >> (8 * (e & 3)) & 255u, fv);
-      }
-    }
-    uint32_t big_m = 0, big_v = 0;
+  const int64_t n = a.n[k];
+  const int64_t i = base + threadIdx.x * kLaneElems;
+  float p[8], g[8], m[8], v[8];
+  load8<Gr, FULL>(a.g[k], i, n, g);
+  if constexpr (MASTER) load8<F32, FULL>(a.master[k], i, n, p);
+  else load8<P, FULL>(a.p[k], i, n, p);
+  if constexpr (BITS == 8) {
+    const uint2 mc = load_codes<FULL>(a.m[k], i, n), vc = load_codes<FULL>(a.v[k], i, n);
+    uint16_t s = 0;
+    if (FULL || i < n) __builtin_memcpy(&s, a.scales[k] + 2 * (i / kBlock), 2);
+    const int em = s & 255, ev = s >> 8;
+    const uint32_t nm = em == 255 ? kNan : 0, nv = ev == 255 ? kNan : 0;
+    const int fm = code_shift<true>(em), fv = code_shift<false>(ev);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float ge = g[u][e];
-      // unfused, each product rounded: what the 8-bit codes are taken from
-      // must not depend on how a compiler contracts
-      m[u][e] = m[u][e] * a.b1 + ge * a.r1;
-      v[u][e] = v[u][e] * a.b2 + (ge * ge) * a.r2;
-      const float d = sqrtf(v[u][e]) / h.root + a.eps;
-      p[u][e] = p[u][e] * h.keep - h.size * (m[u][e] / d);
-      big_m = max(big_m, __float_as_uint(m[u][e]) & 0x7fffffffu);
-      big_v = max(big_v, __float_as_uint(v[u][e]) & 0x7fffffffu);
+      m[e] = decode<true>(e < 4 ? mc.x : mc.y, e & 3, fm, nm);
+      v[e] = decode<false>(e < 4 ? vc.x : vc.y, e & 3, fv, nv);
     }
-    store8<P, FULL>(t.p, i, n, p[u]);
-    if constexpr (MASTER) store8<F32, FULL>(t.master, i, n, p[u]);
-    if constexpr (BITS == 8) {
-      const int em = max((int)(half_max(big_m) >> 23), Code<true>::lowest);
-      const int ev = max((int)(half_max(big_v) >> 23), Code<false>::lowest);
-      const float fm = encode_factor<true>(em), fv = encode_factor<false>(ev);
-      const uint64_t at = t.position + (uint64_t)i;
-      const uint32_t x0 =
-          (uint32_t)at * 0x9e3779b1u + (uint32_t)(at >> 32) * 0xa54ff53bu + h.key;
-      uint2 qm = make_uint2(0, 0), qv = make_uint2(0, 0);
+  } else {
+    load8<F32, FULL>(a.m[k], i, n, m);
+    load8<F32, FULL>(a.v[k], i, n, v);
+  }
+  uint32_t big_m = 0, big_v = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        // positions of a lane's eight elements differ in the low word alone
-        const uint32_t r = dither_bits(x0 + (uint32_t)e * 0x9e3779b1u);
-        const uint32_t cm =
-            em == 255 ? 0 : encode<true>(m[u][e], fm, (r & 0xffffu) * 16 + 8);
-        const uint32_t cv = ev == 255 ? 0 : encode<false>(v[u][e], fv, (r >> 16) * 16 + 8);
-        (e < 4 ? qm.x : qm.y) |= cm << (8 * (e & 3));
-        (e < 4 ? qv.x : qv.y) |= cv << (8 * (e & 3));
-      }
-      store_codes<FULL>(t.m, i, n, qm);
-      store_codes<FULL>(t.v, i, n, qv);
-      if ((threadIdx.x & 31) == 0 && (FULL || i < n)) {
-        const uint16_t s = (uint16_t)(em | ev << 8);
-        __builtin_memcpy(t.scales + 2 * (i / kBlock), &s, 2);
-      }
-    } else {
-      store8<F32, FULL>(t.m, i, n, m[u]);
-      store8<F32, FULL>(t.v, i, n, v[u]);
+  for (int e = 0; e < 8; ++e) {
+    // unfused, each product rounded: what the 8-bit codes are taken from must
+    // not depend on how a compiler contracts
+    m[e] = m[e] * a.b1 + g[e] * a.r1;
+    v[e] = v[e] * a.b2 + (g[e] * g[e]) * a.r2;
+    const float d = root_of(v[e]) * h.root + a.eps;
+    p[e] = p[e] * h.keep - h.size * (m[e] * __builtin_amdgcn_rcpf(d));
+    big_m = max(big_m, __float_as_uint(m[e]) & 0x7fffffffu);
+    big_v = max(big_v, __float_as_uint(v[e]) & 0x7fffffffu);
+  }
+  store8<P, FULL>(a.p[k], i, n, p);
+  if constexpr (MASTER) store8<F32, FULL>(a.master[k], i, n, p);
+  if constexpr (BITS == 8) {
+    const int em = max((int)(half_max(big_m) >> 23), Code<true>::lowest);
+    const int ev = max((int)(half_max(big_v) >> 23), Code<false>::lowest);
+    const int fm = code_shift<true>(em), fv = code_shift<false>(ev);
+    const uint64_t at = (uint64_t)a.block[k] * kBlock + (uint64_t)i;
+    const uint32_t x0 = (uint32_t)at * kDitherStep + (uint32_t)(at >> 32) * 0xa54ff53bu + h.key;
+    uint32_t qm[8], qv[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // positions of a lane's eight elements differ in the low word alone
+      const uint32_t r = dither_bits(x0 + (uint32_t)e * kDitherStep);
+      qm[e] = encode<true>(m[e], fm, (r & 0xffffu) * 16 + 8);
+      qv[e] = encode<false>(v[e], fv, (r >> 16) * 16 + 8);
     }
+    const uint2 none = make_uint2(0, 0);
+    store_codes<FULL>(a.m[k], i, n, em == 255 ? none : top_bytes(qm));
+    store_codes<FULL>(a.v[k], i, n, ev == 255 ? none : top_bytes(qv));
+    if ((threadIdx.x & 31) == 0 && (FULL || i < n)) {
+      const uint16_t s = (uint16_t)(em | ev << 8);
+      __builtin_memcpy(a.scales[k] + 2 * (i / kBlock), &s, 2);
+    }
+  } else {
+    store8<F32, FULL>(a.m[k], i, n, m);
+    store8<F32, FULL>(a.v[k], i, n, v);
   }
 }
 
 template <typename P, typename Gr, int BITS, bool MASTER>
-__global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs a) {
+__global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs<BITS, MASTER> a) {
+  // the last tensor that starts at or before this chunk: one load per wave
+  // instead of a chain of them
   const uint32_t chunk = blockIdx.x;
-  int lo = 0, hi = a.count;  // first[lo] <= chunk < first[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (a.first[mid] <= chunk) lo = mid;
-    else hi = mid;
-  }
-  const AdamTensor& t = a.t[lo];
+  const int lane = threadIdx.x & 63;
+  int k = -1;
+#pragma unroll
+  for (int i = 0; i < AdamArgs<BITS, MASTER>::kTensors; i += 64)
+    k += __popcll(__ballot(i + lane < a.count && a.first[min(i + lane, a.count - 1)] <= chunk));
   float lr = a.lr, c1 = a.c1, c2 = a.c2;
   uint32_t key = a.key;
   if (a.lr_at) lr = *a.lr_at;
@@ -296,10 +310,10 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs a) {
     c1 = c[0], c2 = c[1];
     key = dither_key(a.seed, (uint64_t)step);
   }
-  const AdamStep h{1.0f - lr * a.decay, lr / c1, sqrtf(c2), key};
-  const int64_t base = (int64_t)(chunk - a.first[lo]) * kChunkElems;
-  if (base + kChunkElems <= t.n) adam_chunk<P, Gr, BITS, MASTER, true>(a, t, h, base);
-  else adam_chunk<P, Gr, BITS, MASTER, false>(a, t, h, base);
+  const AdamStep h{1.0f - lr * a.decay, lr / c1, 1.0f / sqrtf(c2), key};
+  const int64_t base = (int64_t)(chunk - a.first[k]) * kChunkElems;
+  if (base + kChunkElems <= a.n[k]) adam_chunk<P, Gr, BITS, MASTER, true>(a, k, h, base);
+  else adam_chunk<P, Gr, BITS, MASTER, false>(a, k, h, base);
 }
 
 // The values of 8-bit states in bf16, which holds their 4 significant bits.
@@ -312,12 +326,14 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_values_kernel(
   uint16_t s;
   __builtin_memcpy(&s, scales + 2 * (i / kBlock), 2);
   const uint2 mc = load_codes<false>(m, i, n), vc = load_codes<false>(v, i, n);
-  const float fm = decode_factor<true>(s & 255), fv = decode_factor<false>(s >> 8);
+  const int em = s & 255, ev = s >> 8;
+  const uint32_t nm = em == 255 ? kNan : 0, nv = ev == 255 ? kNan : 0;
+  const int fm = code_shift<true>(em), fv = code_shift<false>(ev);
   float x[8], y[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    x[e] = decode<true>((e < 4 ? mc.x : mc.y) >> (8 * (e & 3)) & 255u, fm);
-    y[e] = decode<false>((e < 4 ? vc.x : vc.y) >> (8 * (e & 3)) & 255u, fv);
+    x[e] = decode<true>(e < 4 ? mc.x : mc.y, e & 3, fm, nm);
+    y[e] = decode<false>(e < 4 ? vc.x : vc.y, e & 3, fv, nv);
   }
   store8<BF16, false>(out_m, i, n, x);
   store8<BF16, false>(out_v, i, n, y);
@@ -356,62 +372,65 @@ int maxsim_amd_adamw_step(maxsim_dtype param_dtype, maxsim_dtype grad_dtype, int
     if (t.numel > 0 &&
         (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || (state_bits == 8 && !t.scales)))
       return fail(MAXSIM_ERR_INVALID, "null pointer argument");
-    if (t.numel / kChunkElems >= UINT32_MAX / (2 * kAdamThreads))
+    if ((t.numel + kChunkElems - 1) / kChunkElems > kMaxChunks)
       return fail(MAXSIM_ERR_UNSUPPORTED, "tensor too large for one launch");
+    if (state_bits == 8 && (t.position % kBlock != 0 || t.position >= (uint64_t)kMaxElems))
+      return fail(MAXSIM_ERR_INVALID, "position must be a multiple of 256 below 2^40");
   }
   if (master && param_dtype == MAXSIM_FLOAT32)
     return fail(MAXSIM_ERR_INVALID, "float32 parameters have no master");
 
-  AdamArgs a{};
-  a.lr = (float)lr;
-  a.decay = (float)weight_decay;
-  a.b1 = (float)beta1, a.r1 = (float)(1.0 - beta1);
-  a.b2 = (float)beta2, a.r2 = (float)(1.0 - beta2);
-  a.eps = (float)eps;
-  a.c1 = (float)(1.0 - std::pow(beta1, (double)step));
-  a.c2 = (float)(1.0 - std::pow(beta2, (double)step));
-  a.key = dither_key(seed, (uint64_t)step);
-  a.lr_at = lr_on_device, a.step_at = step_on_device;
-  a.beta1 = beta1, a.beta2 = beta2, a.seed = seed;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  auto launch = [&] {
-    const unsigned blocks = a.first[a.count];
-    auto go = [&](auto p, auto g, auto bits, auto mst) {
-      hipLaunchKernelGGL(
-          (adamw_kernel<decltype(p), decltype(g), decltype(bits)::value, decltype(mst)::value>),
-          dim3(blocks), dim3(kAdamThreads), 0, st, a);
+  auto run = [&](auto p, auto g, auto bits, auto with_master) -> int {
+    constexpr int BITS = decltype(bits)::value;
+    constexpr bool MASTER = decltype(with_master)::value;
+    using Args = AdamArgs<BITS, MASTER>;
+    Args a{};
+    a.lr = (float)lr;
+    a.decay = (float)weight_decay;
+    a.b1 = (float)beta1, a.r1 = (float)(1.0 - beta1);
+    a.b2 = (float)beta2, a.r2 = (float)(1.0 - beta2);
+    a.eps = (float)eps;
+    a.c1 = (float)(1.0 - std::pow(beta1, (double)step));
+    a.c2 = (float)(1.0 - std::pow(beta2, (double)step));
+    a.key = dither_key(seed, (uint64_t)step);
+    a.lr_at = lr_on_device, a.step_at = step_on_device;
+    a.beta1 = beta1, a.beta2 = beta2, a.seed = seed;
+    uint32_t chunks = 0;
+    auto launch = [&] {
+      hipLaunchKernelGGL((adamw_kernel<decltype(p), decltype(g), BITS, MASTER>), dim3(chunks),
+                         dim3(kAdamThreads), 0, static_cast<hipStream_t>(stream), a);
+      a.count = 0, chunks = 0;
+      return check_launch("adamw_kernel");
     };
-    auto bits = [&](auto p, auto g, auto mst) {
-      if (state_bits == 8) go(p, g, std::integral_constant<int, 8>{}, mst);
-      else go(p, g, std::integral_constant<int, 32>{}, mst);
-    };
-    auto sixteen = [&](auto p) {
-      auto grad = [&](auto g) {
-        if (master) bits(p, g, std::true_type{});
-        else bits(p, g, std::false_type{});
-      };
-      if (grad_dtype == MAXSIM_FLOAT32) grad(F32{});
-      else grad(p);
-    };
-    if (param_dtype == MAXSIM_FLOAT32) bits(F32{}, F32{}, std::false_type{});
-    else if (param_dtype == MAXSIM_FLOAT16) sixteen(F16{});
-    else sixteen(BF16{});
-    a.count = 0;
-    return check_launch("adamw_kernel");
+    for (int64_t i = 0; i < count; ++i) {
+      const maxsim_adamw_tensor& t = tensors[i];
+      if (t.numel == 0) continue;
+      const uint32_t more = (uint32_t)((t.numel + kChunkElems - 1) / kChunkElems);
+      if (a.count == Args::kTensors || (uint64_t)chunks + more > kMaxChunks)
+        if (int e = launch()) return e;
+      const int k = a.count++;
+      a.p[k] = t.param, a.g[k] = t.grad, a.m[k] = t.exp_avg, a.v[k] = t.exp_avg_sq;
+      a.n[k] = t.numel, a.first[k] = chunks;
+      if constexpr (BITS == 8) {
+        a.scales[k] = t.scales;
+        a.block[k] = (uint32_t)(t.position / kBlock);
+      }
+      if constexpr (MASTER) a.master[k] = t.master;
+      chunks += more;
+    }
+    return a.count > 0 ? launch() : MAXSIM_OK;
   };
-  for (int64_t i = 0; i < count; ++i) {
-    const maxsim_adamw_tensor& t = tensors[i];
-    if (t.numel == 0) continue;
-    const uint32_t chunks = (uint32_t)((t.numel + kChunkElems - 1) / kChunkElems);
-    if (a.count == kTensors ||
-        (a.count > 0 && (uint64_t)a.first[a.count] + chunks > UINT32_MAX / kAdamThreads))
-      if (int e = launch()) return e;
-    a.t[a.count] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.scales, t.master, t.numel,
-                    t.position};
-    a.first[a.count + 1] = a.first[a.count] + chunks;
-    ++a.count;
-  }
-  return a.count > 0 ? launch() : MAXSIM_OK;
+  auto with_bits = [&](auto p, auto g, auto with_master) {
+    return state_bits == 8 ? run(p, g, std::integral_constant<int, 8>{}, with_master)
+                           : run(p, g, std::integral_constant<int, 32>{}, with_master);
+  };
+  auto with_grad = [&](auto p, auto g) {
+    return master ? with_bits(p, g, std::true_type{}) : with_bits(p, g, std::false_type{});
+  };
+  if (param_dtype == MAXSIM_FLOAT32) return with_bits(F32{}, F32{}, std::false_type{});
+  if (param_dtype == MAXSIM_FLOAT16)
+    return grad_dtype == MAXSIM_FLOAT32 ? with_grad(F16{}, F32{}) : with_grad(F16{}, F16{});
+  return grad_dtype == MAXSIM_FLOAT32 ? with_grad(BF16{}, F32{}) : with_grad(BF16{}, BF16{});
 }
 
 int maxsim_amd_adamw_state_values(const uint8_t* exp_avg, const uint8_t* exp_avg_sq,
@@ -423,7 +442,7 @@ int maxsim_amd_adamw_state_values(const uint8_t* exp_avg, const uint8_t* exp_avg
   if (!exp_avg || !exp_avg_sq || !scales || !values || !values_sq)
     return fail(MAXSIM_ERR_INVALID, "null pointer argument");
   const int64_t blocks = (numel + kAdamThreads * kLaneElems - 1) / (kAdamThreads * kLaneElems);
-  if (blocks > UINT32_MAX / kAdamThreads)
+  if (blocks > kMaxChunks)
     return fail(MAXSIM_ERR_UNSUPPORTED, "tensor too large for one launch");
   hipLaunchKernelGGL(adamw_values_kernel, dim3((unsigned)blocks), dim3(kAdamThreads), 0,
                      static_cast<hipStream_t>(stream), exp_avg, exp_avg_sq, scales, numel,
