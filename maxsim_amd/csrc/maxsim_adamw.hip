@@ -147,7 +147,7 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, int64_t n, float
 #pragma unroll
     for (int c = 0; c < 8 / v; ++c) {
       float part[v];
-      unpack16<T>(load16_any(s + c * v), part);
+      unpack<T, v>(load_any<Chunk<T>>(s + c * v), part);
 #pragma unroll
       for (int e = 0; e < v; ++e) f[c * v + e] = part[e];
     }
@@ -166,7 +166,7 @@ __device__ __forceinline__ void store8(void* p, int64_t i, int64_t n, const floa
       float part[v];
 #pragma unroll
       for (int e = 0; e < v; ++e) part[e] = f[c * v + e];
-      store16_any(s + c * v, pack16<T>(part));
+      store_any(s + c * v, pack<T, v>(part));
     }
   } else {
 #pragma unroll

@@ -43,13 +43,14 @@ __global__ __launch_bounds__(row_threads(G)) void ln_forward_kernel(LnForward a)
   const S* x = static_cast<const S*>(a.x);
   S* y = static_cast<S*>(a.y);
   const float inv_dim = 1.0f / (float)dim;
+  const bool whole = dim == G * K * V;
 
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   int64_t row = (int64_t)blockIdx.x * GROUPS + group;
-  uint4 next[K] = {};
+  Chunk<T> next[K] = {};
   if (row < a.rows) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) next[k] = load_chunk<T>(x + row * a.stride, (j + k * G) * V, dim);
+    for (int k = 0; k < K; ++k) next[k] = load_chunk<T, V, takes_short(G)>(x + row * a.stride, (j + k * G) * V, dim);
   }
   float w[K][V], b[K][V];
 #pragma unroll
@@ -61,11 +62,14 @@ __global__ __launch_bounds__(row_threads(G)) void ln_forward_kernel(LnForward a)
   for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < a.rows; base += step, row += step) {
     float f[K][V];
 #pragma unroll
-    for (int k = 0; k < K; ++k) unpack16<T>(next[k], f[k]);
+    for (int k = 0; k < K; ++k) {
+      if (!whole) place_chunk<T, V, takes_short(G)>(next[k], (j + k * G) * V, dim);
+      unpack<T, V>(next[k], f[k]);
+    }
     if (row + step < a.rows) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        next[k] = load_chunk<T>(x + (row + step) * a.stride, (j + k * G) * V, dim);
+        next[k] = load_chunk<T, V, takes_short(G)>(x + (row + step) * a.stride, (j + k * G) * V, dim);
     }
     float sum[1] = {0.0f};
 #pragma unroll
@@ -89,7 +93,7 @@ __global__ __launch_bounds__(row_threads(G)) void ln_forward_kernel(LnForward a)
       for (int k = 0; k < K; ++k) {
 #pragma unroll
         for (int e = 0; e < V; ++e) f[k][e] = f[k][e] * rstd * w[k][e] + b[k][e];
-        store_chunk<T>(y + row * dim, (j + k * G) * V, dim, f[k]);
+        store_chunk<T, V>(y + row * dim, (j + k * G) * V, dim, f[k]);
       }
       if (a.mean && j == 0) {
         a.mean[row] = mean;
@@ -111,13 +115,17 @@ struct LnBackward {
   float* partial;  // [gridDim.x][2][dim] sums of dy xh and dy; NULL: not wanted
 };
 
+// Four elements per chunk in either type: a lane of the backward holds five
+// arrays of its columns (x, dy, the weights and the two sums).
+constexpr int kBackwardVec = 4;
+
 // The rows in turn as in the forward; each lane adds up its columns' share of
 // dw and db over its rows, the workgroup joins its groups' (in one order) and
 // writes one partial row, which ln_weight_grad_kernel adds up.
 template <typename T, typename W, int G, int K>
 __global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward a) {
   using S = typename T::storage;
-  constexpr int V = kVec<T>, GROUPS = row_threads(G) / G;
+  constexpr int V = kBackwardVec, GROUPS = row_threads(G) / G;
   constexpr int COLS = G * K * V;
   // two chunks per lane of 1024 threads leave no registers for the next row
   // and the weights (128 per lane): both are loaded where they are used
@@ -130,16 +138,17 @@ __global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward 
   const S* dy = static_cast<const S*>(a.dy);
   S* dx = static_cast<S*>(a.dx);
   const float inv_dim = 1.0f / (float)dim;
+  const bool whole = dim == G * K * V;
 
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   int64_t row = (int64_t)blockIdx.x * GROUPS + group;
-  uint4 next_x[K] = {}, next_d[K] = {};
+  Chunk<T, V> next_x[K] = {}, next_d[K] = {};
   float next_mean = 0.0f, next_rstd = 0.0f;
   auto load = [&](int64_t r) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      next_x[k] = load_chunk<T>(x + r * a.x_stride, (j + k * G) * V, dim);
-      next_d[k] = load_chunk<T>(dy + r * a.dy_stride, (j + k * G) * V, dim);
+      next_x[k] = load_chunk<T, V, takes_short(G)>(x + r * a.x_stride, (j + k * G) * V, dim);
+      next_d[k] = load_chunk<T, V, takes_short(G)>(dy + r * a.dy_stride, (j + k * G) * V, dim);
     }
     next_mean = a.mean[r];
     next_rstd = a.rstd[r];
@@ -162,8 +171,12 @@ __global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward 
     const float mean = next_mean, rstd = next_rstd;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      unpack16<T>(next_x[k], f[k]);
-      unpack16<T>(next_d[k], d[k]);
+      if (!whole) {
+        place_chunk<T, V, takes_short(G)>(next_x[k], (j + k * G) * V, dim);
+        place_chunk<T, V, takes_short(G)>(next_d[k], (j + k * G) * V, dim);
+      }
+      unpack<T, V>(next_x[k], f[k]);
+      unpack<T, V>(next_d[k], d[k]);
     }
     const bool here = row < a.rows;
     if (AHEAD && row + step < a.rows) load(row + step);
@@ -194,7 +207,7 @@ __global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward 
         for (int k = 0; k < K; ++k) {
 #pragma unroll
           for (int e = 0; e < V; ++e) f[k][e] = rstd * (d[k][e] - c1 - f[k][e] * c2);
-          store_chunk<T>(dx + row * dim, (j + k * G) * V, dim, f[k]);
+          store_chunk<T, V>(dx + row * dim, (j + k * G) * V, dim, f[k]);
         }
       }
     }
@@ -236,29 +249,30 @@ __global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward 
   write(db, out + dim);
 }
 
-// dw and db from the partial rows: a workgroup takes 64 columns of one of the
-// two, its 16 waves every sixteenth partial row each, joined in LDS in one
+// dw and db from the partial rows: a workgroup takes 32 columns of one of the
+// two, and each 32 of its threads every 32nd partial row, joined in LDS in one
 // order.
-constexpr int kGradWaves = 16;
+constexpr int kGradCols = 32, kGradSlices = 32;
 template <typename W>
-__global__ __launch_bounds__(64 * kGradWaves) void ln_weight_grad_kernel(
+__global__ __launch_bounds__(kGradCols * kGradSlices) void ln_weight_grad_kernel(
     const float* __restrict__ partial, int count, int dim, void* dweight, void* dbias) {
-  __shared__ float part[kGradWaves][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane, which = blockIdx.y;
+  __shared__ float part[kGradSlices][kGradCols + 1];
+  const int col = threadIdx.x % kGradCols, slice = threadIdx.x / kGradCols;
+  const int c = blockIdx.x * kGradCols + col, which = blockIdx.y;
   float s = 0.0f;
   if (c < dim) {
     const float* p = partial + (int64_t)which * dim + c;
 #pragma unroll 8
-    for (int i = wave; i < count; i += kGradWaves) s += p[(int64_t)i * 2 * dim];
+    for (int i = slice; i < count; i += kGradSlices) s += p[(int64_t)i * 2 * dim];
   }
-  part[wave][lane] = s;
+  part[slice][col] = s;
   __syncthreads();
-  if (wave != 0 || c >= dim) return;
-#pragma unroll
-  for (int w = 1; w < kGradWaves; ++w) s += part[w][lane];
+  // a wave takes two columns: each half adds one's 32 slices
+  const int row = threadIdx.x & 31, column = threadIdx.x >> 5;
+  s = lanes_sum<32>(part[row][column]);
+  const int at = blockIdx.x * kGradCols + column;
   auto* out = static_cast<typename W::storage*>(which ? dbias : dweight);
-  if (out) out[c] = from_float<W>(s);
+  if (row == 0 && at < dim && out) out[at] = from_float<W>(s);
 }
 
 template <typename F>
@@ -280,16 +294,33 @@ static int check_layer_norm(maxsim_dtype dtype, maxsim_dtype weight_dtype, int64
   return check_dim(dim);
 }
 
-// Workgroups of the backward: at most four per CU, and at least eight passes
-// each where there are rows for that, since every workgroup costs a partial
-// row of 8 dim bytes, written and read again.
-static int64_t backward_blocks(maxsim_dtype dtype, int64_t rows, int64_t dim) {
-  int groups = 1;
-  auto take = [&](auto s) { groups = row_threads(s.G) / s.G; };
-  if (dtype == MAXSIM_FLOAT32) with_shape<F32>(dim, take);
-  else with_shape<BF16>(dim, take);
-  const int64_t turns = (rows + groups - 1) / groups;
-  return std::max<int64_t>(1, std::min<int64_t>({turns, 1024, std::max<int64_t>(256, turns / 8)}));
+// Workgroups take their rows in turn, with this turn's and the next's rows
+// asked for; how many there are per CU sets how much is in flight.  Past 32 KB
+// per CU (forward, one array) and 48 KB (backward, two) more only gets into
+// each other's way in the memory: 294912 x 768 bf16 backward 318 / 256 / 273 us
+// with 24 / 48 / 72 KB, 100000 x 768 fp32 161 / 177 us with 48 / 96 KB, 40000 x
+// 2560 bf16 137 / 121 us with 40 / 60 KB.
+constexpr int64_t kForwardInFlight = 32 << 10, kBackwardInFlight = 48 << 10;
+static int workgroups_for(int64_t in_flight, int64_t bytes_each) {
+  return (int)((in_flight + bytes_each - 1) / bytes_each);
+}
+
+// Workgroups of the backward, at most kMaxPartials (what the workspace holds
+// partial rows for) and with at least kLeastTurns turns each where there are
+// more turns than CUs: a workgroup costs a partial row of 8 dim bytes, written
+// and read again.
+constexpr int64_t kMaxPartials = 1024;
+constexpr int64_t kLeastTurns = 4;
+static int64_t backward_blocks(int64_t turns, int64_t cus, int64_t per_cu) {
+  return std::min<int64_t>({turns, cus * per_cu, kMaxPartials,
+                            std::max<int64_t>(cus, turns / kLeastTurns)});
+}
+
+template <typename F>
+static void with_backward(maxsim_dtype dtype, maxsim_dtype weight_dtype, int64_t dim, F&& f) {
+  with_types(dtype, weight_dtype, [&](auto t, auto w) {
+    with_shape<kBackwardVec>(dim, [&](auto s) { f(t, w, s); });
+  });
 }
 
 }  // namespace maxsim
@@ -311,12 +342,20 @@ int maxsim_amd_layer_norm_forward(maxsim_dtype dtype, maxsim_dtype weight_dtype,
   const LnForward a{x, rows, row_stride, (int)dim, weight, bias, eps, y, mean, rstd};
   with_types(dtype, weight_dtype, [&](auto t, auto w) {
     using T = decltype(t);
-    with_shape<T>(dim, [&](auto s) {
+    with_shape<kVec<T>>(dim, [&](auto s) {
       constexpr int G = decltype(s)::G, K = decltype(s)::K, threads = row_threads(G);
-      const int64_t need = (rows + threads / G - 1) / (threads / G);
-      const int64_t blocks = std::min<int64_t>(need, (int64_t)device_cus() * (2048 / threads));
-      hipLaunchKernelGGL((ln_forward_kernel<T, decltype(w), G, K>), dim3((unsigned)blocks),
-                         dim3(threads), 0, static_cast<hipStream_t>(stream), a);
+      const auto kernel = ln_forward_kernel<T, decltype(w), G, K>;
+      static std::atomic<int> resident[kMaxDevices];
+      const int64_t turns = (rows + threads / G - 1) / (threads / G);
+      // rows wider than a wave: two at least, one to run at the other's barriers
+      // (10000 x 8192 bf16: 64 us against 78 with one)
+      const int per_cu = std::min<int>(
+          resident_per_cu(reinterpret_cast<const void*>(kernel), threads, 0, resident),
+          std::max(G > 64 ? 2 : 1,
+                   workgroups_for(kForwardInFlight, 2 * (threads / G) * dim * T::bytes)));
+      const int64_t blocks = std::min<int64_t>(turns, (int64_t)device_cus() * per_cu);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0,
+                         static_cast<hipStream_t>(stream), a);
     });
   });
   return check_launch("ln_forward_kernel");
@@ -325,7 +364,13 @@ int maxsim_amd_layer_norm_forward(maxsim_dtype dtype, maxsim_dtype weight_dtype,
 size_t maxsim_amd_layer_norm_backward_workspace_size(maxsim_dtype dtype, int64_t rows,
                                                      int64_t dim) {
   if (rows <= 0 || dim <= 0 || dim > MAXSIM_AMD_MAX_DIM) return 0;
-  return (size_t)backward_blocks(dtype, rows, dim) * 2 * dim * sizeof(float);
+  int64_t turns = 0;
+  with_shape<kBackwardVec>(dim, [&](auto s) {
+    constexpr int groups = row_threads(decltype(s)::G) / decltype(s)::G;
+    turns = (rows + groups - 1) / groups;
+  });
+  (void)dtype;  // the shapes go by the elements
+  return (size_t)std::min(turns, kMaxPartials) * 2 * dim * sizeof(float);
 }
 
 int maxsim_amd_layer_norm_backward(maxsim_dtype dtype, maxsim_dtype weight_dtype, const void* dy,
@@ -341,30 +386,33 @@ int maxsim_amd_layer_norm_backward(maxsim_dtype dtype, maxsim_dtype weight_dtype
     return fail(MAXSIM_ERR_INVALID, "null pointer argument");
   const bool weights = dweight || dbias;
   if (!dx && !weights) return MAXSIM_OK;
-  const int64_t blocks = rows > 0 ? backward_blocks(dtype, rows, dim) : 0;
   if (weights && rows > 0 &&
-      (!workspace || workspace_bytes < (size_t)blocks * 2 * dim * sizeof(float)))
+      (!workspace ||
+       workspace_bytes < maxsim_amd_layer_norm_backward_workspace_size(dtype, rows, dim)))
     return fail(MAXSIM_ERR_INVALID,
                 "the weights' gradients need a workspace of "
                 "maxsim_amd_layer_norm_backward_workspace_size() bytes");
   float* partial = weights ? static_cast<float*>(workspace) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  int64_t blocks = 0;
   if (rows > 0) {
     const LnBackward a{dy, x, rows, dy_stride, x_stride, (int)dim, mean, rstd, weight, dx, partial};
-    with_types(dtype, weight_dtype, [&](auto t, auto w) {
-      using T = decltype(t);
-      with_shape<T>(dim, [&](auto s) {
-        constexpr int G = decltype(s)::G, K = decltype(s)::K;
-        hipLaunchKernelGGL((ln_backward_kernel<T, decltype(w), G, K>), dim3((unsigned)blocks),
-                           dim3(row_threads(G)), 0, st, a);
-      });
+    with_backward(dtype, weight_dtype, dim, [&](auto t, auto w, auto s) {
+      constexpr int G = decltype(s)::G, threads = row_threads(G);
+      const auto kernel = ln_backward_kernel<decltype(t), decltype(w), G, decltype(s)::K>;
+      static std::atomic<int> resident[kMaxDevices];
+      const int per_cu = std::min<int>(
+          resident_per_cu(reinterpret_cast<const void*>(kernel), threads, 0, resident),
+          workgroups_for(kBackwardInFlight, 4 * (threads / G) * dim * decltype(t)::bytes));
+      blocks = backward_blocks((rows + threads / G - 1) / (threads / G), device_cus(), per_cu);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, st, a);
     });
     if (int e = check_launch("ln_backward_kernel")) return e;
   }
   if (!weights) return MAXSIM_OK;
   with_types(dtype, weight_dtype, [&](auto, auto w) {
-    hipLaunchKernelGGL((ln_weight_grad_kernel<decltype(w)>), dim3((unsigned)((dim + 63) / 64), 2),
-                       dim3(64 * kGradWaves), 0, st, partial, (int)blocks, (int)dim, dweight,
+    hipLaunchKernelGGL((ln_weight_grad_kernel<decltype(w)>), dim3((unsigned)((dim + kGradCols - 1) / kGradCols), 2),
+                       dim3(kGradCols * kGradSlices), 0, st, partial, (int)blocks, (int)dim, dweight,
                        dbias);
   });
   return check_launch("ln_weight_grad_kernel");

@@ -1,12 +1,12 @@
 // Shared device code of the row operators (layer norm, unit rows): a group of
-// G lanes holds one row of `dim` elements in registers, K chunks of 16 bytes
-// per lane, and reduces over the row without leaving the wave (G <= 64) or
+// G lanes holds one row of `dim` elements in registers, K chunks of V elements
+// (8 or 16 bytes) per lane, and reduces over the row without leaving the wave (G <= 64) or
 // through one LDS word per wave (G = 256, 1024).
 //
 // Lane j of a group holds chunks j, j + G, ...: consecutive lanes read
-// consecutive 16 bytes.  Rows may start at any multiple of the element size
-// (load16_any); the row's last chunk is read and written by elements where
-// dim is no multiple of the chunk.
+// consecutive chunks.  Rows may start at any multiple of the element size;
+// the row's last chunk is read and written in pieces where dim is no multiple
+// of the chunk.
 #pragma once
 
 #include "maxsim_common.h"
@@ -40,63 +40,117 @@ __device__ __forceinline__ typename T::storage from_float(float f) {
   else return f;
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack16(uint4 v, float (&f)[kVec<T>]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// V elements as they are in memory (8 or 16 bytes).
+template <typename T, int V = kVec<T>> struct Chunk {
+  static constexpr int words = V * T::bytes / 4;
+  static_assert(words == 2 || words == 4, "8 or 16 bytes");
+  uint32_t w[words];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Chunk<T, V>& c, float (&f)[V]) {
   if constexpr (T::bytes == 2) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f[2 * e] = from16(w[e] & 0xffffu, T{});
-      f[2 * e + 1] = from16(w[e] >> 16, T{});
+    for (int e = 0; e < V / 2; ++e) {
+      f[2 * e] = from16(c.w[e] & 0xffffu, T{});
+      f[2 * e + 1] = from16(c.w[e] >> 16, T{});
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(w[e]);
+    for (int e = 0; e < V; ++e) f[e] = __uint_as_float(c.w[e]);
   }
 }
 
-template <typename T>
-__device__ __forceinline__ uint4 pack16(const float (&f)[kVec<T>]) {
-  uint32_t w[4];
+template <typename T, int V>
+__device__ __forceinline__ Chunk<T, V> pack(const float (&f)[V]) {
+  Chunk<T, V> c;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < Chunk<T, V>::words; ++e) {
     if constexpr (T::bytes == 2)
-      w[e] = bits16(f[2 * e], T{}) | (bits16(f[2 * e + 1], T{}) << 16);
+      c.w[e] = bits16(f[2 * e], T{}) | (bits16(f[2 * e + 1], T{}) << 16);
     else
-      w[e] = __float_as_uint(f[e]);
+      c.w[e] = __float_as_uint(f[e]);
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return c;
 }
 
-template <typename S>
-__device__ __forceinline__ void store16_any(S* p, uint4 v) {
+// From and to an address that is only a multiple of the element size (the
+// compiler knows what the target's loads and stores need).
+template <typename R, typename S>
+__device__ __forceinline__ R load_any(const S* p) {
+  R v;
+  __builtin_memcpy(&v, p, sizeof(v));
+  return v;
+}
+template <typename R, typename S>
+__device__ __forceinline__ void store_any(S* p, R v) {
   __builtin_memcpy(p, &v, sizeof(v));
 }
 
-// Elements [e0, e0 + kVec) of a row, those at or past dim as zero.
-template <typename T>
-__device__ __forceinline__ uint4 load_chunk(const typename T::storage* row, int e0, int dim) {
-  if (e0 + kVec<T> <= dim) return load16_any(row + e0);
-  uint32_t w[4] = {0, 0, 0, 0};
+// Elements [e0, e0 + V) of a row, those at or past dim as zero, in two parts:
+// the load, whole and without a branch (a chunk that reaches past the row's
+// end reads the row's last V elements instead), and, where the data is used,
+// the move into place.  Keeping the second away from the loads lets a row's
+// loads stay in flight.  SHORT: the row may be shorter than a chunk, and such
+// a one is read by elements.
+template <typename T, int V, bool SHORT>
+__device__ __forceinline__ Chunk<T, V> load_chunk(const typename T::storage* row, int e0,
+                                                  int dim) {
+  if (SHORT && dim < V) {
+    Chunk<T, V> r = {};
 #pragma unroll
-  for (int e = 0; e < kVec<T>; ++e)
-    if (e0 + e < dim) {
-      if constexpr (T::bytes == 2) w[e / 2] |= (uint32_t)row[e0 + e] << (16 * (e & 1));
-      else w[e] = __float_as_uint(row[e0 + e]);
-    }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+    for (int e = 0; e < V - 1; ++e)
+      if (e0 + e < dim) {
+        if constexpr (T::bytes == 2) r.w[e / 2] |= (uint32_t)row[e0 + e] << (16 * (e & 1));
+        else r.w[e] = __float_as_uint(row[e0 + e]);
+      }
+    return r;
+  }
+  return load_any<Chunk<T, V>>(row + min(e0, dim - V));
+}
+template <typename T, int V, bool SHORT>
+__device__ __forceinline__ void place_chunk(Chunk<T, V>& c, int e0, int dim) {
+  if (SHORT && dim < V) return;
+  const int n = T::bytes * max(e0 - (dim - V), 0);  // bytes that belong before e0
+  if (dim % V == 0) {  // all or nothing
+#pragma unroll
+    for (int i = 0; i < Chunk<T, V>::words; ++i) c.w[i] = n ? 0 : c.w[i];
+  } else if constexpr (Chunk<T, V>::words == 2) {
+    const uint64_t v = c.w[0] | (uint64_t)c.w[1] << 32;
+    const uint64_t r = n >= 8 ? 0 : v >> (8 * (n & 7));
+    c.w[0] = (uint32_t)r, c.w[1] = (uint32_t)(r >> 32);
+  } else {
+    const uint4 r = drop_bytes(make_uint4(c.w[0], c.w[1], c.w[2], c.w[3]), n);
+    c.w[0] = r.x, c.w[1] = r.y, c.w[2] = r.z, c.w[3] = r.w;
+  }
 }
 
-template <typename T>
+// The row's cut chunk of n elements goes in at most three pieces, by the bits
+// of n.
+template <typename T, int V>
 __device__ __forceinline__ void store_chunk(typename T::storage* row, int e0, int dim,
-                                            const float (&f)[kVec<T>]) {
-  if (e0 + kVec<T> <= dim) {
-    store16_any(row + e0, pack16<T>(f));
+                                            const float (&f)[V]) {
+  const Chunk<T, V> r = pack<T, V>(f);
+  if (e0 + V <= dim) {
+    store_any(row + e0, r);
     return;
   }
-#pragma unroll
-  for (int e = 0; e < kVec<T>; ++e)
-    if (e0 + e < dim) row[e0 + e] = from_float<T>(f[e]);
+  if (e0 >= dim) return;
+  const int n = dim - e0;
+  typename T::storage* p = row + e0;
+  if constexpr (T::bytes == 4) {
+    if (n & 2) store_any(p, make_uint2(r.w[0], r.w[1]));
+    if (n & 1) store_any(p + (n & 2), n & 2 ? r.w[2] : r.w[0]);
+  } else {
+    uint32_t b = r.w[0], c = r.w[1];
+    if constexpr (V == 8) {
+      if (n & 4) store_any(p, make_uint2(r.w[0], r.w[1]));
+      b = n & 4 ? r.w[2] : b;
+      c = n & 4 ? r.w[3] : c;
+    }
+    if (n & 2) store_any(p + (n & 4), b);
+    if (n & 1) p[n & 6] = (uint16_t)(n & 2 ? c : b);
+  }
 }
 
 // N elements of a parameter row of type W in fp32, `fill` where there is no
@@ -105,16 +159,16 @@ template <typename W, int N>
 __device__ __forceinline__ void load_param(const void* p, int e0, int dim, float fill,
                                            float (&f)[N]) {
   const typename W::storage* w = static_cast<const typename W::storage*>(p);
-  constexpr int v = kVec<W>;
-  static_assert(N % v == 0 || N < v, "whole chunks of the parameter's type");
+  constexpr int v = N < kVec<W> ? N : kVec<W>;
+  static_assert(N % v == 0, "whole chunks of the parameter's type");
   if (!w) {
 #pragma unroll
     for (int e = 0; e < N; ++e) f[e] = fill;
-  } else if (N % v == 0 && e0 + N <= dim) {
+  } else if (e0 + N <= dim) {
 #pragma unroll
     for (int c = 0; c < N / v; ++c) {
       float part[v];
-      unpack16<W>(load16_any(w + e0 + c * v), part);
+      unpack<W, v>(load_any<Chunk<W, v>>(w + e0 + c * v), part);
 #pragma unroll
       for (int e = 0; e < v; ++e) f[c * v + e] = part[e];
     }
@@ -123,6 +177,9 @@ __device__ __forceinline__ void load_param(const void* p, int e0, int dim, float
     for (int e = 0; e < N; ++e) f[e] = e0 + e < dim ? to_float<W>(w[e0 + e]) : 0.0f;
   }
 }
+
+// Whether the shape of G lanes takes rows shorter than a chunk.
+constexpr bool takes_short(int G) { return G == 8; }
 
 // Sum over a group of G <= 64 consecutive lanes, in every lane of it, with
 // the same bits in each (each step adds the same two values).  All lanes of
@@ -204,14 +261,14 @@ __device__ __forceinline__ void group_sums(float (&v)[N], float* part) {
 // ---- the shapes (host) -----------------------------------------------------
 
 // Calls f with the group shape for rows of `dim` elements (up to
-// MAXSIM_AMD_MAX_DIM): the one that leaves fewest lanes idle among those that
-// hold a row in at most three chunks per lane; more lanes than a wave where
-// that is not enough.  (Rows of 768 elements of 16 bits, 96 chunks: 32 lanes
-// x 3.)
+// MAXSIM_AMD_MAX_DIM) in chunks of V: the one that leaves fewest lanes idle
+// among those that hold a row in at most three chunks per lane; more lanes
+// than a wave where that is not enough.  (Rows of 768 elements of 16 bits, 96
+// chunks of 8: 32 lanes x 3.)
 template <int G_, int K_> struct Shape { static constexpr int G = G_, K = K_; };
-template <typename T, typename F>
+template <int V, typename F>
 inline void with_shape(int64_t dim, F&& f) {
-  const int64_t chunks = (dim + kVec<T> - 1) / kVec<T>;
+  const int64_t chunks = (dim + V - 1) / V;
   if (chunks <= 8) f(Shape<8, 1>{});
   else if (chunks <= 16) f(Shape<16, 1>{});
   else if (chunks <= 32) f(Shape<16, 2>{});
@@ -222,9 +279,10 @@ inline void with_shape(int64_t dim, F&& f) {
   else if (chunks <= 192) f(Shape<64, 3>{});
   else if (chunks <= 256) f(Shape<256, 1>{});
   else if (chunks <= 512) f(Shape<256, 2>{});
+  else if (chunks <= 768) f(Shape<256, 3>{});
   else if (chunks <= 1024) f(Shape<1024, 1>{});
-  else if (T::bytes == 2 || chunks <= 2048) f(Shape<1024, 2>{});
-  else if constexpr (T::bytes == 4) f(Shape<1024, 4>{});
+  else if (V == 8 || chunks <= 2048) f(Shape<1024, 2>{});
+  else if constexpr (V == 4) f(Shape<1024, 4>{});
 }
 constexpr int row_threads(int G) { return G > 256 ? G : 256; }
 
