@@ -51,14 +51,15 @@ int maxsim_amd_layer_norm_backward(maxsim_dtype dtype, maxsim_dtype weight_dtype
 
 /* y = x / max(|x|, eps) for each row of x [sequences, length, dim] (sequences
  * x_seq_stride and rows x_row_stride apart).
- * lengths NULL: every row.  lengths [sequences]: rows at or past a sequence's
+ * lengths NULL: every row.  lengths [sequences], int32 (lengths64 0) or int64
+ * (1): rows at or past a sequence's
  * length (below 0 counts as 0) are not read.  offsets NULL: y is
  * [sequences, length, dim] and those rows are 0.  offsets [sequences]: y is
  * [packed_rows, dim], row t of sequence s at offsets[s] + t, and they have no
  * row; nothing is written outside y. */
 int maxsim_amd_unit_rows_forward(maxsim_dtype dtype, const void* x, int64_t sequences,
                                  int64_t length, int64_t dim, int64_t x_seq_stride,
-                                 int64_t x_row_stride, const int32_t* lengths,
+                                 int64_t x_row_stride, const void* lengths, int lengths64,
                                  const int32_t* offsets, int64_t packed_rows, float eps, void* y,
                                  void* stream);
 
@@ -68,14 +69,18 @@ int maxsim_amd_unit_rows_forward(maxsim_dtype dtype, const void* x, int64_t sequ
 int maxsim_amd_unit_rows_backward(maxsim_dtype dtype, const void* dy, int64_t dy_seq_stride,
                                   int64_t dy_row_stride, const void* x, int64_t sequences,
                                   int64_t length, int64_t dim, int64_t x_seq_stride,
-                                  int64_t x_row_stride, const int32_t* lengths,
+                                  int64_t x_row_stride, const void* lengths, int lengths64,
                                   const int32_t* offsets, int64_t packed_rows, float eps, void* dx,
                                   void* stream);
 
 /* clamped[s] = lengths[s] in [0, max_len]; offsets[0] = 0 and
- * offsets[s + 1] = offsets[s] + clamped[s], for `sequences` lengths. */
-int maxsim_amd_length_offsets(const int32_t* lengths, int64_t sequences, int64_t max_len,
-                              int32_t* clamped, int32_t* offsets, void* stream);
+ * offsets[s + 1] = offsets[s] + clamped[s], for `sequences` lengths (int32, or
+ * int64 where lengths64).  total, if not NULL, is a zeroed word of pinned host
+ * memory that gets 2 * offsets[sequences] + 1, for a host that waits for the
+ * size alone. */
+int maxsim_amd_length_offsets(const void* lengths, int lengths64, int64_t sequences,
+                              int64_t max_len, int32_t* clamped, int32_t* offsets,
+                              uint64_t* total, void* stream);
 
 /* ---- AdamW --------------------------------------------------------------- */
 

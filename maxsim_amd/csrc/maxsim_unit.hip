@@ -26,7 +26,8 @@ struct UnitRows {
   int64_t x_seq, x_row, dy_seq, dy_row;  // strides in elements (dy: padded only)
   int64_t rows;                          // sequences * length
   int length, dim;
-  const int32_t* lengths;  // NULL: every token is real
+  const void* lengths;  // int32, or int64; NULL: every token is real
+  int lengths64;
   const int32_t* offsets;  // NULL: padded
   int64_t packed_rows;
   float eps;
@@ -75,7 +76,8 @@ __global__ __launch_bounds__(row_threads(G)) void unit_rows_kernel(UnitRows a) {
     at[u].packed = 0;
     if (a.lengths && at[u].real) {
       if (a.offsets) at[u].packed = (int64_t)a.offsets[at[u].seq] + at[u].t;
-      at[u].real = at[u].t < a.lengths[at[u].seq] &&
+      at[u].real = at[u].t < (a.lengths64 ? static_cast<const int64_t*>(a.lengths)[at[u].seq]
+                                          : static_cast<const int32_t*>(a.lengths)[at[u].seq]) &&
                    (!a.offsets || (at[u].packed >= 0 && at[u].packed < a.packed_rows));
     }
   }
@@ -143,39 +145,57 @@ __global__ __launch_bounds__(row_threads(G)) void unit_rows_kernel(UnitRows a) {
 }
 
 // offsets[s] = sum of the lengths before s, each clamped to [0, max_len];
-// offsets[n] the total.  One workgroup: a batch has few thousand sequences,
-// and a thread's share is added in registers between two passes over them.
-constexpr int kScanThreads = 1024;
+// offsets[n] the total, which also goes to `total` (pinned host memory, if
+// given) as 2 * total + 1.  One workgroup: a batch has a few thousand
+// sequences.  A thread takes eight in a row, the waves are joined by their
+// lanes' prefix sums and one barrier (n = 512: 3 us, most of it the launch and
+// the load).
+constexpr int kScanThreads = 1024, kScanWaves = kScanThreads / 64, kScanRun = 8;
+template <typename L>
 __global__ __launch_bounds__(kScanThreads) void length_offsets_kernel(
-    const int32_t* __restrict__ lengths, int64_t n, int32_t max_len, int32_t* __restrict__ clamped,
-    int32_t* __restrict__ offsets) {
-  __shared__ int32_t part[kScanThreads];
-  __shared__ int32_t carried;
-  const int t = threadIdx.x;
-  if (t == 0) carried = 0;
-  __syncthreads();
-  for (int64_t base = 0; base < n; base += kScanThreads) {
-    const int64_t i = base + t;
-    const int32_t len = i < n ? min(max(lengths[i], 0), max_len) : 0;
-    part[t] = len;
-    __syncthreads();
-    for (int off = 1; off < kScanThreads; off <<= 1) {
-      const int32_t before = t >= off ? part[t - off] : 0;
-      __syncthreads();
-      part[t] += before;
-      __syncthreads();
+    const L* __restrict__ lengths, int64_t n, int32_t max_len, int32_t* __restrict__ clamped,
+    int32_t* __restrict__ offsets, uint64_t* total) {
+  __shared__ int32_t waves[2][kScanWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int32_t before = 0;  // sum of the passes before this one
+  int turn = 0;
+  for (int64_t base = 0; base < n; base += kScanThreads * kScanRun, turn ^= 1) {
+    const int64_t i0 = base + threadIdx.x * kScanRun;
+    int32_t len[kScanRun], mine = 0;
+#pragma unroll
+    for (int e = 0; e < kScanRun; ++e) {
+      const L v = i0 + e < n ? lengths[i0 + e] : (L)0;
+      len[e] = (int32_t)min(max(v, (L)0), (L)max_len);
+      mine += len[e];
     }
-    const int32_t start = carried;
-    if (i < n) {
-      clamped[i] = len;
-      offsets[i] = start + part[t] - len;
-      if (i == n - 1) offsets[n] = start + part[t];
+    int32_t upto = mine;  // this thread's and those of the lanes before it
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int32_t v = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += v;
     }
+    if (lane == 63) waves[turn][wave] = upto;
     __syncthreads();
-    if (t == kScanThreads - 1) carried = start + part[t];
-    __syncthreads();
+    int32_t at = before + upto - mine;
+#pragma unroll
+    for (int w = 0; w < kScanWaves; ++w) {
+      before += waves[turn][w];
+      if (w < wave) at += waves[turn][w];
+    }
+#pragma unroll
+    for (int e = 0; e < kScanRun; ++e)
+      if (i0 + e < n) {
+        clamped[i0 + e] = len[e];
+        offsets[i0 + e] = at;
+        at += len[e];
+      }
   }
-  if (n == 0 && t == 0) offsets[0] = 0;
+  if (threadIdx.x == 0) {
+    offsets[n] = before;
+    if (total)
+      __hip_atomic_store(total, 2ull * (uint64_t)before + 1, __ATOMIC_RELEASE,
+                         __HIP_MEMORY_SCOPE_SYSTEM);
+  }
 }
 
 template <bool BACKWARD>
@@ -213,7 +233,7 @@ static int run_unit_rows(maxsim_dtype dtype, const UnitRows& a, void* stream) {
 }
 
 static int check_unit_rows(maxsim_dtype dtype, int64_t sequences, int64_t length, int64_t dim,
-                           const int32_t* lengths, const int32_t* offsets, int64_t packed_rows,
+                           const void* lengths, const int32_t* offsets, int64_t packed_rows,
                            float eps) {
   if (int e = check_dtype(dtype)) return e;
   if (int e = check_dim(dim)) return e;
@@ -234,7 +254,7 @@ extern "C" {
 
 int maxsim_amd_unit_rows_forward(maxsim_dtype dtype, const void* x, int64_t sequences,
                                  int64_t length, int64_t dim, int64_t x_seq_stride,
-                                 int64_t x_row_stride, const int32_t* lengths,
+                                 int64_t x_row_stride, const void* lengths, int lengths64,
                                  const int32_t* offsets, int64_t packed_rows, float eps, void* y,
                                  void* stream) {
   clear_error();
@@ -244,14 +264,15 @@ int maxsim_amd_unit_rows_forward(maxsim_dtype dtype, const void* x, int64_t sequ
   if (sequences == 0 || length == 0 || (offsets && packed_rows == 0)) return MAXSIM_OK;
   if (!x || !y) return fail(MAXSIM_ERR_INVALID, "null pointer argument");
   const UnitRows a{x,           nullptr, x_seq_stride, x_row_stride, 0,           0,
-                   sequences * length, (int)length, (int)dim, lengths, offsets, packed_rows, eps, y};
+                   sequences * length, (int)length, (int)dim, lengths,
+                   lengths64, offsets, packed_rows, eps, y};
   return run_unit_rows<false>(dtype, a, stream);
 }
 
 int maxsim_amd_unit_rows_backward(maxsim_dtype dtype, const void* dy, int64_t dy_seq_stride,
                                   int64_t dy_row_stride, const void* x, int64_t sequences,
                                   int64_t length, int64_t dim, int64_t x_seq_stride,
-                                  int64_t x_row_stride, const int32_t* lengths,
+                                  int64_t x_row_stride, const void* lengths, int lengths64,
                                   const int32_t* offsets, int64_t packed_rows, float eps, void* dx,
                                   void* stream) {
   clear_error();
@@ -263,21 +284,30 @@ int maxsim_amd_unit_rows_backward(maxsim_dtype dtype, const void* dy, int64_t dy
   if (!x || !dx || (!dy && !(offsets && packed_rows == 0)))
     return fail(MAXSIM_ERR_INVALID, "null pointer argument");
   const UnitRows a{x,       dy,          x_seq_stride, x_row_stride, dy_seq_stride, dy_row_stride,
-                   sequences * length, (int)length, (int)dim, lengths, offsets, packed_rows, eps, dx};
+                   sequences * length, (int)length, (int)dim, lengths,
+                   lengths64, offsets, packed_rows, eps, dx};
   return run_unit_rows<true>(dtype, a, stream);
 }
 
-int maxsim_amd_length_offsets(const int32_t* lengths, int64_t sequences, int64_t max_len,
-                              int32_t* clamped, int32_t* offsets, void* stream) {
+int maxsim_amd_length_offsets(const void* lengths, int lengths64, int64_t sequences,
+                              int64_t max_len, int32_t* clamped, int32_t* offsets,
+                              uint64_t* total, void* stream) {
   clear_error();
   if (sequences < 0 || max_len < 0) return fail(MAXSIM_ERR_INVALID, "negative size");
   if (max_len > 0 && sequences > INT32_MAX / max_len)
     return fail(MAXSIM_ERR_UNSUPPORTED, "more than 2^31 - 1 padded rows: offsets are int32");
   if (!offsets || (sequences > 0 && (!lengths || !clamped)))
     return fail(MAXSIM_ERR_INVALID, "null pointer argument");
-  hipLaunchKernelGGL(length_offsets_kernel, dim3(1), dim3(kScanThreads), 0,
-                     static_cast<hipStream_t>(stream), lengths, sequences, (int32_t)max_len,
-                     clamped, offsets);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int32_t most = (int32_t)std::min<int64_t>(max_len, INT32_MAX);
+  if (lengths64)
+    hipLaunchKernelGGL(length_offsets_kernel<int64_t>, dim3(1), dim3(kScanThreads), 0, st,
+                       static_cast<const int64_t*>(lengths), sequences, most, clamped, offsets,
+                       total);
+  else
+    hipLaunchKernelGGL(length_offsets_kernel<int32_t>, dim3(1), dim3(kScanThreads), 0, st,
+                       static_cast<const int32_t*>(lengths), sequences, most, clamped, offsets,
+                       total);
   return check_launch("length_offsets_kernel");
 }
 

@@ -10,7 +10,6 @@
 #include <ATen/core/CachingHostAllocator.h>
 #include <torch/library.h>
 
-#include <chrono>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -102,10 +101,7 @@ Tensor check_begin(const std::vector<std::tuple<Tensor, int, int64_t>>& checks) 
   const auto s = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index());
   // A graph would keep the address of the words and write them on every
   // replay; and the host cannot wait for a kernel that is only recorded.
-  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-  const hipError_t asked = hipStreamIsCapturing(s.stream(), &capture);
-  if (asked != hipSuccess) (void)hipGetLastError();
-  TORCH_CHECK(asked == hipSuccess && capture == hipStreamCaptureStatusNone,
+  TORCH_CHECK(!capturing(s.stream()),
               "maxsim_amd: the checks of offsets, ids and lengths cannot run while the stream is "
               "captured; turn them off around the capture (set_host_checks(False))");
   for (const auto& [t, kind, limit] : checks) {
@@ -162,9 +158,7 @@ Tensor maxsim_check_contrastive(Tensor document_offsets, int64_t total_d,
 }
 
 // Wait for a check on `like`'s device: the longest segment of its first array
-// (0 unless CSR offsets), or -1 when a value is bad.  Polls the words, and the
-// stream every 100 ms (a query puts a marker into it), so that an error there,
-// or a stream that ended without the words, ends the wait.
+// (0 unless CSR offsets), or -1 when a value is bad.
 int64_t maxsim_check_wait(Tensor status, Tensor like) {
   const int64_t words = status.numel() - 2;
   TORCH_CHECK(status.device().is_cpu() && status.scalar_type() == at::kLong &&
@@ -178,28 +172,8 @@ int64_t maxsim_check_wait(Tensor status, Tensor like) {
   c10::hip::HIPGuardMasqueradingAsCUDA guard(like.device());
   int64_t longest = 0;
   bool bad = false;
-  constexpr std::chrono::milliseconds kLook{100};
-  auto look = std::chrono::steady_clock::now() + kLook;
   for (int64_t i = 0; i < words; ++i) {
-    int64_t v = 0;
-    bool drained = false;
-    for (int64_t spins = 1;; ++spins) {
-      v = __atomic_load_n(w + i, __ATOMIC_ACQUIRE);
-      if (v & 1) break;
-      TORCH_CHECK(!drained, "maxsim_amd: the layout check did not report");
-      if (spins % 4096 == 0 && std::chrono::steady_clock::now() >= look) {
-        look = std::chrono::steady_clock::now() + kLook;
-        const hipError_t e = hipStreamQuery(stream);
-        if (e == hipErrorNotReady) {
-          (void)hipGetLastError();
-        } else {
-          TORCH_CHECK(e == hipSuccess, "maxsim_amd: HIP error: ", hipGetErrorString(e));
-          drained = true;  // one more look
-        }
-      } else {
-        __builtin_ia32_pause();
-      }
-    }
+    const int64_t v = wait_for_word(w + i, stream, "the layout check");
     bad |= (v & 2) != 0;
     longest = std::max(longest, (int64_t)((uint64_t)v >> 32));
   }

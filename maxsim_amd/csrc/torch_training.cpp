@@ -6,6 +6,7 @@
 // the dispatcher, so that torch.compile records the operators themselves.
 // Argument errors are raised here with Python's types (one pass over an
 // optimizer's tensors instead of one per check).
+#include <ATen/core/CachingHostAllocator.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
@@ -221,12 +222,20 @@ void check_unit(const Tensor& x, const optional<Tensor>& lengths, double eps) {
   check_same_device(*lengths, "lengths", x, "x");
 }
 
-// int32 lengths for the kernels, which cut them to [0, L] themselves; int64
-// ones are cut before they are narrowed, so that none wraps into the range.
-Tensor lengths_i32(const optional<Tensor>& lengths, int64_t max_len) {
-  if (!lengths.has_value()) return Tensor();
-  if (lengths->scalar_type() == at::kInt) return lengths->contiguous();
-  return lengths->clamp(0, max_len).to(at::kInt).contiguous();
+// Contiguous lengths (or nothing) and how wide they are; the kernels cut them
+// to [0, L] themselves.
+struct Lengths {
+  Tensor t;
+  const void* data = nullptr;
+  int is64 = 0;
+};
+Lengths lengths_of(const optional<Tensor>& lengths) {
+  Lengths l;
+  if (!lengths.has_value()) return l;
+  l.t = lengths->contiguous();
+  l.is64 = l.t.scalar_type() == at::kLong;
+  l.data = l.t.data_ptr();
+  return l;
 }
 
 const int32_t* i32(const Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; }
@@ -235,7 +244,7 @@ const int32_t* i32(const Tensor& t) { return t.defined() ? t.data_ptr<int32_t>()
 // rows are told apart by two strides at most.
 Rows unit_rows(const Tensor& x) { return rows_of(x, x.dim() >= 3 ? x.dim() - 2 : 0); }
 
-Tensor unit_forward(const Tensor& x, const Tensor& lengths, const Tensor& offsets,
+Tensor unit_forward(const Tensor& x, const Lengths& lengths, const Tensor& offsets,
                     int64_t packed_rows, double eps) {
   const Rows r = unit_rows(x);
   Tensor y = offsets.defined() ? at::empty({packed_rows, x.size(-1)}, x.options())
@@ -243,12 +252,13 @@ Tensor unit_forward(const Tensor& x, const Tensor& lengths, const Tensor& offset
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   check_status(maxsim_amd_unit_rows_forward(
       dtype_of(x, "x"), r.t.data_ptr(), r.outer, r.inner, x.size(-1), r.outer_stride,
-      r.inner_stride, i32(lengths), i32(offsets), packed_rows, (float)eps, y.data_ptr(),
+      r.inner_stride, lengths.data, lengths.is64, i32(offsets), packed_rows, (float)eps,
+      y.data_ptr(),
       current_stream(x)));
   return y;
 }
 
-Tensor unit_backward(const Tensor& dy, const Tensor& x, const Tensor& lengths,
+Tensor unit_backward(const Tensor& dy, const Tensor& x, const Lengths& lengths,
                      const Tensor& offsets, int64_t packed_rows, double eps) {
   TORCH_CHECK(dy.scalar_type() == x.scalar_type(), "dy must have x's dtype");
   check_same_device(dy, "dy", x, "x");
@@ -263,39 +273,53 @@ Tensor unit_backward(const Tensor& dy, const Tensor& x, const Tensor& lengths,
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   check_status(maxsim_amd_unit_rows_backward(
       dtype_of(x, "x"), g.t.data_ptr(), g.outer_stride, g.inner_stride, r.t.data_ptr(), r.outer,
-      r.inner, x.size(-1), r.outer_stride, r.inner_stride, i32(lengths), i32(offsets),
-      packed_rows, (float)eps, dx.data_ptr(), current_stream(x)));
+      r.inner, x.size(-1), r.outer_stride, r.inner_stride, lengths.data, lengths.is64,
+      i32(offsets), packed_rows, (float)eps, dx.data_ptr(), current_stream(x)));
   return dx;
 }
 
 Tensor maxsim_normalize_embeddings(const Tensor& x, const optional<Tensor>& lengths, double eps) {
   check_unit(x, lengths, eps);
-  return unit_forward(x, lengths_i32(lengths, x.dim() == 3 ? x.size(1) : 0), Tensor(), 0, eps);
+  return unit_forward(x, lengths_of(lengths), Tensor(), 0, eps);
 }
 
 Tensor maxsim_normalize_embeddings_backward(const Tensor& dy, const Tensor& x,
                                             const optional<Tensor>& lengths, double eps) {
   check_unit(x, lengths, eps);
   TORCH_CHECK(dy.sizes() == x.sizes(), "dy must have x's shape");
-  return unit_backward(dy, x, lengths_i32(lengths, x.dim() == 3 ? x.size(1) : 0), Tensor(), 0,
-                       eps);
+  return unit_backward(dy, x, lengths_of(lengths), Tensor(), 0, eps);
 }
 
 // Lengths cut to [0, max_len], the offsets of the packed sequences [N + 1] and
-// their rows in all, which the host waits for.
+// their rows in all, which the host waits for: in a word of pinned memory that
+// the kernel writes, which comes sooner than a copy and a synchronization.
 std::tuple<Tensor, Tensor, int64_t> maxsim_length_offsets(const Tensor& lengths,
                                                           int64_t max_len) {
   check_hip(lengths, "lengths");
   check_lengths(lengths);
   TORCH_CHECK_VALUE(lengths.dim() == 1, "lengths must be 1-D; got ", lengths.sizes());
-  const Tensor l = lengths_i32(lengths, max_len);
-  const int64_t n = l.numel();
-  Tensor clamped = at::empty({n}, i32_opts(l)), offsets = at::empty({n + 1}, i32_opts(l));
-  c10::hip::HIPGuardMasqueradingAsCUDA guard(l.device());
-  check_status(maxsim_amd_length_offsets(l.data_ptr<int32_t>(), n, max_len,
-                                         clamped.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(),
-                                         current_stream(l)));
-  return {clamped, offsets, offsets.select(0, n).item<int32_t>()};
+  const Lengths l = lengths_of(lengths);
+  const int64_t n = l.t.numel();
+  Tensor clamped = at::empty({n}, i32_opts(l.t)), offsets = at::empty({n + 1}, i32_opts(l.t));
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(l.t.device());
+  const auto s = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(l.t.device().index());
+  TORCH_CHECK(!capturing(s.stream()),
+              "maxsim_amd: packing waits for the lengths and cannot run while the stream is "
+              "captured");
+  at::DataPtr pinned = at::getHostAllocator(at::kCUDA)->allocate(sizeof(uint64_t));
+  uint64_t* word = static_cast<uint64_t*>(pinned.get());
+  *word = 0;
+  check_status(maxsim_amd_length_offsets(l.data, l.is64, n, max_len, clamped.data_ptr<int32_t>(),
+                                         offsets.data_ptr<int32_t>(), word, s.stream()));
+  int64_t total = 0;
+  try {
+    total = wait_for_word(reinterpret_cast<int64_t*>(word), s.stream(), "the offsets") >> 1;
+  } catch (...) {
+    // the kernel may still write the word
+    at::getHostAllocator(at::kCUDA)->record_event(word, pinned.get_context(), s.unwrap());
+    throw;
+  }
+  return {clamped, offsets, total};
 }
 
 void check_packed(const Tensor& x, const Tensor& lengths, const Tensor& offsets,
@@ -312,14 +336,14 @@ void check_packed(const Tensor& x, const Tensor& lengths, const Tensor& offsets,
 Tensor maxsim_pack_normalized(const Tensor& x, const Tensor& lengths, const Tensor& offsets,
                               int64_t packed_rows, double eps) {
   check_packed(x, lengths, offsets, packed_rows, eps);
-  return unit_forward(x, lengths, offsets, packed_rows, eps);
+  return unit_forward(x, lengths_of(lengths), offsets, packed_rows, eps);
 }
 
 Tensor maxsim_pack_normalized_backward(const Tensor& dy, const Tensor& x, const Tensor& lengths,
                                        const Tensor& offsets, double eps) {
   check_packed(x, lengths, offsets, 0, eps);
   TORCH_CHECK(dy.dim() == 2 && dy.size(1) == x.size(2), "dy must be [rows, dim]");
-  return unit_backward(dy, x, lengths, offsets, dy.size(0), eps);
+  return unit_backward(dy, x, lengths_of(lengths), offsets, dy.size(0), eps);
 }
 
 // ---- autograd ----------------------------------------------------------------

@@ -80,11 +80,11 @@ def test_layer_norm_backward_refusals(lib):
 
 def test_unit_rows_refusals(lib):
     fn = lib.maxsim_amd_unit_rows_forward
-    fn.argtypes = [ctypes.c_int, P, I64, I64, I64, I64, I64, P, P, I64, F, P, P]
+    fn.argtypes = [ctypes.c_int, P, I64, I64, I64, I64, I64, P, ctypes.c_int, P, I64, F, P, P]
 
     def call(dtype=F16, x=ONE, n=2, length=3, dim=64, stride=64, lengths=ONE, offsets=None, rows=0,
              eps=1e-12, y=ONE):
-        return fn(dtype, x, n, length, dim, stride, stride, lengths, offsets, rows, eps, y, None)
+        return fn(dtype, x, n, length, dim, stride, stride, lengths, 0, offsets, rows, eps, y, None)
 
     assert call(n=0, x=None, y=None) == OK and call(length=0, x=None, y=None) == OK
     assert call(offsets=ONE, rows=0, y=None) == OK
@@ -98,14 +98,17 @@ def test_unit_rows_refusals(lib):
         assert text in lib.maxsim_amd_last_error()
     assert call(dim=16385) == UNSUPPORTED and call(length=2 ** 31) == UNSUPPORTED
     back = lib.maxsim_amd_unit_rows_backward
-    back.argtypes = [ctypes.c_int, P, I64, I64, P, I64, I64, I64, I64, I64, P, P, I64, F, P, P]
-    assert back(F16, None, 64, 64, ONE, 2, 3, 64, 64, 64, ONE, None, 0, 1e-12, ONE, None) == INVALID
-    assert back(F16, ONE, -1, 64, ONE, 2, 3, 64, 64, 64, ONE, None, 0, 1e-12, ONE, None) == INVALID
+    back.argtypes = [ctypes.c_int, P, I64, I64, P, I64, I64, I64, I64, I64, P, ctypes.c_int, P, I64,
+                     F, P, P]
+    assert back(F16, None, 64, 64, ONE, 2, 3, 64, 64, 64, ONE, 0, None, 0, 1e-12, ONE,
+                None) == INVALID
+    assert back(F16, ONE, -1, 64, ONE, 2, 3, 64, 64, 64, ONE, 0, None, 0, 1e-12, ONE,
+                None) == INVALID
     scan = lib.maxsim_amd_length_offsets
-    scan.argtypes = [P, I64, I64, P, P, P]
-    assert scan(ONE, -1, 5, ONE, ONE, None) == INVALID
-    assert scan(None, 4, 5, ONE, ONE, None) == INVALID
-    assert scan(ONE, 1 << 16, 1 << 15, ONE, ONE, None) == UNSUPPORTED  # offsets past int32
+    scan.argtypes = [P, ctypes.c_int, I64, I64, P, P, P, P]
+    assert scan(ONE, 0, -1, 5, ONE, ONE, None, None) == INVALID
+    assert scan(None, 0, 4, 5, ONE, ONE, None, None) == INVALID
+    assert scan(ONE, 0, 1 << 16, 1 << 15, ONE, ONE, None, None) == UNSUPPORTED  # offsets past int32
 
 
 def test_adamw_refusals(lib):
