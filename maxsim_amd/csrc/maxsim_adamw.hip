@@ -41,6 +41,13 @@ constexpr int kChunkElems = kAdamThreads * kLaneElems;
 constexpr int64_t kMaxElems = (int64_t)1 << 40;  // of a step: 32-bit block numbers
 constexpr int64_t kMaxChunks = UINT32_MAX / kAdamThreads;  // of a launch: threads in 32 bits
 
+// LDS that a workgroup of the 32-bit step asks for and does not use: it keeps a
+// CU at two workgroups, 64 KB of loads in flight.  More get into each other's
+// way in the memory (66 M fp32 parameters: 346 us with two, 353 with four, 355
+// with eight; bf16 273 / 284).  The 8-bit step has half the bytes and more
+// arithmetic per element, and needs all eight.
+constexpr unsigned kReservedLds = 56 << 10;
+
 // The tensors of a launch, as many as 4 KB of kernel arguments hold (88 in
 // the plain 32-bit step, 61 with 8-bit states and masters).
 template <int BITS, bool MASTER> struct AdamArgs {
@@ -398,7 +405,8 @@ int maxsim_amd_adamw_step(maxsim_dtype param_dtype, maxsim_dtype grad_dtype, int
     uint32_t chunks = 0;
     auto launch = [&] {
       hipLaunchKernelGGL((adamw_kernel<decltype(p), decltype(g), BITS, MASTER>), dim3(chunks),
-                         dim3(kAdamThreads), 0, static_cast<hipStream_t>(stream), a);
+                         dim3(kAdamThreads), BITS == 32 ? kReservedLds : 0,
+                         static_cast<hipStream_t>(stream), a);
       a.count = 0, chunks = 0;
       return check_launch("adamw_kernel");
     };

@@ -87,12 +87,49 @@ __device__ __forceinline__ void store_any(S* p, R v) {
   __builtin_memcpy(p, &v, sizeof(v));
 }
 
-// Elements [e0, e0 + V) of a row, those at or past dim as zero, in two parts:
+// Elements [e0, e0 + V) of a row, those at or past dim as zero: the row's cut
+// chunk of n elements comes in at most three pieces, by the bits of n.  For
+// rows that are asked for once (unit rows): lanes past the row's end read
+// nothing (1000 x 300 x 300 f16: 53 us against 60 with load_chunk).
+template <typename T, int V>
+__device__ __forceinline__ Chunk<T, V> load_pieces(const typename T::storage* row, int e0,
+                                                   int dim) {
+  typedef Chunk<T, V> C;
+  if (e0 + V <= dim) return load_any<C>(row + e0);
+  C r = {};
+  if (e0 >= dim) return r;
+  const int n = dim - e0;
+  const typename T::storage* p = row + e0;
+  if constexpr (T::bytes == 4) {
+    const uint2 a = n & 2 ? load_any<uint2>(p) : make_uint2(0, 0);
+    const uint32_t c = n & 1 ? load_any<uint32_t>(p + (n & 2)) : 0;
+    r.w[0] = n & 2 ? a.x : c;
+    r.w[1] = a.y;
+    r.w[2] = n == 3 ? c : 0;
+  } else {
+    const uint32_t b = n & 2 ? load_any<uint32_t>(p + (n & 4)) : 0;
+    const uint32_t c = n & 1 ? p[n & 6] : 0;
+    const uint32_t bc = n & 2 ? b : c;
+    r.w[0] = bc;
+    r.w[1] = n & 2 ? c : 0;
+    if constexpr (V == 8) {
+      const uint2 a = n & 4 ? load_any<uint2>(p) : make_uint2(0, 0);
+      r.w[2] = n & 4 ? bc : 0;
+      r.w[3] = n & 4 ? r.w[1] : 0;
+      r.w[0] = n & 4 ? a.x : bc;
+      r.w[1] = n & 4 ? a.y : r.w[1];
+    }
+  }
+  return r;
+}
+
+// The same in two parts, for rows that are asked for a turn ahead (layer norm):
 // the load, whole and without a branch (a chunk that reaches past the row's
 // end reads the row's last V elements instead), and, where the data is used,
 // the move into place.  Keeping the second away from the loads lets a row's
-// loads stay in flight.  SHORT: the row may be shorter than a chunk, and such
-// a one is read by elements.
+// loads stay in flight (200000 x 300 bf16, forward and backward: 52 + 78 us
+// against 57 + 86 with the branches of load_pieces).  SHORT: the row may be
+// shorter than a chunk, and such a one is read by elements.
 template <typename T, int V, bool SHORT>
 __device__ __forceinline__ Chunk<T, V> load_chunk(const typename T::storage* row, int e0,
                                                   int dim) {

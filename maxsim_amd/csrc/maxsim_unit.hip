@@ -24,7 +24,7 @@ struct UnitRows {
   const void* x;
   const void* dy;  // backward only
   int64_t x_seq, x_row, dy_seq, dy_row;  // strides in elements (dy: padded only)
-  int64_t rows;                          // sequences * length
+  int64_t sequences, rows;               // rows: sequences * length
   int length, dim;
   const void* lengths;  // int32, or int64; NULL: every token is real
   int lengths64;
@@ -42,12 +42,21 @@ struct Place {
   int64_t packed;
 };
 
+// Both words of an int64 length, the one of an int32 twice: no branch that a
+// load would wait at.
+__device__ __forceinline__ int64_t length_of(const UnitRows& a, int64_t seq) {
+  const int is64 = a.lengths64 ? 1 : 0;
+  const int32_t* l = static_cast<const int32_t*>(a.lengths) + (seq << is64);
+  const int32_t lo = l[0], hi = l[is64];
+  return is64 ? (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo) : lo;
+}
+
 // Workgroup b takes the rows from b * GROUPS * U on, each group of lanes U of
 // them, GROUPS apart: the lengths of all U are asked for together, then the
 // rows themselves, so that a wave waits for two loads in a row however many
 // rows it has (a loop over rows that looked one ahead waited for both in every
 // turn: 38 + 72 us for the forward and backward of 512 x 1024 x 128 packed
-// in bf16, against 31 + 62).
+// in bf16, against 29 + 51).
 template <typename T, int G, int K, int U, bool BACKWARD>
 __global__ __launch_bounds__(row_threads(G)) void unit_rows_kernel(UnitRows a) {
   using S = typename T::storage;
@@ -74,11 +83,37 @@ __global__ __launch_bounds__(row_threads(G)) void unit_rows_kernel(UnitRows a) {
     at[u].t = (int)(past - more * length);
     at[u].real = row0 + u * GROUPS + group < a.rows;
     at[u].packed = 0;
-    if (a.lengths && at[u].real) {
-      if (a.offsets) at[u].packed = (int64_t)a.offsets[at[u].seq] + at[u].t;
-      at[u].real = at[u].t < (a.lengths64 ? static_cast<const int64_t*>(a.lengths)[at[u].seq]
-                                          : static_cast<const int32_t*>(a.lengths)[at[u].seq]) &&
-                   (!a.offsets || (at[u].packed >= 0 && at[u].packed < a.packed_rows));
+  }
+  if (a.lengths) {
+    int64_t len[U];
+    int32_t off[U];
+    const int64_t last = a.sequences - 1;
+    if (length >= (uint32_t)(GROUPS * U)) {
+      // rows of two sequences at most: loads that are the workgroup's own
+      const int64_t seq1 = min(seq0 + 1, last);
+      const int64_t len0 = length_of(a, seq0), len1 = length_of(a, seq1);
+      const int32_t off0 = a.offsets ? a.offsets[seq0] : 0, off1 = a.offsets ? a.offsets[seq1] : 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        len[u] = at[u].seq == seq0 ? len0 : len1;
+        off[u] = at[u].seq == seq0 ? off0 : off1;
+      }
+    } else {
+      // all loads before the first use
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t seq = min(at[u].seq, last);
+        len[u] = length_of(a, seq);
+        off[u] = a.offsets ? a.offsets[seq] : 0;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      at[u].real = at[u].real && at[u].t < len[u];
+      if (a.offsets) {
+        at[u].packed = (int64_t)off[u] + at[u].t;
+        at[u].real = at[u].real && at[u].packed >= 0 && at[u].packed < a.packed_rows;
+      }
     }
   }
   Chunk<T> raw[U][K], raw_d[BACKWARD ? U : 1][K];
@@ -87,24 +122,18 @@ __global__ __launch_bounds__(row_threads(G)) void unit_rows_kernel(UnitRows a) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const S* xr = x + at[u].seq * a.x_seq + at[u].t * a.x_row;
-      raw[u][k] = at[u].real ? load_chunk<T, V, takes_short(G)>(xr, (j + k * G) * V, dim) : Chunk<T>{};
+      raw[u][k] = at[u].real ? load_pieces<T, V>(xr, (j + k * G) * V, dim) : Chunk<T>{};
       if constexpr (BACKWARD) {
         const S* dr = a.offsets ? dy + at[u].packed * dim
                                 : dy + at[u].seq * a.dy_seq + at[u].t * a.dy_row;
-        raw_d[u][k] = at[u].real ? load_chunk<T, V, takes_short(G)>(dr, (j + k * G) * V, dim) : Chunk<T>{};
+        raw_d[u][k] = at[u].real ? load_pieces<T, V>(dr, (j + k * G) * V, dim) : Chunk<T>{};
       }
     }
-  const bool whole = dim == G * K * V;
   float sums[SUMS] = {};
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (!whole) {
-        place_chunk<T, V, takes_short(G)>(raw[u][k], (j + k * G) * V, dim);
-        if constexpr (BACKWARD)
-          place_chunk<T, V, takes_short(G)>(raw_d[u][k], (j + k * G) * V, dim);
-      }
       float f[V], d[V];
       unpack<T, V>(raw[u][k], f);
       if constexpr (BACKWARD) unpack<T, V>(raw_d[u][k], d);
@@ -264,7 +293,7 @@ int maxsim_amd_unit_rows_forward(maxsim_dtype dtype, const void* x, int64_t sequ
   if (sequences == 0 || length == 0 || (offsets && packed_rows == 0)) return MAXSIM_OK;
   if (!x || !y) return fail(MAXSIM_ERR_INVALID, "null pointer argument");
   const UnitRows a{x,           nullptr, x_seq_stride, x_row_stride, 0,           0,
-                   sequences * length, (int)length, (int)dim, lengths,
+                   sequences, sequences * length, (int)length, (int)dim, lengths,
                    lengths64, offsets, packed_rows, eps, y};
   return run_unit_rows<false>(dtype, a, stream);
 }
@@ -284,7 +313,7 @@ int maxsim_amd_unit_rows_backward(maxsim_dtype dtype, const void* dy, int64_t dy
   if (!x || !dx || (!dy && !(offsets && packed_rows == 0)))
     return fail(MAXSIM_ERR_INVALID, "null pointer argument");
   const UnitRows a{x,       dy,          x_seq_stride, x_row_stride, dy_seq_stride, dy_row_stride,
-                   sequences * length, (int)length, (int)dim, lengths,
+                   sequences, sequences * length, (int)length, (int)dim, lengths,
                    lengths64, offsets, packed_rows, eps, dx};
   return run_unit_rows<true>(dtype, a, stream);
 }
