@@ -154,12 +154,11 @@ def _(x, weight, bias, eps):
 
 @torch.library.register_fake("maxsim_amd::maxsim_layer_norm_forward")
 def _(x, weight, bias, eps):
-    rows = (x.numel() // x.shape[-1],)
-    return x.new_empty(x.shape), _f32(x, rows), _f32(x, rows)
+    return x.new_empty(x.shape), _f32(x, (2, x.numel() // x.shape[-1]))
 
 
 @torch.library.register_fake("maxsim_amd::maxsim_layer_norm_backward")
-def _(dy, x, mean, rstd, weight, want_dx, want_dweight, want_dbias, weight_dtype):
+def _(dy, x, stats, weight, want_dx, want_dweight, want_dbias, weight_dtype):
     dim = x.shape[-1]
     return (x.new_empty(x.shape if want_dx else (0,)),
             x.new_empty((dim if want_dweight else 0,), dtype=weight_dtype),

@@ -150,37 +150,33 @@ Tensor maxsim_layer_norm(const Tensor& x, const optional<Tensor>& weight,
   return run_norm(prep_norm(x, weight, bias, eps), eps, nullptr, nullptr);
 }
 
-// With what the backward needs: mean and 1 / sqrt(variance + eps) per row.
-std::tuple<Tensor, Tensor, Tensor> maxsim_layer_norm_forward(const Tensor& x,
-                                                             const optional<Tensor>& weight,
-                                                             const optional<Tensor>& bias,
-                                                             double eps) {
+// With what the backward needs: the rows' means, then 1 / sqrt(variance + eps).
+std::tuple<Tensor, Tensor> maxsim_layer_norm_forward(const Tensor& x,
+                                                     const optional<Tensor>& weight,
+                                                     const optional<Tensor>& bias, double eps) {
   const Norm n = prep_norm(x, weight, bias, eps);
   Tensor stats = at::empty({2, n.x.inner}, f32_opts(x));
   float* s = stats.data_ptr<float>();
-  Tensor y = run_norm(n, eps, s, s + n.x.inner);
-  return {y, stats.select(0, 0), stats.select(0, 1)};
+  return {run_norm(n, eps, s, s + n.x.inner), stats};
 }
 
 // Gradients that are not asked for come back empty.
 std::tuple<Tensor, Tensor, Tensor> maxsim_layer_norm_backward(
-    const Tensor& dy, const Tensor& x, const Tensor& mean, const Tensor& rstd,
-    const optional<Tensor>& weight, bool want_dx, bool want_dweight, bool want_dbias,
-    at::ScalarType weight_dtype) {
+    const Tensor& dy, const Tensor& x, const Tensor& stats, const optional<Tensor>& weight,
+    bool want_dx, bool want_dweight, bool want_dbias, at::ScalarType weight_dtype) {
   check_norm_x(x, 0.0);
   TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(),
               "dy must have x's shape and dtype");
   check_same_device(dy, "dy", x, "x");
   const Rows xr = rows_of(x, 0), gr = rows_of(dy, 0);
-  for (const Tensor* s : {&mean, &rstd}) {
-    TORCH_CHECK(s->scalar_type() == at::kFloat && s->numel() == xr.inner && s->is_contiguous(),
-                "mean and rstd must be float32, one per row");
-    check_same_device(*s, "mean", x, "x");
-  }
+  const int64_t rows = xr.inner, dim = x.size(-1);
+  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.numel() == 2 * rows &&
+                  stats.is_contiguous(),
+              "stats must be float32 [2, rows]");
+  check_same_device(stats, "stats", x, "x");
   const Tensor w = norm_param(weight, "weight", x);
   const maxsim_dtype dt = dtype_of(x, "x");
   const auto wopts = x.options().dtype(weight_dtype);
-  const int64_t rows = xr.inner, dim = x.size(-1);
   Tensor dx = want_dx ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
   Tensor dw = at::empty({want_dweight ? dim : 0}, wopts);
   Tensor db = at::empty({want_dbias ? dim : 0}, wopts);
@@ -188,12 +184,13 @@ std::tuple<Tensor, Tensor, Tensor> maxsim_layer_norm_backward(
   const maxsim_dtype wdt = dtype_of(dw, "weight");
   const bool sums = want_dweight || want_dbias;
   const size_t bytes = sums ? maxsim_amd_layer_norm_backward_workspace_size(dt, rows, dim) : 0;
-  Tensor ws = at::empty({(int64_t)(bytes / sizeof(float))}, f32_opts(x));
+  Tensor ws;
+  if (bytes > 0) ws = at::empty({(int64_t)(bytes / sizeof(float))}, f32_opts(x));
+  const float* s = stats.data_ptr<float>();
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   check_status(maxsim_amd_layer_norm_backward(
-      dt, wdt, gr.t.data_ptr(), gr.inner_stride, xr.t.data_ptr(), xr.inner_stride,
-      mean.data_ptr<float>(), rstd.data_ptr<float>(), ptr(w), rows, dim,
-      want_dx ? dx.data_ptr() : nullptr, want_dweight ? dw.data_ptr() : nullptr,
+      dt, wdt, gr.t.data_ptr(), gr.inner_stride, xr.t.data_ptr(), xr.inner_stride, s, s + rows,
+      ptr(w), rows, dim, want_dx ? dx.data_ptr() : nullptr, want_dweight ? dw.data_ptr() : nullptr,
       want_dbias ? db.data_ptr() : nullptr, bytes > 0 ? ws.data_ptr() : nullptr, bytes,
       current_stream(x)));
   return {dx, dw, db};
@@ -364,9 +361,9 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& weight,
                         const optional<Tensor>& bias, double eps) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [y, mean, rstd] = MAXSIM_CALL(maxsim_layer_norm_forward, x, weight, bias, eps);
+    auto [y, stats] = MAXSIM_CALL(maxsim_layer_norm_forward, x, weight, bias, eps);
     const bool has_w = weight.has_value(), has_b = bias.has_value();
-    ctx->save_for_backward({x, has_w ? *weight : Tensor(), mean, rstd});
+    ctx->save_for_backward({x, has_w ? *weight : Tensor(), stats});
     ctx->saved_data["has_w"] = has_w;
     ctx->saved_data["has_b"] = has_b;
     ctx->saved_data["dtype"] =
@@ -382,8 +379,8 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     const bool want_b = has_b && ctx->needs_input_grad(1 + has_w);
     const optional<Tensor> weight = has_w ? optional<Tensor>(saved[1]) : std::nullopt;
     auto [dx, dw, db] = MAXSIM_CALL(
-        maxsim_layer_norm_backward, grads[0], saved[0], saved[2], saved[3], weight, want_x, want_w,
-        want_b, (at::ScalarType)ctx->saved_data["dtype"].toInt());
+        maxsim_layer_norm_backward, grads[0], saved[0], saved[2], weight, want_x, want_w, want_b,
+        (at::ScalarType)ctx->saved_data["dtype"].toInt());
     return {want_x ? dx : Tensor(), want_w ? dw : Tensor(), want_b ? db : Tensor(), Tensor()};
   }
 };
@@ -600,10 +597,10 @@ TORCH_LIBRARY_FRAGMENT(maxsim_amd, m) {
   // none of these is the reference's, whose training example leaves them to torch
   m.def("maxsim_layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor");
   m.def("maxsim_layer_norm_forward(Tensor x, Tensor? weight, Tensor? bias, float eps) "
+        "-> (Tensor, Tensor)");
+  m.def("maxsim_layer_norm_backward(Tensor dy, Tensor x, Tensor stats, Tensor? weight, "
+        "bool want_dx, bool want_dweight, bool want_dbias, ScalarType weight_dtype) "
         "-> (Tensor, Tensor, Tensor)");
-  m.def("maxsim_layer_norm_backward(Tensor dy, Tensor x, Tensor mean, Tensor rstd, "
-        "Tensor? weight, bool want_dx, bool want_dweight, bool want_dbias, "
-        "ScalarType weight_dtype) -> (Tensor, Tensor, Tensor)");
   m.def("maxsim_normalize_embeddings(Tensor x, Tensor? lengths, float eps) -> Tensor");
   m.def("maxsim_normalize_embeddings_backward(Tensor dy, Tensor x, Tensor? lengths, float eps) "
         "-> Tensor");
@@ -642,4 +639,6 @@ TORCH_LIBRARY_IMPL(maxsim_amd, AutogradCUDA, m) {
   m.impl("maxsim_layer_norm", &layer_norm_autograd);
   m.impl("maxsim_normalize_embeddings", &normalize_autograd);
   m.impl("maxsim_pack_normalized", &pack_normalized_autograd);
+  // nothing to record, and its hundreds of tensors need not be looked at for it
+  m.impl("maxsim_adamw_step", torch::CppFunction::makeFallthrough());
 }
