@@ -25,6 +25,7 @@ struct UnitRows {
   const void* dy;  // backward only
   int64_t x_seq, x_row, dy_seq, dy_row;  // strides in elements (dy: padded only)
   int64_t sequences, rows;               // rows: sequences * length
+  int64_t begin;                         // first row of this launch
   int length, dim;
   const void* lengths;  // int32, or int64; NULL: every token is real
   int lengths64;
@@ -51,7 +52,7 @@ __device__ __forceinline__ int64_t length_of(const UnitRows& a, int64_t seq) {
   return is64 ? (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo) : lo;
 }
 
-// Workgroup b takes the rows from b * GROUPS * U on, each group of lanes U of
+// Workgroup b takes the rows from begin + b * GROUPS * U on, each group of lanes U of
 // them, GROUPS apart: the lengths of all U are asked for together, then the
 // rows themselves, so that a wave waits for two loads in a row however many
 // rows it has (a loop over rows that looked one ahead waited for both in every
@@ -70,7 +71,7 @@ __global__ __launch_bounds__(row_threads(G)) void unit_rows_kernel(UnitRows a) {
   S* out = static_cast<S*>(a.out);
 
   // the workgroup's first row by one division, its others by what they are past it
-  const int64_t row0 = (int64_t)blockIdx.x * GROUPS * U;
+  const int64_t row0 = a.begin + (int64_t)blockIdx.x * GROUPS * U;
   const uint32_t length = (uint32_t)a.length;
   const int64_t seq0 = row0 >> 32 ? row0 / length : (int64_t)((uint32_t)row0 / length);
   const uint32_t t0 = (uint32_t)(row0 - seq0 * length);
@@ -234,13 +235,14 @@ static int run_unit_rows(maxsim_dtype dtype, const UnitRows& a, void* stream) {
     using T = decltype(t);
     constexpr int G = decltype(s)::G, K = decltype(s)::K, U = decltype(rows)::value;
     constexpr int threads = row_threads(G), each = threads / G * U;
-    const int64_t blocks = (a.rows + each - 1) / each;
-    if (blocks > UINT32_MAX / threads) {
-      rc = fail(MAXSIM_ERR_UNSUPPORTED, "too many rows for one launch");
-      return;
+    constexpr int64_t most = UINT32_MAX / threads;  // a launch's threads fit 32 bits
+    UnitRows part = a;
+    for (; part.begin < a.rows && rc == MAXSIM_OK; part.begin += most * each) {
+      const int64_t blocks = std::min<int64_t>((a.rows - part.begin + each - 1) / each, most);
+      hipLaunchKernelGGL((unit_rows_kernel<T, G, K, U, BACKWARD>), dim3((unsigned)blocks),
+                         dim3(threads), 0, static_cast<hipStream_t>(stream), part);
+      rc = check_launch("unit_rows_kernel");
     }
-    hipLaunchKernelGGL((unit_rows_kernel<T, G, K, U, BACKWARD>), dim3((unsigned)blocks),
-                       dim3(threads), 0, static_cast<hipStream_t>(stream), a);
   };
   // Rows per group: more where each waits for its sequence's length first
   // (32000 x 300 x 128 f16, forward: 673 us with four against 705 with two;
@@ -258,7 +260,7 @@ static int run_unit_rows(maxsim_dtype dtype, const UnitRows& a, void* stream) {
   if (dtype == MAXSIM_FLOAT32) go(F32{});
   else if (dtype == MAXSIM_FLOAT16) go(F16{});
   else go(BF16{});
-  return rc ? rc : check_launch("unit_rows_kernel");
+  return rc;
 }
 
 static int check_unit_rows(maxsim_dtype dtype, int64_t sequences, int64_t length, int64_t dim,
@@ -293,7 +295,7 @@ int maxsim_amd_unit_rows_forward(maxsim_dtype dtype, const void* x, int64_t sequ
   if (sequences == 0 || length == 0 || (offsets && packed_rows == 0)) return MAXSIM_OK;
   if (!x || !y) return fail(MAXSIM_ERR_INVALID, "null pointer argument");
   const UnitRows a{x,           nullptr, x_seq_stride, x_row_stride, 0,           0,
-                   sequences, sequences * length, (int)length, (int)dim, lengths,
+                   sequences, sequences * length, 0, (int)length, (int)dim, lengths,
                    lengths64, offsets, packed_rows, eps, y};
   return run_unit_rows<false>(dtype, a, stream);
 }
@@ -313,7 +315,7 @@ int maxsim_amd_unit_rows_backward(maxsim_dtype dtype, const void* dy, int64_t dy
   if (!x || !dx || (!dy && !(offsets && packed_rows == 0)))
     return fail(MAXSIM_ERR_INVALID, "null pointer argument");
   const UnitRows a{x,       dy,          x_seq_stride, x_row_stride, dy_seq_stride, dy_row_stride,
-                   sequences, sequences * length, (int)length, (int)dim, lengths,
+                   sequences, sequences * length, 0, (int)length, (int)dim, lengths,
                    lengths64, offsets, packed_rows, eps, dx};
   return run_unit_rows<true>(dtype, a, stream);
 }
