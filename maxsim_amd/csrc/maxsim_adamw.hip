@@ -261,7 +261,9 @@ __device__ __forceinline__ void adam_chunk(const AdamArgs<BITS, MASTER>& a, int 
     // not depend on how a compiler contracts
     m[e] = m[e] * a.b1 + g[e] * a.r1;
     v[e] = v[e] * a.b2 + (g[e] * g[e]) * a.r2;
-    const float d = root_of(v[e]) * h.root + a.eps;
+    const float d = __builtin_fmaf(root_of(v[e]), h.root, a.eps);
+    // unfused too: a fused one is rounded to 16 bits in one step with the sum,
+    // and a parameter would no longer be its master's rounding
     p[e] = p[e] * h.keep - h.size * (m[e] * __builtin_amdgcn_rcpf(d));
     big_m = max(big_m, __float_as_uint(m[e]) & 0x7fffffffu);
     big_v = max(big_v, __float_as_uint(v[e]) & 0x7fffffffu);
