@@ -175,19 +175,25 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, min_8bit_size: int = 4096,
                  master_weights: bool = False, seed: int = 0):
-        if state_bits not in (8, 32):
-            raise ValueError(f"state_bits must be 8 or 32; got {state_bits}")
-        if not isinstance(lr, torch.Tensor) and not (lr >= 0.0 and math.isfinite(lr)):
-            raise ValueError(f"lr must be finite and >= 0; got {lr}")
-        for name, value in (("eps", eps), ("weight_decay", weight_decay)):
-            if not (value >= 0.0 and math.isfinite(value)):
-                raise ValueError(f"{name} must be finite and >= 0; got {value}")
-        if not all(0.0 <= b < 1.0 for b in betas):
-            raise ValueError(f"betas must be in [0, 1); got {tuple(betas)}")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
                                       weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_size=min_8bit_size,
                                       master_weights=master_weights, seed=seed))
+
+    def add_param_group(self, param_group) -> None:
+        """As torch's; a group's own options are checked like the defaults."""
+        group = {**self.defaults, **param_group}
+        if group["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32; got {group['state_bits']}")
+        for name in ("lr", "eps", "weight_decay"):
+            value = group[name]
+            if name == "lr" and isinstance(value, torch.Tensor):
+                continue  # on the device; checked where it is used, but for its value
+            if not (value >= 0.0 and math.isfinite(value)):
+                raise ValueError(f"{name} must be finite and >= 0; got {value}")
+        if len(group["betas"]) != 2 or not all(0.0 <= b < 1.0 for b in group["betas"]):
+            raise ValueError(f"betas must be two numbers in [0, 1); got {tuple(group['betas'])}")
+        super().add_param_group(param_group)
 
     def _new_state(self, p, group) -> dict:
         eight = group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]

@@ -466,6 +466,8 @@ def test_refusals():
                      (dict(weight_decay=-1), "weight_decay")):
         with pytest.raises(ValueError, match=text):
             maxsim_amd.AdamW([x.float().requires_grad_(True)], **kw)
+        with pytest.raises(ValueError, match=text):  # a group's own options too
+            maxsim_amd.AdamW([dict(params=[x.float().requires_grad_(True)], **kw)])
     p = torch.zeros(4, 8, device="cuda", requires_grad=True)
     p.grad = torch.ones(4, 8, device="cuda").to_sparse()
     with pytest.raises(RuntimeError, match="sparse"):
