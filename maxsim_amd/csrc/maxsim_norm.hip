@@ -127,7 +127,7 @@ __global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward 
   using S = typename T::storage;
   constexpr int V = kBackwardVec, GROUPS = row_threads(G) / G;
   constexpr int COLS = G * K * V;
-  // two chunks per lane of 1024 threads leave no registers for the next row
+  // four chunks per lane of 1024 threads leave no registers for the next row
   // and the weights (128 per lane): both are loaded where they are used
   constexpr bool AHEAD = G < 1024 || K == 1;
   __shared__ float part[2][G > 64 ? 2 * G / 64 : 1];
