@@ -83,20 +83,24 @@ def train(steps=200, batch=64, lq=32, ld=180, hidden=768, dim=128, dtype=torch.b
                                  state_bits=state_bits, master_weights=dtype != torch.float32)
     data = Batches(batch, lq, ld, hidden, dtype, seed)
     losses = []
-    for step in range(steps):
-        if step == 1:  # the first one loads kernels and fills allocators
-            began = time.perf_counter()
-        queries, documents, lengths = data.next()
-        q = head.queries(queries)
-        d, offsets = head.documents(documents, lengths)
-        loss = maxsim_amd.score_contrastive_cross_entropy(q, d, offsets, temperature=temperature)
-        optimizer.zero_grad()
-        loss.backward()
-        optimizer.step()
-        losses.append(loss.detach())
-        if report and step > 0 and (step + 1) % report == 0:
-            print(f"step {step + 1:5d}  loss {float(loss.detach()):.4f}  "
-                  f"{(time.perf_counter() - began) / step * 1e3:.2f} ms per step", flush=True)
+    # one GPU per process: backward on this thread saves the hand-over to the
+    # engine's, which costs more than the kernels of a small batch
+    with torch.autograd.set_multithreading_enabled(False):
+        for step in range(steps):
+            if step == 1:  # the first one loads kernels and fills allocators
+                began = time.perf_counter()
+            queries, documents, lengths = data.next()
+            q = head.queries(queries)
+            d, offsets = head.documents(documents, lengths)
+            loss = maxsim_amd.score_contrastive_cross_entropy(q, d, offsets,
+                                                              temperature=temperature)
+            optimizer.zero_grad()
+            loss.backward()
+            optimizer.step()
+            losses.append(loss.detach())
+            if report and step > 0 and (step + 1) % report == 0:
+                print(f"step {step + 1:5d}  loss {float(loss.detach()):.4f}  "
+                      f"{(time.perf_counter() - began) / step * 1e3:.2f} ms per step", flush=True)
     return torch.stack(losses).tolist()
 
 
