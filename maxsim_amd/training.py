@@ -77,6 +77,12 @@ def normalize_embeddings(x, lengths=None, *, eps: float = 1e-12) -> torch.Tensor
     return ops.maxsim_normalize_embeddings(x, lengths, eps)
 
 
+# The host waits in it; torch.compile runs it at a graph break.
+@torch.compiler.disable
+def _packed_layout(lengths, max_len: int):
+    return ops.maxsim_length_offsets(lengths, max_len)
+
+
 def pack_normalized_documents(doc_emb, doc_lengths, *,
                               eps: float = 1e-12) -> Tuple[torch.Tensor, torch.Tensor]:
     """:func:`maxsim_amd.pack_documents` of :func:`normalize_embeddings` in one
@@ -93,7 +99,7 @@ def pack_normalized_documents(doc_emb, doc_lengths, *,
         raise ValueError(
             f"doc_lengths must have shape [Nb={Nb}]; got {tuple(doc_lengths.shape)}")
     _require_hip("doc_emb", doc_emb)
-    lengths, offsets, total = ops.maxsim_length_offsets(
+    lengths, offsets, total = _packed_layout(
         doc_lengths.to(doc_emb.device, non_blocking=True), Ld)
     return ops.maxsim_pack_normalized(doc_emb, lengths, offsets, total, eps), offsets
 

@@ -276,6 +276,20 @@ def test_compiles():
     assert torch.equal(want[0], got[0])
 
 
+def test_packing_under_compile():
+    gen = torch.Generator().manual_seed(12)
+    x = rand(gen, 4, 6, 128).requires_grad_(True)
+    lengths = torch.tensor([6, 0, 2, 5], device="cuda")
+
+    def f(x):
+        docs, offsets = maxsim_amd.pack_normalized_documents(x * 3, lengths)
+        return (docs * docs[:1]).sum() + offsets.sum()
+
+    want = torch.autograd.grad(f(x), x)
+    got = torch.autograd.grad(torch.compile(f, backend="aot_eager")(x), x)
+    assert torch.equal(want[0], got[0])
+
+
 def test_refusals():
     x = torch.randn(4, 5, 64, device="cuda")
     ln = torch.tensor([1, 2, 3, 4], device="cuda")
