@@ -107,7 +107,6 @@ def pack_normalized_documents(doc_emb, doc_lengths, *,
 # ---------------------------------------------------------------------------
 # AdamW
 # ---------------------------------------------------------------------------
-@torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.9, 0.999),
                eps: float = 1e-8, weight_decay: float = 1e-2, scales=None, masters=None,
                seed: int = 0) -> None:
