@@ -115,23 +115,22 @@ struct LnBackward {
   float* partial;  // [gridDim.x][2][dim] sums of dy xh and dy; NULL: not wanted
 };
 
-// Four elements per chunk in either type: a lane of the backward holds five
-// arrays of its columns (x, dy, the weights and the two sums).
-constexpr int kBackwardVec = 4;
-
 // The rows in turn as in the forward; each lane adds up its columns' share of
 // dw and db over its rows, the workgroup joins its groups' (in one order) and
-// writes one partial row, which ln_weight_grad_kernel adds up.
+// writes one partial row, which ln_weight_grad_kernel adds up.  Chunks of 16
+// bytes cost 16-bit rows 200 registers, two waves per SIMD, and still win
+// (294912 x 768 bf16 235 us = 5.8 TB/s, in chunks of 8 bytes 255).
 template <typename T, typename W, int G, int K>
 __global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward a) {
   using S = typename T::storage;
-  constexpr int V = kBackwardVec, GROUPS = row_threads(G) / G;
+  constexpr int V = kVec<T>, GROUPS = row_threads(G) / G;
   constexpr int COLS = G * K * V;
-  // four chunks per lane of 1024 threads leave no registers for the next row
-  // and the weights (128 per lane): both are loaded where they are used
-  constexpr bool AHEAD = G < 1024 || K == 1;
+  // lanes of 1024 threads have 128 registers, too few for the next row and the
+  // weights besides: both are loaded where they are used (10000 x 8192 fp32 185
+  // us, with them kept 190)
+  constexpr bool AHEAD = G < 1024;
   __shared__ float part[2][G > 64 ? 2 * G / 64 : 1];
-  __shared__ float cols[G < 256 ? COLS : 1];
+  __shared__ alignas(16) float cols[G < 256 ? row_threads(G) / 64 : 1][G < 256 ? COLS : 4];
   const int j = threadIdx.x % G, group = threadIdx.x / G;
   const int dim = a.dim;
   const S* x = static_cast<const S*>(a.x);
@@ -216,33 +215,36 @@ __global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward 
   float* out = a.partial + (int64_t)blockIdx.x * 2 * dim;
   auto write = [&](float (&v)[K][V], float* to) {
     if constexpr (G < 256) {
-      // a wave's groups in registers, then one wave after the other
+      // a wave's groups in registers, the waves in LDS
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+      for (int k = 0; k < K; ++k) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[k][e] = groups_sum<G>(v[k][e]);
-      for (int wave = 0; wave < row_threads(G) / 64; ++wave) {
-        if ((int)threadIdx.x >> 6 == wave && (threadIdx.x & 63) < G) {
+        if ((threadIdx.x & 63) < G) {
 #pragma unroll
-          for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const int c = (j + k * G) * V + e;
-              cols[c] = wave == 0 ? v[k][e] : cols[c] + v[k][e];
-            }
+          for (int e = 0; e < V; ++e) cols[threadIdx.x >> 6][(j + k * G) * V + e] = v[k][e];
         }
-        __syncthreads();
       }
-      for (int c = threadIdx.x; c < dim; c += row_threads(G)) to[c] = cols[c];
+      __syncthreads();
+      for (int c = threadIdx.x; c < dim; c += row_threads(G)) {
+        float sum = cols[0][c];
+#pragma unroll
+        for (int wave = 1; wave < row_threads(G) / 64; ++wave) sum += cols[wave][c];
+        to[c] = sum;
+      }
       __syncthreads();
     } else {
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+      for (int k = 0; k < K; ++k) {
+        const int c = (j + k * G) * V;
+        if (c + V <= dim) {
+          __builtin_memcpy(to + c, v[k], sizeof v[k]);
+        } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const int c = (j + k * G) * V + e;
-          if (c < dim) to[c] = v[k][e];
+          for (int e = 0; e < V; ++e)
+            if (c + e < dim) to[c + e] = v[k][e];
         }
+      }
     }
   };
   write(dw, out);
@@ -262,8 +264,15 @@ __global__ __launch_bounds__(kGradCols * kGradSlices) void ln_weight_grad_kernel
   float s = 0.0f;
   if (c < dim) {
     const float* p = partial + (int64_t)which * dim + c;
-#pragma unroll 8
-    for (int i = slice; i < count; i += kGradSlices) s += p[(int64_t)i * 2 * dim];
+    // eight rows asked for at a time, also at the end
+    for (int i = slice; i < count; i += 8 * kGradSlices) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        v[u] = p[(int64_t)min(i + u * kGradSlices, count - 1) * 2 * dim];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += i + u * kGradSlices < count ? v[u] : 0.0f;
+    }
   }
   part[slice][col] = s;
   __syncthreads();
@@ -297,9 +306,8 @@ static int check_layer_norm(maxsim_dtype dtype, maxsim_dtype weight_dtype, int64
 // Workgroups take their rows in turn, with this turn's and the next's rows
 // asked for; how many there are per CU sets how much is in flight.  Past 32 KB
 // per CU (forward, one array) and 48 KB (backward, two) more only gets into
-// each other's way in the memory: 294912 x 768 bf16 backward 318 / 256 / 273 us
-// with 24 / 48 / 72 KB, 100000 x 768 fp32 161 / 177 us with 48 / 96 KB, 40000 x
-// 2560 bf16 137 / 121 us with 40 / 60 KB.
+// each other's way in the memory: 294912 x 768 bf16 backward 235 / 254 us with
+// 48 / 72 KB, 65000 x 1024 76 / 82, 100000 x 768 fp32 161 / 177 with 48 / 96.
 constexpr int64_t kForwardInFlight = 32 << 10, kBackwardInFlight = 48 << 10;
 static int workgroups_for(int64_t in_flight, int64_t bytes_each) {
   return (int)((in_flight + bytes_each - 1) / bytes_each);
@@ -308,9 +316,10 @@ static int workgroups_for(int64_t in_flight, int64_t bytes_each) {
 // Workgroups of the backward, at most kMaxPartials (what the workspace holds
 // partial rows for) and with at least kLeastTurns turns each where there are
 // more turns than CUs: a workgroup costs a partial row of 8 dim bytes, written
-// and read again.
+// and read again (4000 x 2048 bf16 15.0 us, with four turns 16.4; 16000 x 768
+// 18.8 with either).
 constexpr int64_t kMaxPartials = 1024;
-constexpr int64_t kLeastTurns = 4;
+constexpr int64_t kLeastTurns = 8;
 static int64_t backward_blocks(int64_t turns, int64_t cus, int64_t per_cu) {
   return std::min<int64_t>({turns, cus * per_cu, kMaxPartials,
                             std::max<int64_t>(cus, turns / kLeastTurns)});
@@ -319,7 +328,7 @@ static int64_t backward_blocks(int64_t turns, int64_t cus, int64_t per_cu) {
 template <typename F>
 static void with_backward(maxsim_dtype dtype, maxsim_dtype weight_dtype, int64_t dim, F&& f) {
   with_types(dtype, weight_dtype, [&](auto t, auto w) {
-    with_shape<kBackwardVec>(dim, [&](auto s) { f(t, w, s); });
+    with_shape<kVec<decltype(t)>>(dim, [&](auto s) { f(t, w, s); });
   });
 }
 
@@ -365,11 +374,10 @@ size_t maxsim_amd_layer_norm_backward_workspace_size(maxsim_dtype dtype, int64_t
                                                      int64_t dim) {
   if (rows <= 0 || dim <= 0 || dim > MAXSIM_AMD_MAX_DIM) return 0;
   int64_t turns = 0;
-  with_shape<kBackwardVec>(dim, [&](auto s) {
+  with_backward(dtype, dtype, dim, [&](auto, auto, auto s) {
     constexpr int groups = row_threads(decltype(s)::G) / decltype(s)::G;
     turns = (rows + groups - 1) / groups;
   });
-  (void)dtype;  // the shapes go by the elements
   return (size_t)std::min(turns, kMaxPartials) * 2 * dim * sizeof(float);
 }
 

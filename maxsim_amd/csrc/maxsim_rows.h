@@ -301,9 +301,10 @@ __device__ __forceinline__ void group_sums(float (&v)[N], float* part) {
 // MAXSIM_AMD_MAX_DIM) in chunks of V: the one that leaves fewest lanes idle
 // among those that hold a row in at most three chunks per lane; more lanes
 // than a wave where that is not enough.  (Rows of 768 elements of 16 bits, 96
-// chunks of 8: 32 lanes x 3.)  Wide rows in chunks of 4 are the layer norm's
-// backward: two workgroups of 512 threads on a CU work at each other's
-// barriers, of 1024 there is one (10000 x 8192 bf16: 100 against 123 us).
+// chunks of 8: 32 lanes x 3.)  512 threads where they hold a row:
+// two such workgroups on a CU work at each other's barriers (layer norm of 8000
+// x 12288 bf16 backward 122 us, with 1024 threads 137; 12000 x 8192 forward 72
+// against 75).
 template <int G_, int K_> struct Shape { static constexpr int G = G_, K = K_; };
 template <int V, typename F>
 inline void with_shape(int64_t dim, F&& f) {
@@ -319,15 +320,10 @@ inline void with_shape(int64_t dim, F&& f) {
   else if (chunks <= 256) f(Shape<256, 1>{});
   else if (chunks <= 512) f(Shape<256, 2>{});
   else if (chunks <= 768) f(Shape<256, 3>{});
-  else if constexpr (V == 8) {
-    if (chunks <= 1024) f(Shape<1024, 1>{});
-    else f(Shape<1024, 2>{});
-  } else {
-    if (chunks <= 1024) f(Shape<512, 2>{});
-    else if (chunks <= 1536) f(Shape<512, 3>{});
-    else if (chunks <= 2048) f(Shape<512, 4>{});
-    else f(Shape<1024, 4>{});
-  }
+  else if (chunks <= 1024) f(Shape<512, 2>{});
+  else if (chunks <= 1536) f(Shape<512, 3>{});
+  else if (V == 8 || chunks <= 2048) f(Shape<1024, 2>{});
+  else if constexpr (V < 8) f(Shape<1024, 4>{});
 }
 constexpr int row_threads(int G) { return G > 256 ? G : 256; }
 
