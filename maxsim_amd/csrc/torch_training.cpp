@@ -366,6 +366,35 @@ Tensor maxsim_pack_normalized_backward(const Tensor& dy, const Tensor& x, const 
 bool wants(const Tensor& t) { return t.requires_grad(); }
 bool wants(const optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
 
+// A backward's results where its caller records a graph through it
+// (create_graph): they hang on what they came from, and a second derivative
+// raises instead of counting as 0.
+struct OnlyOnce : torch::autograd::Function<OnlyOnce> {
+  static variable_list forward(AutogradContext*, const Tensor&, const Tensor&,
+                               const optional<Tensor>&, variable_list results) {
+    return results;
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "maxsim_amd: the gradient of this function has no derivative of its own");
+  }
+};
+
+// count: results and the arguments of the forward that have no gradient.
+variable_list backward_results(variable_list results, size_t count, const Tensor& dy,
+                               const Tensor& x, const optional<Tensor>& weight) {
+  if (at::GradMode::is_enabled()) {
+    variable_list defined;
+    for (const Tensor& t : results)
+      if (t.defined()) defined.push_back(t);
+    defined = OnlyOnce::apply(dy, x, weight, std::move(defined));
+    size_t next = 0;
+    for (Tensor& t : results)
+      if (t.defined()) t = defined[next++];
+  }
+  results.resize(count);
+  return results;
+}
+
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& weight,
                         const optional<Tensor>& bias, double eps) {
@@ -387,10 +416,14 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     const bool want_w = has_w && ctx->needs_input_grad(1);
     const bool want_b = has_b && ctx->needs_input_grad(1 + has_w);
     const optional<Tensor> weight = has_w ? optional<Tensor>(saved[1]) : std::nullopt;
-    auto [dx, dw, db] = MAXSIM_CALL(
-        maxsim_layer_norm_backward, grads[0], saved[0], saved[2], weight, want_x, want_w, want_b,
-        (at::ScalarType)ctx->saved_data["dtype"].toInt());
-    return {want_x ? dx : Tensor(), want_w ? dw : Tensor(), want_b ? db : Tensor(), Tensor()};
+    const auto run = [&] {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      return MAXSIM_CALL(maxsim_layer_norm_backward, grads[0], saved[0], saved[2], weight, want_x,
+                         want_w, want_b, (at::ScalarType)ctx->saved_data["dtype"].toInt());
+    };
+    auto [dx, dw, db] = run();
+    return backward_results({want_x ? dx : Tensor(), want_w ? dw : Tensor(), want_b ? db : Tensor()},
+                            4, grads[0], saved[0], weight);
   }
 };
 
@@ -414,9 +447,12 @@ struct NormalizeFn : torch::autograd::Function<NormalizeFn> {
     const auto saved = ctx->get_saved_variables();
     const optional<Tensor> lengths =
         saved[1].defined() ? optional<Tensor>(saved[1]) : std::nullopt;
-    return {MAXSIM_CALL(maxsim_normalize_embeddings_backward, grads[0], saved[0], lengths,
-                        ctx->saved_data["eps"].toDouble()),
-            Tensor(), Tensor()};
+    const auto run = [&] {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      return MAXSIM_CALL(maxsim_normalize_embeddings_backward, grads[0], saved[0], lengths,
+                         ctx->saved_data["eps"].toDouble());
+    };
+    return backward_results({run()}, 3, grads[0], saved[0], std::nullopt);
   }
 };
 
@@ -436,9 +472,12 @@ struct PackNormalizedFn : torch::autograd::Function<PackNormalizedFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    return {MAXSIM_CALL(maxsim_pack_normalized_backward, grads[0], saved[0], saved[1], saved[2],
-                        ctx->saved_data["eps"].toDouble()),
-            Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto run = [&] {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      return MAXSIM_CALL(maxsim_pack_normalized_backward, grads[0], saved[0], saved[1], saved[2],
+                         ctx->saved_data["eps"].toDouble());
+    };
+    return backward_results({run()}, 5, grads[0], saved[0], std::nullopt);
   }
 };
 

@@ -274,3 +274,16 @@ def test_refusals():
     for error, text, f in cases:
         with pytest.raises(error, match=text):
             f()
+
+
+@pytest.mark.parametrize("of", ["x", "weight", "bias"])
+def test_a_second_derivative_raises(of):
+    leaves = {"x": torch.randn(5, 64, device="cuda", requires_grad=True),
+              "weight": torch.ones(64, device="cuda", requires_grad=True),
+              "bias": torch.zeros(64, device="cuda", requires_grad=True)}
+    y = maxsim_amd.layer_norm(*leaves.values())
+    once, = torch.autograd.grad(y.square().sum(), leaves[of], retain_graph=True)
+    grad, = torch.autograd.grad(y.square().sum(), leaves[of], create_graph=True)
+    assert torch.equal(once, grad)
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.autograd.grad(grad.square().sum(), leaves["x"])

@@ -313,3 +313,17 @@ def test_refusals():
     for error, text, f in cases:
         with pytest.raises(error, match=text):
             f()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_second_derivative_raises(packed):
+    x = torch.randn(4, 6, 64, device="cuda", requires_grad=True)
+    lengths = torch.tensor([1, 6, 0, 3], device="cuda")
+    y = (maxsim_amd.pack_normalized_documents(x, lengths)[0] if packed
+         else maxsim_amd.normalize_embeddings(x, lengths))
+    down = torch.randn_like(y)
+    once, = torch.autograd.grad(y, x, down, retain_graph=True)
+    grad, = torch.autograd.grad(y, x, down, create_graph=True)
+    assert torch.equal(once, grad)
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.autograd.grad(grad.square().sum(), x)
