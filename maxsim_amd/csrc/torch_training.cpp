@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <map>
 #include <optional>
 #include <tuple>
@@ -556,6 +557,8 @@ void maxsim_adamw_step(at::TensorList params, at::TensorList grads, at::TensorLi
   // tensors of one (parameter, gradient) type go together
   std::map<std::pair<maxsim_dtype, maxsim_dtype>, std::vector<maxsim_adamw_tensor>> groups;
   std::vector<Tensor> copies;  // gradients in their parameters' order
+  std::vector<std::pair<const char*, size_t>> places;  // where the parameters lie
+  places.reserve(n);
   uint64_t position = 0;
   for (size_t i = 0; i < n; ++i) {
     const Tensor& p = params[i];
@@ -601,6 +604,13 @@ void maxsim_adamw_step(at::TensorList params, at::TensorList grads, at::TensorLi
          eight ? scales[i].data_ptr<uint8_t>() : nullptr,
          masters.empty() ? nullptr : masters[i].data_ptr<float>(), numel, position});
     position += (uint64_t)blocks * MAXSIM_AMD_STATE_BLOCK;
+    if (numel > 0) places.emplace_back(static_cast<const char*>(p.data_ptr()), i);
+  }
+  std::sort(places.begin(), places.end());
+  for (size_t k = 1; k < places.size(); ++k) {
+    const auto& [at, i] = places[k - 1];
+    TORCH_CHECK_VALUE(at + params[i].nbytes() <= places[k].first, "params[", i, "] and params[",
+                      places[k].second, "] share memory");
   }
   c10::hip::HIPGuardMasqueradingAsCUDA guard(params[0].device());
   for (const auto& [types, tensors] : groups)

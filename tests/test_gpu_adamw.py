@@ -472,3 +472,23 @@ def test_refusals():
     p.grad = torch.ones(4, 8, device="cuda").to_sparse()
     with pytest.raises(RuntimeError, match="sparse"):
         maxsim_amd.AdamW([p]).step()
+
+
+def test_refuses_parameters_that_share_memory():
+    # in one launch their blocks would run over each other
+    flat = torch.zeros(700, device="cuda")
+    for a, b in ((slice(0, 300), slice(0, 300)), (slice(0, 300), slice(299, 700))):
+        t = _make([300, b.stop - b.start], torch.float32, torch.float32, 32, False, seed=4)
+        t["params"] = [flat[b], flat[a]] if a != b else [flat[a], flat[a]]
+        if a != b:
+            for key in ("grads", "exp_avgs", "exp_avg_sqs"):
+                t[key] = t[key][::-1]
+        with pytest.raises(ValueError, match="share memory"):
+            _step(t)
+    # neighbours in one buffer and empty parameters do not
+    t = _make([300, 400], torch.float32, torch.float32, 32, False, seed=4)
+    t["params"] = [flat[:300], flat[300:]]
+    for key in ("params", "grads", "exp_avgs", "exp_avg_sqs"):
+        t[key] += [torch.zeros(0, device="cuda"), torch.zeros(0, device="cuda")]
+    _step(t)
+    assert flat.isfinite().all() and flat.count_nonzero() > 650
