@@ -101,7 +101,8 @@ typedef struct {
 } maxsim_adamw_tensor;
 
 /* One AdamW step with decoupled weight decay over `count` tensors (host array,
- * read before the call returns):
+ * read before the call returns; nothing that one of them updates overlaps
+ * another's):
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = p (1 - lr weight_decay)
  *       - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps).
