@@ -9,6 +9,7 @@
 #include <ATen/core/CachingHostAllocator.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -367,6 +368,16 @@ Tensor maxsim_pack_normalized_backward(const Tensor& dy, const Tensor& x, const 
 bool wants(const Tensor& t) { return t.requires_grad(); }
 bool wants(const optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
 
+// No function here carries forward-mode tangents, and one that is dropped on
+// the way would count as 0.
+void refuse_tangents(const char* name, const Tensor& a, const optional<Tensor>& b = std::nullopt,
+                     const optional<Tensor>& c = std::nullopt) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  const auto has = [](const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); };
+  TORCH_CHECK_NOT_IMPLEMENTED(!has(a) && !(b.has_value() && has(*b)) && !(c.has_value() && has(*c)),
+                              "maxsim_amd: ", name, " has no derivative in forward mode");
+}
+
 // A backward's results where its caller records a graph through it
 // (create_graph): they hang on what they came from, and a second derivative
 // raises instead of counting as 0.
@@ -430,6 +441,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
 
 Tensor layer_norm_autograd(const Tensor& x, const optional<Tensor>& weight,
                            const optional<Tensor>& bias, double eps) {
+  refuse_tangents("layer_norm", x, weight, bias);
   if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias)))
     return LayerNormFn::apply(x, weight, bias, eps);
   at::AutoDispatchBelowADInplaceOrView guard;
@@ -458,6 +470,7 @@ struct NormalizeFn : torch::autograd::Function<NormalizeFn> {
 };
 
 Tensor normalize_autograd(const Tensor& x, const optional<Tensor>& lengths, double eps) {
+  refuse_tangents("normalize_embeddings", x);
   if (at::GradMode::is_enabled() && wants(x)) return NormalizeFn::apply(x, lengths, eps);
   at::AutoDispatchBelowADInplaceOrView guard;
   return MAXSIM_CALL(maxsim_normalize_embeddings, x, lengths, eps);
@@ -484,6 +497,7 @@ struct PackNormalizedFn : torch::autograd::Function<PackNormalizedFn> {
 
 Tensor pack_normalized_autograd(const Tensor& x, const Tensor& lengths, const Tensor& offsets,
                                 int64_t packed_rows, double eps) {
+  refuse_tangents("pack_normalized_documents", x);
   if (at::GradMode::is_enabled() && wants(x))
     return PackNormalizedFn::apply(x, lengths, offsets, packed_rows, eps);
   at::AutoDispatchBelowADInplaceOrView guard;

@@ -10,9 +10,10 @@ hidden states to scored token embeddings, and the step that trains both.
 
 The reference leaves these to torch (its training example, README.md:160-205).
 Here they are hand-written HIP kernels behind ``include/maxsim_amd_training.h``:
-one pass over memory each, sums in fp32, 16-bit results rounded once.  The
-gradients have no derivatives of their own (a second derivative raises).  All
-are exported from :mod:`maxsim_amd`.
+one pass over memory each, sums in fp32, 16-bit results rounded once.
+Differentiable means first derivatives in reverse mode: the gradients have no
+derivatives of their own and forward-mode tangents are not carried (both raise).
+All are exported from :mod:`maxsim_amd`.
 """
 
 from __future__ import annotations
