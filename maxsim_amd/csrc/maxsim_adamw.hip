@@ -1,7 +1,8 @@
 // The AdamW step over many tensors at once, with states in 32 or 8 bits.
 //
 //   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
-//   p = p (1 - lr decay) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//   p = p (1 - lr decay) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps),
+//       the two things that leave p added up before the one subtraction
 //
 // Memory-bound: 28 bytes per element in fp32, 10 in bf16 with 8-bit states.
 // A launch takes up to kTensors tensors by their addresses in its arguments
@@ -63,12 +64,13 @@ template <int BITS, bool MASTER> struct AdamArgs {
   uint32_t block[BITS == 8 ? kTensors : 1];  // position of element 0, in blocks
   uint32_t first[kTensors];                  // chunk number of element 0
   int count;
-  float lr, decay, b1, r1, b2, r2, eps;  // r: 1 - b
+  float lr, decay, b1, r1, b2, r2, eps;  // decay: lr weight_decay; r: 1 - b
   float c1, c2;                          // 1 - b^t
   uint32_t key;
   // read on the device where given: the learning rate, and the step count
   const float* lr_at;
   const int64_t* step_at;
+  float weight_decay;
   double beta1, beta2;
   uint64_t seed;
 };
@@ -220,7 +222,7 @@ __device__ __forceinline__ uint2 top_bytes(const uint32_t (&q)[8]) {
 }
 
 struct AdamStep {
-  float keep, size, root;  // 1 - lr decay, lr / c1, 1 / sqrt(c2)
+  float decay, size, root;  // lr weight_decay, lr / c1, 1 / sqrt(c2)
   uint32_t key;
 };
 
@@ -262,9 +264,14 @@ __device__ __forceinline__ void adam_chunk(const AdamArgs<BITS, MASTER>& a, int 
     m[e] = m[e] * a.b1 + g[e] * a.r1;
     v[e] = v[e] * a.b2 + (g[e] * g[e]) * a.r2;
     const float d = __builtin_fmaf(root_of(v[e]), h.root, a.eps);
-    // unfused too: a fused one is rounded to 16 bits in one step with the sum,
-    // and a parameter would no longer be its master's rounding
-    p[e] = p[e] * h.keep - h.size * (m[e] * __builtin_amdgcn_rcpf(d));
+    // All that leaves p in one number, then one subtraction and its rounding:
+    // p (1 - lr decay) first would round twice at p's spacing, and 1 - lr decay
+    // itself to steps of 2^-24 (lr decay = 5e-8 decayed 1.6 times as much, 2e-8
+    // not at all).  The clamp keeps an infinite p from becoming inf - inf.  The
+    // subtraction stays one of its own: fused with a product it is rounded to
+    // 16 bits in one step, and a parameter is no longer its master's rounding.
+    const float finite = __builtin_amdgcn_fmed3f(p[e], -__FLT_MAX__, __FLT_MAX__);
+    p[e] -= __builtin_fmaf(h.decay, finite, h.size * (m[e] * __builtin_amdgcn_rcpf(d)));
     big_m = max(big_m, __float_as_uint(m[e]) & 0x7fffffffu);
     big_v = max(big_v, __float_as_uint(v[e]) & 0x7fffffffu);
   }
@@ -307,9 +314,9 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs<BITS, MAST
 #pragma unroll
   for (int i = 0; i < AdamArgs<BITS, MASTER>::kTensors; i += 64)
     k += __popcll(__ballot(i + lane < a.count && a.first[min(i + lane, a.count - 1)] <= chunk));
-  float lr = a.lr, c1 = a.c1, c2 = a.c2;
+  float lr = a.lr, decay = a.decay, c1 = a.c1, c2 = a.c2;
   uint32_t key = a.key;
-  if (a.lr_at) lr = *a.lr_at;
+  if (a.lr_at) lr = *a.lr_at, decay = lr * a.weight_decay;
   if (a.step_at) {
     __shared__ float c[2];
     const int64_t step = *a.step_at;
@@ -319,7 +326,7 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs<BITS, MAST
     c1 = c[0], c2 = c[1];
     key = dither_key(a.seed, (uint64_t)step);
   }
-  const AdamStep h{1.0f - lr * a.decay, lr / c1, 1.0f / sqrtf(c2), key};
+  const AdamStep h{decay, lr / c1, 1.0f / sqrtf(c2), key};
   const int64_t base = (int64_t)(chunk - a.first[k]) * kChunkElems;
   if (base + kChunkElems <= a.n[k]) adam_chunk<P, Gr, BITS, MASTER, true>(a, k, h, base);
   else adam_chunk<P, Gr, BITS, MASTER, false>(a, k, h, base);
@@ -395,7 +402,8 @@ int maxsim_amd_adamw_step(maxsim_dtype param_dtype, maxsim_dtype grad_dtype, int
     using Args = AdamArgs<BITS, MASTER>;
     Args a{};
     a.lr = (float)lr;
-    a.decay = (float)weight_decay;
+    a.decay = (float)(lr * weight_decay);
+    a.weight_decay = (float)weight_decay;
     a.b1 = (float)beta1, a.r1 = (float)(1.0 - beta1);
     a.b2 = (float)beta2, a.r2 = (float)(1.0 - beta2);
     a.eps = (float)eps;

@@ -132,7 +132,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
         masters: fp32 tensors that 16-bit parameters are the rounding of; the
             step is taken on them.  Without them a 16-bit parameter is read,
             moved in fp32 and rounded to nearest, which loses steps smaller
-            than half its spacing.
+            than half its spacing.  (What a step takes off an fp32 value,
+            update and decay together, is rounded once, to the value's
+            spacing.)
         seed: of the random rounding of 8-bit states, which depends on
             (seed, step, position of the element in the lists) alone.
 

@@ -1,0 +1,99 @@
+"""maxsim_amd.adamw_step over many steps, at the limits of a launch and with
+memory that is shared, beside test_gpu_adamw.py's single steps."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import training_oracle as oracle
+
+from ._training_helpers import U32, f64
+from .test_gpu_adamw import HYPER, _clone, _make, _step
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- weight decay ------------------------------------------------------------
+DECAY_FORMS = {
+    "fp32": {},
+    "fp32, rate on the device": dict(device_lr=True),
+    "fp32, 8-bit states": dict(bits=8),
+    "bf16 with masters": dict(dtype=torch.bfloat16, master=True),
+}
+
+
+@pytest.mark.parametrize("lr", [2e-6, 5e-6, 1e-5])
+@pytest.mark.parametrize("form", DECAY_FORMS)
+def test_small_weight_decay_adds_up(form, lr):
+    """lr * weight_decay of 2e-8 to 1e-7, near the spacing of fp32 below 1.  Two
+    copies of the parameters get gradients of opposite sign, so that their mean
+    moves by the decay alone: p0 (1 - lr decay)^t.  Each step rounds an element
+    once, by at most half of 2^-28 (the elements stay below 2^-4), independently
+    as long as the gradients are; 65536 pairs and 1000 steps leave a thousandth
+    of the decay of that at six sigma, and the decay's own product and sum are
+    good to 1e-6."""
+    opt = dict(dtype=torch.float32, bits=32, master=False, device_lr=False)
+    opt.update(DECAY_FORMS[form])
+    n, steps, decay = 65536, 1000, 0.01
+    gen = torch.Generator().manual_seed(1)
+    start = torch.rand(n, generator=gen) * 0.05 + 0.01
+    sides = []
+    for _ in range(2):
+        t = _make([n], opt["dtype"], opt["dtype"], opt["bits"], opt["master"], seed=2)
+        for key in ("exp_avgs", "exp_avg_sqs", "scales"):
+            for x in t[key]:
+                x.zero_()
+        t["params"][0].copy_(start)
+        if opt["master"]:
+            t["masters"][0].copy_(start)
+        sides.append(t)
+    rate = torch.full((1,), lr, device="cuda") if opt["device_lr"] else lr
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for step in range(steps):
+        noise = torch.randn(n, generator=gen, device="cuda").to(opt["dtype"])
+        for t, sign in zip(sides, (1, -1)):
+            t["grads"][0] = sign * noise
+            _step(t, step=step + 1, lr=rate, weight_decay=decay)
+    held = "masters" if opt["master"] else "params"
+    assert max(float(t[held][0].abs().max()) for t in sides) < 2.0 ** -4
+    got = np.mean([f64(t[held][0]).mean() for t in sides]) - f64(start).mean()
+    want = f64(start).mean() * ((1 - lr * decay) ** steps - 1)
+    sigma = 2.0 ** -28 / np.sqrt(12) * np.sqrt(steps / (2 * n))
+    assert abs(got - want) <= 6 * sigma + 1e-3 * abs(want), (got / want, sigma)
+
+
+@pytest.mark.parametrize("lr,decay", [(2e-6, 0.01), (1e-4, 0.1), (3e-3, 0.1), (0.5, 1.0)])
+@pytest.mark.parametrize("master", [False, True])
+def test_a_step_rounds_the_parameter_once(master, lr, decay):
+    # half a spacing of the result, and the errors of what is subtracted: the
+    # update's as in test_gpu_adamw.py and a few roundings of the two parts
+    dtype = torch.bfloat16 if master else torch.float32
+    t = _make([70001], dtype, dtype, 32, master, seed=4)
+    held = "masters" if master else "params"
+    p, g, m, v = (f64(t[k][0]) for k in (held, "grads", "exp_avgs", "exp_avg_sqs"))
+    b1, b2 = HYPER["betas"]
+    want, wm, wv = oracle.adamw(p, g, m, v, 7, lr, b1, b2, HYPER["eps"], decay)
+    _step(t, step=7, lr=lr, weight_decay=decay)
+    em = 4 * U32 * (b1 * np.abs(m) + (1 - b1) * np.abs(g))
+    moved = lr / (1 - b1 ** 7) / (np.sqrt(wv / (1 - b2 ** 7)) + HYPER["eps"])
+    bound = (np.spacing((np.abs(want) * (1 + 2.0 ** -22)).astype(np.float32)).astype(float) / 2
+             + moved * (em + 32 * U32 * np.abs(wm)) + 4 * U32 * lr * decay * np.abs(p))
+    assert (np.abs(f64(t[held][0]) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("decay", [0.0, 0.1])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_parameters_that_are_not_finite_stay_so(value, decay):
+    # p (1 - lr decay) of an infinity is the infinity, and its neighbours do not see it
+    for bits in (32, 8):
+        t = _make([600], torch.float32, torch.float32, bits, False, seed=3)
+        clean = _clone(t)
+        _step(clean, weight_decay=decay)
+        t["params"][0][300] = value
+        _step(t, weight_decay=decay)
+        keep = torch.arange(600, device="cuda") != 300
+        assert torch.equal(t["params"][0][keep], clean["params"][0][keep])
+        got = float(t["params"][0][300])
+        assert got == value or (got != got and value != value)
