@@ -541,6 +541,41 @@ const Tensor* device_scalar(const optional<Tensor>& t, const char* name, at::Sca
   return &*t;
 }
 
+// Where a tensor of a step's lists lies; of a gradient, which is only read,
+// or of one that is updated.
+struct Place {
+  uintptr_t begin, end;
+  uint32_t list, index;
+  bool operator<(const Place& o) const { return begin < o.begin; }
+};
+constexpr const char* kLists[] = {"params", "grads", "exp_avgs", "exp_avg_sqs", "scales", "masters"};
+constexpr uint32_t kGradList = 1;
+
+// Nothing that is updated shares memory with anything else: workgroups of one
+// launch would write over each other.  Lists mostly lie in memory as they were
+// allocated, one tensor after the other, so that each is merged as it is.
+void check_places(std::vector<Place> (&lists)[6]) {
+  std::vector<Place> all;
+  for (std::vector<Place>& list : lists) {
+    if (!std::is_sorted(list.begin(), list.end())) std::sort(list.begin(), list.end());
+    const auto before = (ptrdiff_t)all.size();
+    all.insert(all.end(), list.begin(), list.end());
+    std::inplace_merge(all.begin(), all.begin() + before, all.end());
+  }
+  const Place none{};
+  const Place *written = &none, *read = &none;  // those that reach farthest
+  for (const Place& p : all) {
+    const bool reads = p.list == kGradList;
+    const Place* met = p.begin < written->end          ? written
+                       : !reads && p.begin < read->end ? read
+                                                       : nullptr;
+    TORCH_CHECK_VALUE(!met, kLists[met->list], "[", met->index, "] and ", kLists[p.list], "[",
+                      p.index, "] share memory");
+    if (!reads) written = &p;
+    else if (p.end > read->end) read = &p;
+  }
+}
+
 void maxsim_adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs,
                        at::TensorList exp_avg_sqs, at::TensorList scales, at::TensorList masters,
                        double lr, const optional<Tensor>& lr_tensor, double beta1, double beta2,
@@ -571,8 +606,12 @@ void maxsim_adamw_step(at::TensorList params, at::TensorList grads, at::TensorLi
   // tensors of one (parameter, gradient) type go together
   std::map<std::pair<maxsim_dtype, maxsim_dtype>, std::vector<maxsim_adamw_tensor>> groups;
   std::vector<Tensor> copies;  // gradients in their parameters' order
-  std::vector<std::pair<const char*, size_t>> places;  // where the parameters lie
-  places.reserve(n);
+  std::vector<Place> places[6];
+  for (auto& list : places) list.reserve(n);
+  const auto place = [&](uint32_t list, const void* at, int64_t bytes, size_t i) {
+    const auto begin = reinterpret_cast<uintptr_t>(at);
+    places[list].push_back({begin, begin + (uintptr_t)bytes, list, (uint32_t)i});
+  };
   uint64_t position = 0;
   for (size_t i = 0; i < n; ++i) {
     const Tensor& p = params[i];
@@ -613,19 +652,29 @@ void maxsim_adamw_step(at::TensorList params, at::TensorList grads, at::TensorLi
       TORCH_CHECK_TYPE(dt != MAXSIM_FLOAT32, "params[", i, "] is float32 and takes no master");
       check_partner(masters[i], "masters", p, at::kFloat, (int64_t)i);
     }
-    groups[{dt, dtype_of(g, "grads")}].push_back(
-        {p.data_ptr(), g.data_ptr(), exp_avgs[i].data_ptr(), exp_avg_sqs[i].data_ptr(),
-         eight ? scales[i].data_ptr<uint8_t>() : nullptr,
-         masters.empty() ? nullptr : masters[i].data_ptr<float>(), numel, position});
+    const maxsim_adamw_tensor t{p.data_ptr(), g.data_ptr(), exp_avgs[i].data_ptr(),
+                                exp_avg_sqs[i].data_ptr(),
+                                eight ? scales[i].data_ptr<uint8_t>() : nullptr,
+                                masters.empty() ? nullptr : masters[i].data_ptr<float>(), numel,
+                                position};
+    groups[{dt, dtype_of(g, "grads")}].push_back(t);
     position += (uint64_t)blocks * MAXSIM_AMD_STATE_BLOCK;
-    if (numel > 0) places.emplace_back(static_cast<const char*>(p.data_ptr()), i);
+    if (numel == 0) continue;
+    const int64_t held = numel * (int64_t)p.element_size(), f32 = 4 * numel;
+    place(0, t.param, held, i);
+    place(2, t.exp_avg, eight ? numel : f32, i);
+    place(3, t.exp_avg_sq, eight ? numel : f32, i);
+    if (eight) place(4, t.scales, 2 * blocks, i);
+    if (t.master) place(5, t.master, f32, i);
+    // a thread has read its elements before it writes them: a gradient may be
+    // a tensor of its own type that its parameter's step updates
+    const bool wide = g.scalar_type() == at::kFloat, alike = g.scalar_type() == p.scalar_type();
+    const bool own = (alike && t.grad == t.param) ||
+                     (wide && t.grad == t.master) ||
+                     (wide && !eight && (t.grad == t.exp_avg || t.grad == t.exp_avg_sq));
+    if (!own) place(kGradList, t.grad, alike ? held : f32, i);
   }
-  std::sort(places.begin(), places.end());
-  for (size_t k = 1; k < places.size(); ++k) {
-    const auto& [at, i] = places[k - 1];
-    TORCH_CHECK_VALUE(at + params[i].nbytes() <= places[k].first, "params[", i, "] and params[",
-                      places[k].second, "] share memory");
-  }
+  check_places(places);
   c10::hip::HIPGuardMasqueradingAsCUDA guard(params[0].device());
   for (const auto& [types, tensors] : groups)
     check_status(maxsim_amd_adamw_step(

@@ -120,7 +120,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
 
     Args:
         params: fp32 / fp16 / bf16 tensors on one device, each dense in memory
-            in any order of its axes; no two share memory (ValueError).
+            in any order of its axes.  Nothing that the step updates may
+            share memory with another tensor of the lists (ValueError).
         grads: their gradients, in the parameter's dtype or fp32.
         exp_avgs, exp_avg_sqs: the states, in the parameters' order in memory:
             fp32, or uint8 codes with ``scales``.

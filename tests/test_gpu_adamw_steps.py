@@ -97,3 +97,83 @@ def test_parameters_that_are_not_finite_stay_so(value, decay):
         assert torch.equal(t["params"][0][keep], clean["params"][0][keep])
         got = float(t["params"][0][300])
         assert got == value or (got != got and value != value)
+
+
+# ---- memory that is shared ---------------------------------------------------
+def _shared(bits=32, master=False):
+    dtype = torch.bfloat16 if master else torch.float32
+    return _make([300, 700, 300], dtype, dtype, bits, master, seed=5)
+
+
+def _put(key, i, value):
+    return lambda t: t[key].__setitem__(i, value(t))
+
+
+SHARED = [
+    ("one state for all", {}, lambda t: t.update(exp_avgs=[t["exp_avgs"][0], t["exp_avgs"][1],
+                                                          t["exp_avgs"][0]])),
+    ("second moments", {}, _put("exp_avg_sqs", 2, lambda t: t["exp_avg_sqs"][0])),
+    ("both moments of a parameter", {}, _put("exp_avg_sqs", 0, lambda t: t["exp_avgs"][0])),
+    ("moments of two parameters", {}, _put("exp_avg_sqs", 2, lambda t: t["exp_avgs"][0])),
+    ("a moment and a parameter", {}, _put("exp_avgs", 2, lambda t: t["params"][0])),
+    ("a moment inside another", {}, _put("exp_avgs", 0, lambda t: t["exp_avgs"][1][200:500])),
+    ("8-bit codes", dict(bits=8), _put("exp_avgs", 2, lambda t: t["exp_avgs"][0])),
+    ("8-bit codes of both moments", dict(bits=8), _put("exp_avg_sqs", 1, lambda t: t["exp_avgs"][1])),
+    ("codes in the gradient", dict(bits=8),
+     _put("exp_avgs", 1, lambda t: t["grads"][1].view(torch.uint8)[:700])),
+    ("scales", dict(bits=8), _put("scales", 2, lambda t: t["scales"][0])),
+    ("scales inside others", dict(bits=8), _put("scales", 0, lambda t: t["scales"][1][1:])),
+    ("masters", dict(master=True), _put("masters", 2, lambda t: t["masters"][0])),
+    ("a master and a moment", dict(master=True), _put("masters", 2, lambda t: t["exp_avgs"][0])),
+    ("a gradient in another's parameter", {}, _put("grads", 2, lambda t: t["params"][0])),
+    ("a gradient across its parameter", {},
+     lambda t: t.update(params=[t["params"][1][:300]], grads=[t["params"][1][1:301]],
+                        exp_avgs=t["exp_avgs"][:1], exp_avg_sqs=t["exp_avg_sqs"][:1])),
+]
+
+
+@pytest.mark.parametrize("case", SHARED, ids=lambda c: c[0])
+def test_refuses_what_it_updates_to_share_memory(case):
+    # workgroups of one launch would write over each other, or read what
+    # another has already moved
+    _, make, change = case
+    t = _shared(**make)
+    change(t)
+    before = _clone(t)
+    with pytest.raises(ValueError, match="share memory"):
+        _step(t)
+    assert all(torch.equal(a, b) for k in t for a, b in zip(before[k], t[k]))
+
+
+def test_takes_gradients_that_share_memory():
+    # they are only read; one may also be its own parameter, or its own moment
+    t = _shared()
+    want = _clone(t)
+    want["grads"][2] = want["grads"][0].clone()
+    _step(want)
+    t["grads"][2] = t["grads"][0]
+    _step(t)
+    assert all(torch.equal(a, b) for k in ("params", "exp_avgs") for a, b in zip(want[k], t[k]))
+    t = _shared()
+    want = _clone(t)
+    want["grads"] = [want["params"][0].clone(), want["exp_avgs"][1].clone(), want["grads"][2]]
+    _step(want)
+    t["grads"] = [t["params"][0], t["exp_avgs"][1], t["grads"][2]]
+    _step(t)
+    assert all(torch.equal(a, b) for k in ("params", "exp_avgs") for a, b in zip(want[k], t[k]))
+
+
+def test_neighbours_in_one_buffer_do_not_share():
+    # everything in one allocation, in any order
+    t = _shared()
+    want = _clone(t)
+    _step(want)
+    flat = torch.empty(4 * 1300, device="cuda")
+    at = 4 * 1300
+    for k in ("exp_avg_sqs", "params", "grads", "exp_avgs"):
+        for i in (1, 0, 2):
+            at -= t[k][i].numel()
+            flat[at:at + t[k][i].numel()] = t[k][i]
+            t[k][i] = flat[at:at + t[k][i].numel()]
+    _step(t)
+    assert all(torch.equal(a, b) for k in want for a, b in zip(want[k], t[k]))
