@@ -556,6 +556,9 @@ constexpr uint32_t kGradList = 1;
 // allocated, one tensor after the other, so that each is merged as it is.
 void check_places(std::vector<Place> (&lists)[6]) {
   std::vector<Place> all;
+  size_t count = 0;
+  for (const std::vector<Place>& list : lists) count += list.size();
+  all.reserve(count);
   for (std::vector<Place>& list : lists) {
     if (!std::is_sorted(list.begin(), list.end())) std::sort(list.begin(), list.end());
     const auto before = (ptrdiff_t)all.size();
@@ -604,7 +607,10 @@ void maxsim_adamw_step(at::TensorList params, at::TensorList grads, at::TensorLi
 
   at::AutoDispatchBelowADInplaceOrView below;  // a gradient's copy records nothing
   // tensors of one (parameter, gradient) type go together
-  std::map<std::pair<maxsim_dtype, maxsim_dtype>, std::vector<maxsim_adamw_tensor>> groups;
+  using Types = std::pair<maxsim_dtype, maxsim_dtype>;
+  std::map<Types, std::vector<maxsim_adamw_tensor>> groups;
+  Types of{};  // of the tensor before, whose group is `group`
+  std::vector<maxsim_adamw_tensor>* group = nullptr;
   std::vector<Tensor> copies;  // gradients in their parameters' order
   std::vector<Place> places[6];
   for (auto& list : places) list.reserve(n);
@@ -657,7 +663,13 @@ void maxsim_adamw_step(at::TensorList params, at::TensorList grads, at::TensorLi
                                 eight ? scales[i].data_ptr<uint8_t>() : nullptr,
                                 masters.empty() ? nullptr : masters[i].data_ptr<float>(), numel,
                                 position};
-    groups[{dt, dtype_of(g, "grads")}].push_back(t);
+    const Types types{dt, dtype_of(g, "grads")};
+    if (!group || types != of) {
+      of = types;
+      group = &groups[types];
+      group->reserve(n);
+    }
+    group->push_back(t);
     position += (uint64_t)blocks * MAXSIM_AMD_STATE_BLOCK;
     if (numel == 0) continue;
     const int64_t held = numel * (int64_t)p.element_size(), f32 = 4 * numel;
