@@ -295,6 +295,23 @@ __device__ __forceinline__ void group_sums(float (&v)[N], float* part) {
   }
 }
 
+// Largest over a group of G lanes, in every lane (wider groups through G / 64
+// words of LDS, between barriers of its own).
+template <int G>
+__device__ __forceinline__ uint32_t group_max(uint32_t v, uint32_t* part) {
+#pragma unroll
+  for (int off = 1; off < (G < 64 ? G : 64); off <<= 1) v = max(v, __shfl_xor(v, off, 64));
+  if constexpr (G > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < G / 64; ++w) v = max(v, part[w]);
+    __syncthreads();
+  }
+  return v;
+}
+
 // ---- the shapes (host) -----------------------------------------------------
 
 // Calls f with the group shape for rows of `dim` elements (up to

@@ -11,8 +11,11 @@
 // Memory-bound: each row is read once into one group of lanes
 // (maxsim_rows.h).  The backward takes |x| from x again instead of reading
 // the rounded y and a saved norm: the same bytes, and nothing is saved.  Sums
-// are fp32, y and dx are rounded once, to nearest even.
+// are fp32, y and dx are rounded once, to nearest even.  A row whose squares
+// leave fp32 (longer than 2^63, or shorter than 2^-45 beside an eps that is
+// too) is moved to where they do not, by a power of two: rescale_row.
 #include <algorithm>
+#include <cfloat>
 
 #include "maxsim_host.h"
 #include "maxsim_rows.h"
@@ -32,8 +35,20 @@ struct UnitRows {
   const int32_t* offsets;  // NULL: padded
   int64_t packed_rows;
   float eps;
-  void* out;  // y or dx
+  float least;  // squares' sums below it are not trusted
+  void* out;    // y or dx
 };
+
+// Sums of squares, and products, above this may have passed fp32's largest
+// number on the way or be about to.
+constexpr float kMostSquares = 0x1p126f;
+// fp16's squares stay far from both.
+template <typename T> constexpr bool kWideRange = true;
+template <> constexpr bool kWideRange<F16> = false;
+// Sums of squares below this have lost part of themselves to fp32's smallest
+// one.  No loss where eps is larger than their root: the quotient is by eps.
+constexpr float kLeastSquares = 0x1p-90f, kLeastRoot = 0x1p-45f;
+static float least_squares(float eps) { return eps < kLeastRoot ? kLeastSquares : 0.0f; }
 
 // Where a row of the padded layout is, and whether it is a real token.
 struct Place {
@@ -50,6 +65,51 @@ __device__ __forceinline__ int64_t length_of(const UnitRows& a, int64_t seq) {
   const int32_t* l = static_cast<const int32_t*>(a.lengths) + (seq << is64);
   const int32_t lo = l[0], hi = l[is64];
   return is64 ? (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo) : lo;
+}
+
+// The words as they are in memory: the numbers unpacked from them before are
+// not kept for those after.
+template <typename T, int K>
+__device__ __forceinline__ void keep_packed(Chunk<T> (&c)[K]) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (uint32_t& w : c[k].w) asm("" : "+v"(w));
+}
+
+// For a row x with its dy and eps: all three times 2^-e, with e the exponent
+// of the larger of eps and x's largest element.  That changes neither
+// x / max(|x|, eps) nor dx, and the squares are then of numbers around 1.
+// Numbers that are not finite stay as they are.
+template <typename T, int G, int K, bool BACKWARD>
+__device__ void rescale_row(Chunk<T> (&x)[K], Chunk<T> (&dy)[K], float& eps, bool far,
+                            uint32_t* part) {
+  constexpr int V = kVec<T>;
+  uint32_t big = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    float f[V];
+    unpack<T, V>(x[k], f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) big = max(big, __float_as_uint(f[e]) & 0x7fffffffu);
+  }
+  big = group_max<G>(big, part);
+  keep_packed(x);
+  if (!far || big >= 0x7f800000u) return;
+  const int shift = 127 - (int)(max(big, __float_as_uint(eps)) >> 23);
+  eps = __builtin_amdgcn_ldexpf(eps, shift);
+  auto move = [&](Chunk<T>& c) {
+    float f[V];
+    unpack<T, V>(c, f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = __builtin_amdgcn_ldexpf(f[e], shift);
+    c = pack<T, V>(f);
+  };
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    move(x[k]);
+    if constexpr (BACKWARD) move(dy[k]);
+  }
 }
 
 // Workgroup b takes the rows from begin + b * GROUPS * U on, each group of lanes U of
@@ -118,59 +178,103 @@ __global__ __launch_bounds__(row_threads(G)) void unit_rows_kernel(UnitRows a) {
     }
   }
   Chunk<T> raw[U][K], raw_d[BACKWARD ? U : 1][K];
+  auto load = [&] {
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const S* xr = x + at[u].seq * a.x_seq + at[u].t * a.x_row;
-      raw[u][k] = at[u].real ? load_pieces<T, V>(xr, (j + k * G) * V, dim) : Chunk<T>{};
+      for (int k = 0; k < K; ++k) {
+        const S* xr = x + at[u].seq * a.x_seq + at[u].t * a.x_row;
+        raw[u][k] = at[u].real ? load_pieces<T, V>(xr, (j + k * G) * V, dim) : Chunk<T>{};
+        if constexpr (BACKWARD) {
+          const S* dr = a.offsets ? dy + at[u].packed * dim
+                                  : dy + at[u].seq * a.dy_seq + at[u].t * a.dy_row;
+          raw_d[u][k] = at[u].real ? load_pieces<T, V>(dr, (j + k * G) * V, dim) : Chunk<T>{};
+        }
+      }
+  };
+  float sums[SUMS];
+  auto add_up = [&] {
+#pragma unroll
+    for (int i = 0; i < SUMS; ++i) sums[i] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float f[V], d[V];
+        unpack<T, V>(raw[u][k], f);
+        if constexpr (BACKWARD) unpack<T, V>(raw_d[u][k], d);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          sums[u] += f[e] * f[e];
+          if constexpr (BACKWARD) sums[U + u] += f[e] * d[e];
+        }
+      }
+    group_sums<G>(sums, part);
+  };
+  bool far[U];  // the sums are not to be trusted
+  // Writes the rows whose far is `which`.
+  auto finish = [&](bool which, auto eps_of) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = row0 + u * GROUPS + group;
+      const bool real = at[u].real;
+      if (row >= a.rows || far[u] != which || (!BACKWARD && a.offsets && !real)) continue;
+      const float norm = sqrtf(sums[u]), eps = eps_of(u);
+      float scale = 1.0f / fmaxf(norm, eps), along = 0.0f;
       if constexpr (BACKWARD) {
-        const S* dr = a.offsets ? dy + at[u].packed * dim
-                                : dy + at[u].seq * a.dy_seq + at[u].t * a.dy_row;
-        raw_d[u][k] = at[u].real ? load_pieces<T, V>(dr, (j + k * G) * V, dim) : Chunk<T>{};
+        // y <y, dy> / |x| = x <x, dy> / |x|^3; a NaN norm stays NaN
+        if (!(norm <= eps)) along = sums[U + u] * scale * scale;
+      } else {
+        if (norm != norm) scale = norm;
+      }
+      S* to = out + (!BACKWARD && a.offsets ? at[u].packed : row) * dim;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float f[V], d[V];
+        unpack<T, V>(raw[u][k], f);
+        if constexpr (BACKWARD) unpack<T, V>(raw_d[u][k], d);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          if constexpr (BACKWARD) f[e] = d[e] - f[e] * along;
+          f[e] = real ? f[e] * scale : 0.0f;
+        }
+        store_chunk<T, V>(to, (j + k * G) * V, dim, f);
       }
     }
-  float sums[SUMS] = {};
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float f[V], d[V];
-      unpack<T, V>(raw[u][k], f);
-      if constexpr (BACKWARD) unpack<T, V>(raw_d[u][k], d);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        sums[u] += f[e] * f[e];
-        if constexpr (BACKWARD) sums[U + u] += f[e] * d[e];
-      }
-    }
-  group_sums<G>(sums, part);
+  };
+  load();
+  add_up();
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t row = row0 + u * GROUPS + group;
-    const bool real = at[u].real;
-    if (row >= a.rows || (!BACKWARD && a.offsets && !real)) continue;
-    const float norm = sqrtf(sums[u]);
-    float scale = 1.0f / fmaxf(norm, a.eps), along = 0.0f;
-    if constexpr (BACKWARD) {
-      // y <y, dy> / |x| = x <x, dy> / |x|^3; a NaN norm stays NaN
-      if (!(norm <= a.eps)) along = sums[U + u] * scale * scale;
-    } else {
-      if (norm != norm) scale = norm;
-    }
-    S* to = out + (!BACKWARD && a.offsets ? at[u].packed : row) * dim;
+    bool near = sums[u] >= a.least && sums[u] < kMostSquares;
+    if constexpr (BACKWARD) near = near && fabsf(sums[U + u]) < kMostSquares;
+    far[u] = kWideRange<T> && at[u].real && !near;
+  }
+  finish(false, [&](int) { return a.eps; });
+  if constexpr (kWideRange<T>) {
+    // The far ones from their loads on again: nothing is held or waited for
+    // above for their sake.  A wave's rows go through it together, and a
+    // workgroup's where it has one row: the sums, and so the answer, are the
+    // same in all its threads.
+    bool any = false;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float f[V], d[V];
-      unpack<T, V>(raw[u][k], f);
-      if constexpr (BACKWARD) unpack<T, V>(raw_d[u][k], d);
+    for (int u = 0; u < U; ++u) any |= far[u];
+    if (__ballot(any) == 0) return;
+    load();
+    float eps[U];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if constexpr (BACKWARD) f[e] = d[e] - f[e] * along;
-        f[e] = real ? f[e] * scale : 0.0f;
-      }
-      store_chunk<T, V>(to, (j + k * G) * V, dim, f);
+    for (int u = 0; u < U; ++u) {
+      eps[u] = a.eps;
+      rescale_row<T, G, K, BACKWARD>(raw[u], raw_d[BACKWARD ? u : 0], eps[u], far[u],
+                                     reinterpret_cast<uint32_t*>(part));
     }
+    add_up();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      keep_packed(raw[u]);
+      if constexpr (BACKWARD) keep_packed(raw_d[u]);
+    }
+    finish(true, [&](int u) { return eps[u]; });
   }
 }
 
@@ -271,7 +375,8 @@ static int check_unit_rows(maxsim_dtype dtype, int64_t sequences, int64_t length
   if (sequences < 0 || length < 0 || packed_rows < 0)
     return fail(MAXSIM_ERR_INVALID, "negative size");
   if (length > INT32_MAX) return fail(MAXSIM_ERR_UNSUPPORTED, "length exceeds 2^31 - 1");
-  if (!(eps > 0.0f)) return fail(MAXSIM_ERR_INVALID, "eps must be > 0");
+  // 1 / eps has to be a number too
+  if (!(eps >= FLT_MIN)) return fail(MAXSIM_ERR_INVALID, "eps must be at least 2^-126");
   if (sequences > 0 && offsets && !lengths)
     return fail(MAXSIM_ERR_INVALID, "offsets without lengths");
   return MAXSIM_OK;
@@ -296,7 +401,7 @@ int maxsim_amd_unit_rows_forward(maxsim_dtype dtype, const void* x, int64_t sequ
   if (!x || !y) return fail(MAXSIM_ERR_INVALID, "null pointer argument");
   const UnitRows a{x,           nullptr, x_seq_stride, x_row_stride, 0,           0,
                    sequences, sequences * length, 0, (int)length, (int)dim, lengths,
-                   lengths64, offsets, packed_rows, eps, y};
+                   lengths64, offsets, packed_rows, eps, least_squares(eps), y};
   return run_unit_rows<false>(dtype, a, stream);
 }
 
@@ -316,7 +421,7 @@ int maxsim_amd_unit_rows_backward(maxsim_dtype dtype, const void* dy, int64_t dy
     return fail(MAXSIM_ERR_INVALID, "null pointer argument");
   const UnitRows a{x,       dy,          x_seq_stride, x_row_stride, dy_seq_stride, dy_row_stride,
                    sequences, sequences * length, 0, (int)length, (int)dim, lengths,
-                   lengths64, offsets, packed_rows, eps, dx};
+                   lengths64, offsets, packed_rows, eps, least_squares(eps), dx};
   return run_unit_rows<true>(dtype, a, stream);
 }
 

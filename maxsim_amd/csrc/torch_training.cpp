@@ -14,6 +14,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <map>
 #include <optional>
 #include <tuple>
@@ -220,7 +221,8 @@ void check_unit(const Tensor& x, const optional<Tensor>& lengths, double eps) {
                                         : "x must have at least 1 dimension; got ",
                     x.sizes());
   TORCH_CHECK_VALUE(x.size(-1) > 0, "dim must be > 0; got ", x.size(-1));
-  TORCH_CHECK_VALUE(eps > 0.0 && eps < 1e30, "eps must be finite and > 0; got ", eps);
+  TORCH_CHECK_VALUE((float)eps >= FLT_MIN && eps < 1e30, "eps must be finite and at least 2^-126, "
+                    "the smallest normal float32; got ", eps);
   check_hip(x, "x");
   if (!lengths.has_value()) return;
   check_lengths(*lengths);

@@ -51,7 +51,8 @@ def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5) -> torch.Tensor:
     Returns:
         ``x.shape`` in x's dtype.  Differentiable with respect to x, weight
         and bias, each gradient in its tensor's dtype (fp32 sums rounded
-        once, in an order that the sizes alone decide).
+        once, in an order that the sizes alone decide).  Squares are fp32
+        numbers: rows with elements past 1e19 have an infinite variance.
     """
     _require_hip("x", x)
     return ops.maxsim_layer_norm(x, weight, bias, eps)
@@ -69,11 +70,12 @@ def normalize_embeddings(x, lengths=None, *, eps: float = 1e-12) -> torch.Tensor
             a sequence's length become 0 and are never read (they may hold
             NaN).  A length of 0 leaves the sequence without a token; lengths
             outside ``[0, L]`` are clamped.
-        eps: > 0; a token no longer than it is divided by it.
+        eps: at least 2^-126; a token no longer than it is divided by it.
 
     Returns:
         ``x.shape`` in x's dtype, differentiable with respect to x (padding
-        gets a gradient of 0, whatever comes down for it).
+        gets a gradient of 0, whatever comes down for it).  Tokens of any
+        finite length: the squares of long and short ones stay in range.
     """
     _require_hip("x", x)
     return ops.maxsim_normalize_embeddings(x, lengths, eps)
