@@ -11,7 +11,9 @@ Produces, next to this file:
 
 Run ``python maxsim_amd/_build.py`` (or ``__graft_entry__.build()``); not as
 ``python -m``, which would import the package and its previous build first.  The HIP
-objects are compiled in parallel; nothing is cached between runs.
+objects are compiled in parallel; nothing is cached between runs.  Both libraries
+are linked in ``_objs`` and put in place together: the binding calls the C ABI of
+the library it was built with, and a build that fails leaves the pair before it.
 """
 
 from __future__ import annotations
@@ -32,7 +34,7 @@ HIP_SOURCES = ["maxsim_fwd.hip", "maxsim_kloop.hip", "maxsim_bwd.hip", "maxsim_p
                "maxsim_ce.hip", "maxsim_check.hip", "maxsim_norm.hip", "maxsim_unit.hip",
                "maxsim_adamw.hip", "maxsim_capi.hip"]
 TORCH_SOURCES = ["torch_binding.cpp", "torch_training.cpp"]
-LIB = PKG / "libmaxsim_amd.so"
+LIB = PKG / "libmaxsim_amd.so"  # the two libraries, where they are loaded from
 TORCH_LIB = PKG / "_maxsim_amd_torch.so"
 
 HIPCC_FLAGS = [
@@ -68,10 +70,16 @@ def _run(cmds: list[list[str]]) -> None:
         raise RuntimeError(f"native build failed:\n{msg}")
 
 
-def build_hip_library() -> Path:
-    hipcc = str(ROCM / "bin" / "hipcc")
+def _objdir() -> Path:
     objdir = PKG / "_objs"
     objdir.mkdir(exist_ok=True)
+    return objdir
+
+
+def build_hip_library() -> Path:
+    """The kernels' library, in ``_objs``."""
+    hipcc = str(ROCM / "bin" / "hipcc")
+    objdir = _objdir()
     objs = []
     cmds = []
     for src in HIP_SOURCES:
@@ -79,20 +87,20 @@ def build_hip_library() -> Path:
         objs.append(obj)
         cmds.append([hipcc, *HIPCC_FLAGS, "-c", str(CSRC / src), "-o", str(obj)])
     _run(cmds)
-    tmp = LIB.with_suffix(".so.tmp")
-    _run([[hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp),
+    lib = objdir / LIB.name
+    _run([[hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(lib),
            *map(str, objs)]])
-    os.replace(tmp, LIB)
-    return LIB
+    return lib
 
 
 def build_torch_binding() -> Path:
+    """The binding for the library in ``_objs``, beside it."""
     import torch
 
     tdir = Path(torch.__file__).resolve().parent
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    tmp = TORCH_LIB.with_suffix(".so.tmp")
-    objdir = PKG / "_objs"
+    objdir = _objdir()
+    lib = objdir / TORCH_LIB.name
     objs = [objdir / (Path(src).stem + ".o") for src in TORCH_SOURCES]
     _run([[
         "g++", "-O2", "-std=c++17", "-fPIC",
@@ -104,15 +112,14 @@ def build_torch_binding() -> Path:
         "-c", str(CSRC / src), "-o", str(obj),
     ] for src, obj in zip(TORCH_SOURCES, objs)])
     cmd = [
-        "g++", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs),
-        "-L", str(PKG), "-lmaxsim_amd",
+        "g++", "-shared", "-fPIC", "-o", str(lib), *map(str, objs),
+        "-L", str(objdir), "-lmaxsim_amd",
         "-L", str(tdir / "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip",
         "-Wl,-rpath,$ORIGIN",
         "-Wl,-rpath," + str(tdir / "lib"),
     ]
     _run([cmd])
-    os.replace(tmp, TORCH_LIB)
-    return TORCH_LIB
+    return lib
 
 
 BUILD_INFO = PKG / "_build_info.json"
@@ -141,8 +148,9 @@ def write_build_info() -> None:
 
 
 def build() -> None:
-    build_hip_library()
-    build_torch_binding()
+    lib, torch_lib = build_hip_library(), build_torch_binding()
+    os.replace(lib, LIB)
+    os.replace(torch_lib, TORCH_LIB)
     write_build_info()
 
 
