@@ -258,11 +258,35 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """As torch's, which casts a state to its parameter's dtype; here each
         keeps its own (8-bit codes, fp32 moments and masters)."""
-        super().load_state_dict(state_dict)
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(saved, params):
-            for name, value in state_dict["state"].get(i, {}).items():
-                if isinstance(value, torch.Tensor):
-                    value = value.to(device=p.device, copy=True)
-                self.state[p][name] = value
+        # the last hook before torch's cast, which leaves what is no tensor
+        handle = self.register_load_state_dict_pre_hook(_hold_states)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            handle.remove()
+
+    def __setstate__(self, state) -> None:
+        # called with what is loaded, before the hooks that come after it
+        for p, held in state["state"].items():
+            if isinstance(p, torch.Tensor):
+                for name, value in held.items():
+                    if isinstance(value, _Held):
+                        held[name] = value.tensor.to(device=p.device, copy=True)
+        super().__setstate__(state)
+
+
+class _Held:
+    """A state's tensor on its way through torch's load_state_dict."""
+
+    def __init__(self, tensor: torch.Tensor):
+        self.tensor = tensor
+
+
+def _hold_states(optimizer, state_dict) -> dict:
+    def hold(value):
+        return _Held(value) if isinstance(value, torch.Tensor) else value
+
+    ours = {i for group in state_dict["param_groups"] for i in group["params"]}
+    return {**state_dict, "state": {
+        i: {name: hold(value) for name, value in state.items()} if i in ours else state
+        for i, state in state_dict["state"].items()}}
