@@ -164,6 +164,19 @@ def adamw_state_values(exp_avg, exp_avg_sq, scales) -> Tuple[torch.Tensor, torch
     return ops.maxsim_adamw_state_values(exp_avg, exp_avg_sq, scales)
 
 
+def _check_options(group) -> None:
+    if group["state_bits"] not in (8, 32):
+        raise ValueError(f"state_bits must be 8 or 32; got {group['state_bits']}")
+    for name in ("lr", "eps", "weight_decay"):
+        value = group[name]
+        if name == "lr" and isinstance(value, torch.Tensor):
+            continue  # on the device; checked where it is used, but for its value
+        if not (value >= 0.0 and math.isfinite(value)):
+            raise ValueError(f"{name} must be finite and >= 0; got {value}")
+    if len(group["betas"]) != 2 or not all(0.0 <= b < 1.0 for b in group["betas"]):
+        raise ValueError(f"betas must be two numbers in [0, 1); got {tuple(group['betas'])}")
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW on :func:`adamw_step`: every parameter of a group in a few
     launches, states in 32 or 8 bits.
@@ -180,8 +193,9 @@ class AdamW(torch.optim.Optimizer):
 
     State of a parameter: ``step`` (an int), ``exp_avg``, ``exp_avg_sq``, and
     ``scales`` / ``master`` where they apply.  ``state_dict`` round trips keep
-    the states' own dtypes.  The step count lives on the host: a captured graph
-    would replay one step's, so ``step()`` refuses to be captured
+    the states' own dtypes, and ``load_state_dict`` takes
+    ``torch.optim.AdamW``'s too.  The step count lives on the host: a captured
+    graph would replay one step's, so ``step()`` refuses to be captured
     (:func:`adamw_step` takes it as a tensor)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -194,17 +208,7 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, param_group) -> None:
         """As torch's; a group's own options are checked like the defaults."""
-        group = {**self.defaults, **param_group}
-        if group["state_bits"] not in (8, 32):
-            raise ValueError(f"state_bits must be 8 or 32; got {group['state_bits']}")
-        for name in ("lr", "eps", "weight_decay"):
-            value = group[name]
-            if name == "lr" and isinstance(value, torch.Tensor):
-                continue  # on the device; checked where it is used, but for its value
-            if not (value >= 0.0 and math.isfinite(value)):
-                raise ValueError(f"{name} must be finite and >= 0; got {value}")
-        if len(group["betas"]) != 2 or not all(0.0 <= b < 1.0 for b in group["betas"]):
-            raise ValueError(f"betas must be two numbers in [0, 1); got {tuple(group['betas'])}")
+        _check_options({**self.defaults, **param_group})
         super().add_param_group(param_group)
 
     def _new_state(self, p, group) -> dict:
@@ -240,6 +244,8 @@ class AdamW(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     state.update(self._new_state(p, group))
+                elif group["master_weights"] and "master" not in state and p.dtype != torch.float32:
+                    state["master"] = p.detach().to(torch.float32)  # loaded from elsewhere
                 key = (p.device, state["step"], "scales" in state, "master" in state)
                 calls.setdefault(key, []).append((p, state))
             for (_, step, eight, master), found in calls.items():
@@ -257,7 +263,14 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As torch's, which casts a state to its parameter's dtype; here each
-        keeps its own (8-bit codes, fp32 moments and masters)."""
+        keeps its own (8-bit codes, fp32 moments and masters).
+
+        A ``torch.optim.AdamW``'s state dict is taken as well: its moments as
+        fp32 states, whatever ``state_bits`` says of new ones, and a master is
+        made at the next step where ``master_weights`` asks for one.  Options of
+        this class that the dict does not have stay as they are.  ValueError for
+        what this optimizer would step otherwise: ``amsgrad``, ``maximize``, a
+        decay that is not decoupled, another optimizer's states."""
         # the last hook before torch's cast, which leaves what is no tensor
         handle = self.register_load_state_dict_pre_hook(_hold_states)
         try:
@@ -283,10 +296,38 @@ class _Held:
 
 
 def _hold_states(optimizer, state_dict) -> dict:
-    def hold(value):
-        return _Held(value) if isinstance(value, torch.Tensor) else value
+    """state_dict as this optimizer has it, its states' tensors held."""
+    groups, owner = [], {}
+    for saved, group in zip(state_dict["param_groups"], optimizer.param_groups):
+        if saved.get("amsgrad") or saved.get("maximize"):
+            raise ValueError("AdamW has no amsgrad and no maximize")
+        if not saved.get("decoupled_weight_decay", True) and saved.get("weight_decay"):
+            raise ValueError("AdamW's weight decay is decoupled; the loaded one is not")
+        groups.append({**{k: v for k, v in group.items() if k != "params"}, **saved})
+        _check_options(groups[-1])
+        owner.update(zip(saved["params"], group["params"]))
+    groups += state_dict["param_groups"][len(groups):]  # torch refuses another number of them
+    states = {i: _hold_state(i, state, owner[i]) if i in owner else state
+              for i, state in state_dict["state"].items()}
+    return {**state_dict, "param_groups": groups, "state": states}
 
-    ours = {i for group in state_dict["param_groups"] for i in group["params"]}
-    return {**state_dict, "state": {
-        i: {name: hold(value) for name, value in state.items()} if i in ours else state
-        for i, state in state_dict["state"].items()}}
+
+def _hold_state(i, state, p) -> dict:
+    held = {}
+    for name, value in state.items():
+        if not isinstance(value, torch.Tensor):
+            held[name] = value
+        elif name == "step":
+            held[name] = int(value)
+        else:
+            if name in ("exp_avg", "exp_avg_sq", "master") and value.shape == p.shape:
+                if value.is_floating_point() and (value.dtype != torch.float32
+                                                  or value.stride() != p.stride()):
+                    value = torch.empty_like(p, dtype=torch.float32).copy_(value)
+            held[name] = _Held(value)
+    if held and not {"step", "exp_avg", "exp_avg_sq"} <= held.keys():
+        raise ValueError(f"the state of parameter {i} has no step, exp_avg and exp_avg_sq: "
+                         f"{sorted(held)}")
+    if held and held["exp_avg"].tensor.dtype == torch.uint8 and "scales" not in held:
+        raise ValueError(f"the state of parameter {i} has 8-bit codes without their scales")
+    return held

@@ -1,11 +1,12 @@
-"""State dicts that maxsim_amd.AdamW takes: its own, and what
-load hooks make of them (CPU only: nothing steps on a device here)."""
+"""State dicts that maxsim_amd.AdamW takes: its own, torch.optim.AdamW's, and
+what load hooks make of them (CPU only: nothing steps on a device here)."""
 
 from __future__ import annotations
 
 import copy
 import io
 
+import pytest
 import torch
 
 import maxsim_amd
@@ -16,9 +17,67 @@ def _params(dtype=torch.float32):
     return [torch.randn(s, generator=gen).to(dtype).requires_grad_(True) for s in ((6, 5), (7,))]
 
 
+def _torch_state(dtype=torch.float32, steps=3, cls=torch.optim.AdamW, **kw):
+    params = _params(dtype)
+    opt = cls(params, lr=1e-2, weight_decay=0.05, **kw)
+    gen = torch.Generator().manual_seed(1)
+    for _ in range(steps):
+        for p in params:
+            p.grad = torch.randn(p.shape, generator=gen).to(dtype)
+        opt.step()
+    return opt.state_dict()
+
+
 def _own(dtype=torch.float32, **kw):
     params = _params(dtype)
     return params, maxsim_amd.AdamW(params, **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_takes_torch_adamw(dtype):
+    saved = _torch_state(dtype)
+    params, opt = _own(dtype, lr=5.0, state_bits=8, master_weights=True, seed=3)
+    opt.load_state_dict(saved)
+    group = opt.param_groups[0]
+    assert group["lr"] == 1e-2 and group["weight_decay"] == 0.05
+    # its own options stay as they were
+    assert (group["state_bits"], group["min_8bit_size"]) == (8, 4096)
+    assert (group["master_weights"], group["seed"]) == (True, 3)
+    for i, p in enumerate(params):
+        s, want = opt.state[p], saved["state"][i]
+        assert s["step"] == 3 and type(s["step"]) is int
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert s[name].dtype == torch.float32
+            assert torch.equal(s[name], want[name].float())
+            assert s[name].data_ptr() != want[name].data_ptr()
+
+
+@pytest.mark.parametrize("saved,text", [
+    (lambda: _torch_state(amsgrad=True), "amsgrad"),
+    (lambda: _torch_state(maximize=True), "maximize"),
+    (lambda: _torch_state(cls=torch.optim.Adam), "decoupled"),
+    (lambda: _torch_state(cls=torch.optim.SGD, momentum=0.9), "exp_avg"),
+])
+def test_refuses_what_it_cannot_step(saved, text):
+    params, opt = _own()
+    before = copy.deepcopy(opt.state_dict())
+    with pytest.raises(ValueError, match=text):
+        opt.load_state_dict(saved())
+    assert opt.state_dict() == before
+
+
+def test_refuses_codes_without_scales_and_bad_options():
+    params, opt = _own()
+    saved = _torch_state()
+    codes = copy.deepcopy(saved)
+    codes["state"][0]["exp_avg"] = torch.zeros(6, 5, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="scales"):
+        opt.load_state_dict(codes)
+    for name, value in (("lr", -1.0), ("betas", (0.9, 1.0)), ("state_bits", 4)):
+        bad = copy.deepcopy(saved)
+        bad["param_groups"][0][name] = value
+        with pytest.raises(ValueError, match=name):
+            opt.load_state_dict(bad)
 
 
 def _own_state(dtype=torch.bfloat16):
@@ -82,3 +141,13 @@ def test_load_hooks_count():
     assert torch.equal(other.state[others[1]]["exp_avg_sq"], opt.state[params[1]]["exp_avg_sq"])
 
 
+def test_states_come_in_their_parameters_order():
+    # saved for a contiguous parameter, loaded for a transposed one
+    saved = _torch_state()
+    first, second = _params()
+    first = first.detach().t().contiguous().t().requires_grad_(True)
+    opt = maxsim_amd.AdamW([first, second])
+    opt.load_state_dict(saved)
+    s = opt.state[first]
+    assert s["exp_avg"].stride() == first.stride()
+    assert torch.equal(s["exp_avg"], saved["state"][0]["exp_avg"])

@@ -7,10 +7,11 @@ import numpy as np
 import pytest
 import torch
 
+import maxsim_amd
 from oracle import training_oracle as oracle
 
 from ._training_helpers import U32, f64
-from .test_gpu_adamw import HYPER, _clone, _make, _step
+from .test_gpu_adamw import HYPER, _clone, _make, _model, _step, _train
 
 pytestmark = pytest.mark.gpu
 
@@ -177,3 +178,40 @@ def test_neighbours_in_one_buffer_do_not_share():
             t[k][i] = flat[at:at + t[k][i].numel()]
     _step(t)
     assert all(torch.equal(a, b) for k in want for a, b in zip(want[k], t[k]))
+
+
+# ---- torch.optim.AdamW's states ----------------------------------------------
+def test_goes_on_from_torch_adamw():
+    # three steps by torch, then five by either
+    kw = dict(lr=1e-2, betas=(0.9, 0.99), eps=1e-6, weight_decay=0.05)
+    a, b = _model(), _model()
+    theirs = torch.optim.AdamW(a.parameters(), **kw, foreach=False, fused=False)
+    _train(a, theirs, 3)
+    b.load_state_dict(a.state_dict())
+    opt = maxsim_amd.AdamW(b.parameters())
+    opt.load_state_dict(theirs.state_dict())
+    _train(a, theirs, 5, seed=2)
+    _train(b, opt, 5, seed=2)
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert opt.state[q]["step"] == 8
+        torch.testing.assert_close(p, q, rtol=1e-4, atol=1e-5)
+
+
+def test_masters_of_states_from_torch():
+    # made at the first step that follows, from the parameter as it is then
+    params = [torch.randn(40, 30, device="cuda").bfloat16().requires_grad_(True)]
+    theirs = torch.optim.AdamW(params, foreach=False, fused=False)
+    params[0].grad = torch.randn_like(params[0])
+    theirs.step()
+    saved = theirs.state_dict()
+    opt = maxsim_amd.AdamW(params, master_weights=True)
+    opt.load_state_dict(saved)
+    with torch.no_grad():
+        params[0].mul_(2)
+    p, master = params[0].detach().clone(), params[0].detach().float()
+    m, v = (saved["state"][0][k].float() for k in ("exp_avg", "exp_avg_sq"))
+    maxsim_amd.adamw_step([p], [params[0].grad], [m], [v], step=2, masters=[master])
+    opt.step()
+    s = opt.state[params[0]]
+    assert torch.equal(params[0], p) and torch.equal(s["master"], master)
+    assert torch.equal(s["exp_avg"], m) and torch.equal(s["exp_avg_sq"], v) and s["step"] == 2
