@@ -51,7 +51,7 @@ int maxsim_amd_layer_norm_backward(maxsim_dtype dtype, maxsim_dtype weight_dtype
 
 /* y = x / max(|x|, eps) for each row of x [sequences, length, dim] (sequences
  * x_seq_stride and rows x_row_stride apart), rows of any finite length; eps at
- * least 2^-126.
+ * least 2^-126; `length` below 2^31 (more rows: as many sequences of one).
  * lengths NULL: every row.  lengths [sequences], int32 (lengths64 0) or int64
  * (1): rows at or past a sequence's
  * length (below 0 counts as 0) are not read.  offsets NULL: y is

@@ -250,12 +250,17 @@ Lengths lengths_of(const optional<Tensor>& lengths) {
 const int32_t* i32(const Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; }
 
 // x as sequences x length x dim: with lengths they are given, without them
-// rows are told apart by two strides at most.
-Rows unit_rows(const Tensor& x) { return rows_of(x, x.dim() >= 3 ? x.dim() - 2 : 0); }
+// rows are told apart by two strides at most.  More rows than a sequence can
+// have are as many sequences of one.
+Rows unit_rows(const Tensor& x, const Lengths& lengths) {
+  Rows r = rows_of(x, x.dim() >= 3 ? x.dim() - 2 : 0);
+  if (r.inner > INT32_MAX && !lengths.data) r = rows_of(x, x.dim() - 1);
+  return r;
+}
 
 Tensor unit_forward(const Tensor& x, const Lengths& lengths, const Tensor& offsets,
                     int64_t packed_rows, double eps) {
-  const Rows r = unit_rows(x);
+  const Rows r = unit_rows(x, lengths);
   Tensor y = offsets.defined() ? empty_like_on(x, {packed_rows, x.size(-1)})
                                : empty_like_on(x, x.sizes());
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
@@ -271,12 +276,12 @@ Tensor unit_backward(const Tensor& dy, const Tensor& x, const Lengths& lengths,
                      const Tensor& offsets, int64_t packed_rows, double eps) {
   TORCH_CHECK(dy.scalar_type() == x.scalar_type(), "dy must have x's dtype");
   check_same_device(dy, "dy", x, "x");
-  Rows r = unit_rows(x);
+  const Rows r = unit_rows(x, lengths);
   Rows g;
   if (offsets.defined()) {
     g.t = dy.contiguous();
   } else {
-    g = unit_rows(dy);
+    g = unit_rows(dy, lengths);
   }
   Tensor dx = empty_like_on(x, x.sizes());
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());

@@ -126,3 +126,20 @@ def test_oracle_divides_by_the_length():
     x = np.array([[[3e38, 0.0, 4e37]]])
     assert np.allclose((oracle.unit_rows(x, None, 1e-12) ** 2).sum(), 1.0)
     assert f64(torch.tensor([2.0 ** 127])).tolist() == [2.0 ** 127]
+
+
+def test_more_than_two_to_the_31_rows():
+    # [rows, dim] is one axis of rows, as long as memory has room for
+    rows = 2 ** 31 + 5
+    x = torch.ones(rows, 1, dtype=torch.float16, device="cuda")
+    tail = torch.tensor([-3.0, 0.0, 5.0, 2.0 ** -20, -1.0], device="cuda").half()[:, None]
+    x[-5:] = tail
+    leaf = x.requires_grad_(True)
+    y = maxsim_amd.normalize_embeddings(leaf)
+    assert y.shape == x.shape and torch.equal(y[-5:].detach(), tail.sign())
+    assert bool((y[:-5] == 1).all())
+    del y
+    y = maxsim_amd.normalize_embeddings(leaf, eps=0.5)  # below it the gradient is dy / eps
+    (dx,) = torch.autograd.grad(y, leaf, torch.ones((1, 1), dtype=torch.float16,
+                                                    device="cuda").expand(rows, 1))
+    assert dx[-5:, 0].tolist() == [0.0, 2.0, 0.0, 2.0, 0.0] and bool((dx[:-5] == 0).all())
