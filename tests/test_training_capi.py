@@ -144,3 +144,13 @@ def test_adamw_refusals(lib):
     assert values(ONE, ONE, ONE, -1, ONE, ONE, None) == INVALID
     assert values(ONE, None, ONE, 4, ONE, ONE, None) == INVALID
     assert values(None, None, None, 0, None, None, None) == OK
+
+
+def test_unit_rows_refuse_an_eps_below_the_normal_numbers(lib):
+    # its reciprocal is past fp32's largest number
+    fn = lib.maxsim_amd_unit_rows_forward
+    fn.argtypes = [ctypes.c_int, P, I64, I64, I64, I64, I64, P, ctypes.c_int, P, I64, F, P, P]
+    for eps in (1e-39, 1e-45, -1.0):
+        assert fn(F32, ONE, 2, 3, 64, 192, 64, None, 0, None, 0, eps, ONE, None) == INVALID
+        assert b"eps" in lib.maxsim_amd_last_error()
+    assert fn(F32, ONE, 0, 3, 64, 192, 64, None, 0, None, 0, 2.0 ** -126, ONE, None) == OK
