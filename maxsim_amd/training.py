@@ -146,15 +146,19 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     moving averages keep moving by less than their spacing.  The step itself
     uses them unrounded.  A value that is not finite makes its block NaN."""
     params = list(params)
+    grads, exp_avgs, exp_avg_sqs = list(grads), list(exp_avgs), list(exp_avg_sqs)
+    scales, masters = list(scales or ()), list(masters or ())
     lr_tensor = lr if isinstance(lr, torch.Tensor) else None
     step_tensor = step if isinstance(step, torch.Tensor) else None
     if not params:
+        if grads or exp_avgs or exp_avg_sqs or scales or masters:
+            raise ValueError("adamw_step needs lists of one length; got no params")
         return
     _require_hip("params", params[0])
     ops.maxsim_adamw_step(
-        params, list(grads), list(exp_avgs), list(exp_avg_sqs), list(scales or ()),
-        list(masters or ()), 0.0 if lr_tensor is not None else lr, lr_tensor, betas[0], betas[1],
-        eps, weight_decay, 1 if step_tensor is not None else step, step_tensor, seed)
+        params, grads, exp_avgs, exp_avg_sqs, scales, masters,
+        0.0 if lr_tensor is not None else lr, lr_tensor, betas[0], betas[1], eps, weight_decay,
+        1 if step_tensor is not None else step, step_tensor, seed)
 
 
 def adamw_state_values(exp_avg, exp_avg_sq, scales) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -215,3 +215,13 @@ def test_masters_of_states_from_torch():
     s = opt.state[params[0]]
     assert torch.equal(params[0], p) and torch.equal(s["master"], master)
     assert torch.equal(s["exp_avg"], m) and torch.equal(s["exp_avg_sq"], v) and s["step"] == 2
+
+
+def test_no_parameters_beside_other_lists():
+    x = [torch.zeros(3, device="cuda")]
+    maxsim_amd.adamw_step([], [], [], [], step=1, scales=[], masters=())
+    for lists in (([], x, [], []), ([], [], x, []), ([], [], [], x)):
+        with pytest.raises(ValueError, match="one length"):
+            maxsim_amd.adamw_step(*lists, step=1)
+    with pytest.raises(ValueError, match="one length"):
+        maxsim_amd.adamw_step([], [], [], [], step=1, masters=x)
