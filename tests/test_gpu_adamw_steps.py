@@ -11,7 +11,7 @@ import maxsim_amd
 from oracle import training_oracle as oracle
 
 from ._training_helpers import U32, f64
-from .test_gpu_adamw import HYPER, _clone, _make, _model, _step, _train
+from .test_gpu_adamw import HYPER, _check, _clone, _make, _model, _step, _train
 
 pytestmark = pytest.mark.gpu
 
@@ -215,6 +215,24 @@ def test_masters_of_states_from_torch():
     s = opt.state[params[0]]
     assert torch.equal(params[0], p) and torch.equal(s["master"], master)
     assert torch.equal(s["exp_avg"], m) and torch.equal(s["exp_avg_sq"], v) and s["step"] == 2
+
+
+# ---- the limits of a launch --------------------------------------------------
+# tensors that 4 KB of arguments hold: 3968 bytes at 44 each, 12 more with 8-bit
+# states and 8 more with masters
+LIMITS = {(32, False): 90, (32, True): 76, (8, False): 70, (8, True): 62}
+
+
+@pytest.mark.parametrize("bits,master", LIMITS)
+@pytest.mark.parametrize("times,more", [(1, -1), (1, 0), (1, 1), (2, 0), (2, 1)])
+def test_launches_filled_to_the_last_tensor(bits, master, times, more):
+    count = times * LIMITS[bits, master] + more
+    dtype = torch.bfloat16 if master else torch.float32
+    t = _make([(53 * i) % 900 + 1 for i in range(count - 1)] + [5000], dtype, dtype, bits, master,
+              seed=count)
+    before = _clone(t)
+    _step(t)
+    _check(before, t)
 
 
 def test_no_parameters_beside_other_lists():
