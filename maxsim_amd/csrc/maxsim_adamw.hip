@@ -156,7 +156,7 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, int64_t n, float
 #pragma unroll
     for (int c = 0; c < 8 / v; ++c) {
       float part[v];
-      unpack<T, v>(load_any<Chunk<T>>(s + c * v), part);
+      unpack<T>(load_any<Chunk<T>>(s + c * v), part);
 #pragma unroll
       for (int e = 0; e < v; ++e) f[c * v + e] = part[e];
     }
@@ -175,7 +175,7 @@ __device__ __forceinline__ void store8(void* p, int64_t i, int64_t n, const floa
       float part[v];
 #pragma unroll
       for (int e = 0; e < v; ++e) part[e] = f[c * v + e];
-      store_any(s + c * v, pack<T, v>(part));
+      store_any(s + c * v, pack<T>(part));
     }
   } else {
 #pragma unroll

@@ -50,7 +50,7 @@ __global__ __launch_bounds__(row_threads(G)) void ln_forward_kernel(LnForward a)
   Chunk<T> next[K] = {};
   if (row < a.rows) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) next[k] = load_chunk<T, V, takes_short(G)>(x + row * a.stride, (j + k * G) * V, dim);
+    for (int k = 0; k < K; ++k) next[k] = load_chunk<T, takes_short(G)>(x + row * a.stride, (j + k * G) * V, dim);
   }
   float w[K][V], b[K][V];
 #pragma unroll
@@ -63,13 +63,13 @@ __global__ __launch_bounds__(row_threads(G)) void ln_forward_kernel(LnForward a)
     float f[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (!whole) place_chunk<T, V, takes_short(G)>(next[k], (j + k * G) * V, dim);
-      unpack<T, V>(next[k], f[k]);
+      if (!whole) place_chunk<T, takes_short(G)>(next[k], (j + k * G) * V, dim);
+      unpack<T>(next[k], f[k]);
     }
     if (row + step < a.rows) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        next[k] = load_chunk<T, V, takes_short(G)>(x + (row + step) * a.stride, (j + k * G) * V, dim);
+        next[k] = load_chunk<T, takes_short(G)>(x + (row + step) * a.stride, (j + k * G) * V, dim);
     }
     float sum[1] = {0.0f};
 #pragma unroll
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(row_threads(G)) void ln_forward_kernel(LnForward a)
       for (int k = 0; k < K; ++k) {
 #pragma unroll
         for (int e = 0; e < V; ++e) f[k][e] = f[k][e] * rstd * w[k][e] + b[k][e];
-        store_chunk<T, V>(y + row * dim, (j + k * G) * V, dim, f[k]);
+        store_chunk<T>(y + row * dim, (j + k * G) * V, dim, f[k]);
       }
       if (a.mean && j == 0) {
         a.mean[row] = mean;
@@ -141,13 +141,13 @@ __global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward 
 
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   int64_t row = (int64_t)blockIdx.x * GROUPS + group;
-  Chunk<T, V> next_x[K] = {}, next_d[K] = {};
+  Chunk<T> next_x[K] = {}, next_d[K] = {};
   float next_mean = 0.0f, next_rstd = 0.0f;
   auto load = [&](int64_t r) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      next_x[k] = load_chunk<T, V, takes_short(G)>(x + r * a.x_stride, (j + k * G) * V, dim);
-      next_d[k] = load_chunk<T, V, takes_short(G)>(dy + r * a.dy_stride, (j + k * G) * V, dim);
+      next_x[k] = load_chunk<T, takes_short(G)>(x + r * a.x_stride, (j + k * G) * V, dim);
+      next_d[k] = load_chunk<T, takes_short(G)>(dy + r * a.dy_stride, (j + k * G) * V, dim);
     }
     next_mean = a.mean[r];
     next_rstd = a.rstd[r];
@@ -171,11 +171,11 @@ __global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward 
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!whole) {
-        place_chunk<T, V, takes_short(G)>(next_x[k], (j + k * G) * V, dim);
-        place_chunk<T, V, takes_short(G)>(next_d[k], (j + k * G) * V, dim);
+        place_chunk<T, takes_short(G)>(next_x[k], (j + k * G) * V, dim);
+        place_chunk<T, takes_short(G)>(next_d[k], (j + k * G) * V, dim);
       }
-      unpack<T, V>(next_x[k], f[k]);
-      unpack<T, V>(next_d[k], d[k]);
+      unpack<T>(next_x[k], f[k]);
+      unpack<T>(next_d[k], d[k]);
     }
     const bool here = row < a.rows;
     if (AHEAD && row + step < a.rows) load(row + step);
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(row_threads(G)) void ln_backward_kernel(LnBackward 
         for (int k = 0; k < K; ++k) {
 #pragma unroll
           for (int e = 0; e < V; ++e) f[k][e] = rstd * (d[k][e] - c1 - f[k][e] * c2);
-          store_chunk<T, V>(dx + row * dim, (j + k * G) * V, dim, f[k]);
+          store_chunk<T>(dx + row * dim, (j + k * G) * V, dim, f[k]);
         }
       }
     }

@@ -1,7 +1,7 @@
 // Shared device code of the row operators (layer norm, unit rows): a group of
-// G lanes holds one row of `dim` elements in registers, K chunks of V elements
-// (8 or 16 bytes) per lane, and reduces over the row without leaving the wave (G <= 64) or
-// through one LDS word per wave (G = 256, 512, 1024).
+// G lanes holds one row of `dim` elements in registers, K chunks of 16 bytes
+// (V elements) per lane, and reduces over the row without leaving the wave
+// (G <= 64) or through one LDS word per wave (G = 256, 512, 1024).
 //
 // Lane j of a group holds chunks j, j + G, ...: consecutive lanes read
 // consecutive chunks.  Rows may start at any multiple of the element size;
@@ -40,32 +40,28 @@ __device__ __forceinline__ typename T::storage from_float(float f) {
   else return f;
 }
 
-// V elements as they are in memory (8 or 16 bytes).
-template <typename T, int V = kVec<T>> struct Chunk {
-  static constexpr int words = V * T::bytes / 4;
-  static_assert(words == 2 || words == 4, "8 or 16 bytes");
-  uint32_t w[words];
-};
+// A chunk as it is in memory.
+template <typename T> struct Chunk { uint32_t w[4]; };
 
-template <typename T, int V>
-__device__ __forceinline__ void unpack(const Chunk<T, V>& c, float (&f)[V]) {
+template <typename T>
+__device__ __forceinline__ void unpack(const Chunk<T>& c, float (&f)[kVec<T>]) {
   if constexpr (T::bytes == 2) {
 #pragma unroll
-    for (int e = 0; e < V / 2; ++e) {
+    for (int e = 0; e < 4; ++e) {
       f[2 * e] = from16(c.w[e] & 0xffffu, T{});
       f[2 * e + 1] = from16(c.w[e] >> 16, T{});
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = __uint_as_float(c.w[e]);
+    for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(c.w[e]);
   }
 }
 
-template <typename T, int V>
-__device__ __forceinline__ Chunk<T, V> pack(const float (&f)[V]) {
-  Chunk<T, V> c;
+template <typename T>
+__device__ __forceinline__ Chunk<T> pack(const float (&f)[kVec<T>]) {
+  Chunk<T> c;
 #pragma unroll
-  for (int e = 0; e < Chunk<T, V>::words; ++e) {
+  for (int e = 0; e < 4; ++e) {
     if constexpr (T::bytes == 2)
       c.w[e] = bits16(f[2 * e], T{}) | (bits16(f[2 * e + 1], T{}) << 16);
     else
@@ -91,12 +87,10 @@ __device__ __forceinline__ void store_any(S* p, R v) {
 // chunk of n elements comes in at most three pieces, by the bits of n.  For
 // rows that are asked for once (unit rows): lanes past the row's end read
 // nothing (1000 x 300 x 300 f16: 53 us against 60 with load_chunk).
-template <typename T, int V>
-__device__ __forceinline__ Chunk<T, V> load_pieces(const typename T::storage* row, int e0,
-                                                   int dim) {
-  typedef Chunk<T, V> C;
-  if (e0 + V <= dim) return load_any<C>(row + e0);
-  C r = {};
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_pieces(const typename T::storage* row, int e0, int dim) {
+  if (e0 + kVec<T> <= dim) return load_any<Chunk<T>>(row + e0);
+  Chunk<T> r = {};
   if (e0 >= dim) return r;
   const int n = dim - e0;
   const typename T::storage* p = row + e0;
@@ -109,16 +103,12 @@ __device__ __forceinline__ Chunk<T, V> load_pieces(const typename T::storage* ro
   } else {
     const uint32_t b = n & 2 ? load_any<uint32_t>(p + (n & 4)) : 0;
     const uint32_t c = n & 1 ? p[n & 6] : 0;
-    const uint32_t bc = n & 2 ? b : c;
-    r.w[0] = bc;
-    r.w[1] = n & 2 ? c : 0;
-    if constexpr (V == 8) {
-      const uint2 a = n & 4 ? load_any<uint2>(p) : make_uint2(0, 0);
-      r.w[2] = n & 4 ? bc : 0;
-      r.w[3] = n & 4 ? r.w[1] : 0;
-      r.w[0] = n & 4 ? a.x : bc;
-      r.w[1] = n & 4 ? a.y : r.w[1];
-    }
+    const uint32_t bc = n & 2 ? b : c, last = n & 2 ? c : 0;
+    const uint2 a = n & 4 ? load_any<uint2>(p) : make_uint2(0, 0);
+    r.w[0] = n & 4 ? a.x : bc;
+    r.w[1] = n & 4 ? a.y : last;
+    r.w[2] = n & 4 ? bc : 0;
+    r.w[3] = n & 4 ? last : 0;
   }
   return r;
 }
@@ -130,11 +120,11 @@ __device__ __forceinline__ Chunk<T, V> load_pieces(const typename T::storage* ro
 // loads stay in flight (200000 x 300 bf16, forward and backward: 52 + 78 us
 // against 57 + 86 with the branches of load_pieces).  SHORT: the row may be
 // shorter than a chunk, and such a one is read by elements.
-template <typename T, int V, bool SHORT>
-__device__ __forceinline__ Chunk<T, V> load_chunk(const typename T::storage* row, int e0,
-                                                  int dim) {
+template <typename T, bool SHORT>
+__device__ __forceinline__ Chunk<T> load_chunk(const typename T::storage* row, int e0, int dim) {
+  constexpr int V = kVec<T>;
   if (SHORT && dim < V) {
-    Chunk<T, V> r = {};
+    Chunk<T> r = {};
 #pragma unroll
     for (int e = 0; e < V - 1; ++e)
       if (e0 + e < dim) {
@@ -143,19 +133,16 @@ __device__ __forceinline__ Chunk<T, V> load_chunk(const typename T::storage* row
       }
     return r;
   }
-  return load_any<Chunk<T, V>>(row + min(e0, dim - V));
+  return load_any<Chunk<T>>(row + min(e0, dim - V));
 }
-template <typename T, int V, bool SHORT>
-__device__ __forceinline__ void place_chunk(Chunk<T, V>& c, int e0, int dim) {
+template <typename T, bool SHORT>
+__device__ __forceinline__ void place_chunk(Chunk<T>& c, int e0, int dim) {
+  constexpr int V = kVec<T>;
   if (SHORT && dim < V) return;
   const int n = T::bytes * max(e0 - (dim - V), 0);  // bytes that belong before e0
   if (dim % V == 0) {  // all or nothing
 #pragma unroll
-    for (int i = 0; i < Chunk<T, V>::words; ++i) c.w[i] = n ? 0 : c.w[i];
-  } else if constexpr (Chunk<T, V>::words == 2) {
-    const uint64_t v = c.w[0] | (uint64_t)c.w[1] << 32;
-    const uint64_t r = n >= 8 ? 0 : v >> (8 * (n & 7));
-    c.w[0] = (uint32_t)r, c.w[1] = (uint32_t)(r >> 32);
+    for (int i = 0; i < 4; ++i) c.w[i] = n ? 0 : c.w[i];
   } else {
     const uint4 r = drop_bytes(make_uint4(c.w[0], c.w[1], c.w[2], c.w[3]), n);
     c.w[0] = r.x, c.w[1] = r.y, c.w[2] = r.z, c.w[3] = r.w;
@@ -164,11 +151,11 @@ __device__ __forceinline__ void place_chunk(Chunk<T, V>& c, int e0, int dim) {
 
 // The row's cut chunk of n elements goes in at most three pieces, by the bits
 // of n.
-template <typename T, int V>
+template <typename T>
 __device__ __forceinline__ void store_chunk(typename T::storage* row, int e0, int dim,
-                                            const float (&f)[V]) {
-  const Chunk<T, V> r = pack<T, V>(f);
-  if (e0 + V <= dim) {
+                                            const float (&f)[kVec<T>]) {
+  const Chunk<T> r = pack<T>(f);
+  if (e0 + kVec<T> <= dim) {
     store_any(row + e0, r);
     return;
   }
@@ -179,12 +166,8 @@ __device__ __forceinline__ void store_chunk(typename T::storage* row, int e0, in
     if (n & 2) store_any(p, make_uint2(r.w[0], r.w[1]));
     if (n & 1) store_any(p + (n & 2), n & 2 ? r.w[2] : r.w[0]);
   } else {
-    uint32_t b = r.w[0], c = r.w[1];
-    if constexpr (V == 8) {
-      if (n & 4) store_any(p, make_uint2(r.w[0], r.w[1]));
-      b = n & 4 ? r.w[2] : b;
-      c = n & 4 ? r.w[3] : c;
-    }
+    if (n & 4) store_any(p, make_uint2(r.w[0], r.w[1]));
+    const uint32_t b = n & 4 ? r.w[2] : r.w[0], c = n & 4 ? r.w[3] : r.w[1];
     if (n & 2) store_any(p + (n & 4), b);
     if (n & 1) p[n & 6] = (uint16_t)(n & 2 ? c : b);
   }
@@ -196,7 +179,7 @@ template <typename W, int N>
 __device__ __forceinline__ void load_param(const void* p, int e0, int dim, float fill,
                                            float (&f)[N]) {
   const typename W::storage* w = static_cast<const typename W::storage*>(p);
-  constexpr int v = N < kVec<W> ? N : kVec<W>;
+  constexpr int v = kVec<W>;
   static_assert(N % v == 0, "whole chunks of the parameter's type");
   if (!w) {
 #pragma unroll
@@ -205,7 +188,7 @@ __device__ __forceinline__ void load_param(const void* p, int e0, int dim, float
 #pragma unroll
     for (int c = 0; c < N / v; ++c) {
       float part[v];
-      unpack<W, v>(load_any<Chunk<W, v>>(w + e0 + c * v), part);
+      unpack<W>(load_any<Chunk<W>>(w + e0 + c * v), part);
 #pragma unroll
       for (int e = 0; e < v; ++e) f[c * v + e] = part[e];
     }
@@ -316,8 +299,8 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v, uint32_t* part) {
 
 // Calls f with the group shape for rows of `dim` elements (up to
 // MAXSIM_AMD_MAX_DIM) in chunks of V: the one that leaves fewest lanes idle
-// among those that hold a row in at most three chunks per lane; more lanes
-// than a wave where that is not enough.  (Rows of 768 elements of 16 bits, 96
+// among those that hold a row in at most three chunks per lane (four in fp32
+// rows past 8192 elements); more lanes than a wave where that is not enough.  (Rows of 768 elements of 16 bits, 96
 // chunks of 8: 32 lanes x 3.)  512 threads where they hold a row:
 // two such workgroups on a CU work at each other's barriers (layer norm of 8000
 // x 12288 bf16 backward 122 us, with 1024 threads 137; 12000 x 8192 forward 72

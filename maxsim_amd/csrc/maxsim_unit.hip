@@ -89,7 +89,7 @@ __device__ void rescale_row(Chunk<T> (&x)[K], Chunk<T> (&dy)[K], float& eps, boo
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     float f[V];
-    unpack<T, V>(x[k], f);
+    unpack<T>(x[k], f);
 #pragma unroll
     for (int e = 0; e < V; ++e) big = max(big, __float_as_uint(f[e]) & 0x7fffffffu);
   }
@@ -100,10 +100,10 @@ __device__ void rescale_row(Chunk<T> (&x)[K], Chunk<T> (&dy)[K], float& eps, boo
   eps = __builtin_amdgcn_ldexpf(eps, shift);
   auto move = [&](Chunk<T>& c) {
     float f[V];
-    unpack<T, V>(c, f);
+    unpack<T>(c, f);
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = __builtin_amdgcn_ldexpf(f[e], shift);
-    c = pack<T, V>(f);
+    c = pack<T>(f);
   };
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -184,11 +184,11 @@ __global__ __launch_bounds__(row_threads(G)) void unit_rows_kernel(UnitRows a) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const S* xr = x + at[u].seq * a.x_seq + at[u].t * a.x_row;
-        raw[u][k] = at[u].real ? load_pieces<T, V>(xr, (j + k * G) * V, dim) : Chunk<T>{};
+        raw[u][k] = at[u].real ? load_pieces<T>(xr, (j + k * G) * V, dim) : Chunk<T>{};
         if constexpr (BACKWARD) {
           const S* dr = a.offsets ? dy + at[u].packed * dim
                                   : dy + at[u].seq * a.dy_seq + at[u].t * a.dy_row;
-          raw_d[u][k] = at[u].real ? load_pieces<T, V>(dr, (j + k * G) * V, dim) : Chunk<T>{};
+          raw_d[u][k] = at[u].real ? load_pieces<T>(dr, (j + k * G) * V, dim) : Chunk<T>{};
         }
       }
   };
@@ -201,8 +201,8 @@ __global__ __launch_bounds__(row_threads(G)) void unit_rows_kernel(UnitRows a) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float f[V], d[V];
-        unpack<T, V>(raw[u][k], f);
-        if constexpr (BACKWARD) unpack<T, V>(raw_d[u][k], d);
+        unpack<T>(raw[u][k], f);
+        if constexpr (BACKWARD) unpack<T>(raw_d[u][k], d);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           sums[u] += f[e] * f[e];
@@ -231,14 +231,14 @@ __global__ __launch_bounds__(row_threads(G)) void unit_rows_kernel(UnitRows a) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float f[V], d[V];
-        unpack<T, V>(raw[u][k], f);
-        if constexpr (BACKWARD) unpack<T, V>(raw_d[u][k], d);
+        unpack<T>(raw[u][k], f);
+        if constexpr (BACKWARD) unpack<T>(raw_d[u][k], d);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           if constexpr (BACKWARD) f[e] = d[e] - f[e] * along;
           f[e] = real ? f[e] * scale : 0.0f;
         }
-        store_chunk<T, V>(to, (j + k * G) * V, dim, f);
+        store_chunk<T>(to, (j + k * G) * V, dim, f);
       }
     }
   };
