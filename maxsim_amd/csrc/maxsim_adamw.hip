@@ -7,8 +7,8 @@
 // Memory-bound: 28 bytes per element in fp32, 10 in bf16 with 8-bit states.
 // A launch takes up to kTensors tensors by their addresses in its arguments
 // (nothing is copied to the device or kept there) and cuts each into chunks,
-// one per workgroup; a workgroup finds its tensor by bisection of the chunk
-// counts.
+// one per workgroup; a workgroup finds its tensor by one load of the first
+// chunks' numbers, a tensor per lane, and a count of those up to its own.
 //
 // 8-bit states.  A block of 256 elements of a tensor shares, per state, one
 // byte: the exponent field E of its largest magnitude.  The code of an element
@@ -17,7 +17,8 @@
 // (v: 5 and 3 bits, no sign), so that the block's small values reach into
 // fp32's subnormal numbers, whose even spacing is the codes' own lowest step.
 // The 20 bits below the cut decide the rounding, up or down in proportion, by
-// adding 20 random bits: with b2 = 0.999 a second moment moves by a thousandth
+// adding 16 random bits in their upper places and half of the last of those (a
+// rounding to 2^-16 of a step, without a bias): with b2 = 0.999 a second moment moves by a thousandth
 // per step, and nearest rounding to steps of an eighth would never let it
 // move.  The random bits are a hash of the element's position, the step and a
 // seed: the same call gives the same bits.  A second moment above 0 keeps a
@@ -49,8 +50,8 @@ constexpr int64_t kMaxChunks = UINT32_MAX / kAdamThreads;  // of a launch: threa
 // arithmetic per element, and needs all eight.
 constexpr unsigned kReservedLds = 56 << 10;
 
-// The tensors of a launch, as many as 4 KB of kernel arguments hold (88 in
-// the plain 32-bit step, 61 with 8-bit states and masters).
+// The tensors of a launch, as many as 4 KB of kernel arguments hold (90 in
+// the plain 32-bit step, 62 with 8-bit states and masters).
 template <int BITS, bool MASTER> struct AdamArgs {
   static constexpr int kTensors =
       (4096 - 128) / (5 * 8 + 4 + (BITS == 8 ? 8 + 4 : 0) + (MASTER ? 8 : 0));

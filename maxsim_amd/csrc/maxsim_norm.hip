@@ -316,8 +316,10 @@ static int workgroups_for(int64_t in_flight, int64_t bytes_each) {
 // Workgroups of the backward, at most kMaxPartials (what the workspace holds
 // partial rows for) and with at least kLeastTurns turns each where there are
 // more turns than CUs: a workgroup costs a partial row of 8 dim bytes, written
-// and read again (18433 x 301 fp32 17.7 us, with eight turns 19.0; 2049 x 2560
-// bf16 15.9 and 16.9, 4000 x 2048 16.4 and 15.2, 16000 x 768 18.8 with either).
+// and read again.  Four is no sharp optimum: 18433 x 301 fp32 takes 17.7 us
+// with four and 19.0 with eight, 2049 x 2560 bf16 15.9 and 16.9, 16000 x 768
+// 18.8 with either, and 4000 x 2048 is better with eight, 16.4 and 15.2.  How
+// evenly the turns divide, which this rule does not look at, counts as much.
 constexpr int64_t kMaxPartials = 1024;
 constexpr int64_t kLeastTurns = 4;
 static int64_t backward_blocks(int64_t turns, int64_t cus, int64_t per_cu) {

@@ -139,7 +139,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
             update and decay together, is rounded once, to the value's
             spacing.)
         seed: of the random rounding of 8-bit states, which depends on
-            (seed, step, position of the element in the lists) alone.
+            (seed, step, position of the element in the lists) alone; its low
+            32 bits count.
 
     8-bit states keep 4 significant bits per element and a power-of-two scale
     per 256; they are rounded up or down at random in proportion, so that the

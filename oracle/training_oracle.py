@@ -120,8 +120,9 @@ LOWEST = {True: 32, False: 48}
 
 
 def dither(position, step, seed):
-    """The 20 random bits of the first and second moment of the elements at
-    ``position`` (uint64 array)."""
+    """What is added to the 20 bits below a code of the first and second moment
+    of the elements at ``position`` (uint64 array): 16 random bits, and half of
+    the last of them."""
     low = np.uint64(0xFFFFFFFF)
     key = np.uint64((seed * 0x9E3779B1 + step * 0x3C6EF373) & 0xFFFFFFFF)
     with np.errstate(over="ignore"):
