@@ -20,8 +20,8 @@ of fp32 gradients would give, without the separate cast pass.
 
 Not in ``__all__``, which stays the reference's list: the training loss
 (:func:`score_contrastive_cross_entropy`), :func:`pack_documents`, and the
-operators around the scores (:mod:`maxsim_amd.training`: layer norm, unit
-embeddings, AdamW).
+operators around the scores (:mod:`maxsim_amd.training`: token embeddings,
+layer norm, unit embeddings, gradient clipping, AdamW).
 
 The pure-PyTorch ``*_reference`` functions of the reference package are
 exported too (:mod:`maxsim_amd.reference`) for benchmarks and comparisons;
@@ -55,6 +55,10 @@ from .training import (
     AdamW,
     adamw_state_values,
     adamw_step,
+    clip_factor,
+    clip_grad_norm,
+    embed_tokens,
+    grad_norm,
     layer_norm,
     normalize_embeddings,
     pack_normalized_documents,

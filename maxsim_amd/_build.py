@@ -3,8 +3,8 @@
 Produces, next to this file:
 
 * ``libmaxsim_amd.so`` -- the HIP kernels and the C ABI of
-  ``include/maxsim_amd.h`` and ``include/maxsim_amd_training.h`` (hipcc,
-  gfx950; no torch dependency);
+  ``include/maxsim_amd.h``, ``include/maxsim_amd_training.h`` and
+  ``include/maxsim_amd_encoder.h`` (hipcc, gfx950; no torch dependency);
 * ``_maxsim_amd_torch.so`` -- the torch operator registrations
   (``torch_binding.cpp``, ``torch_training.cpp``), linked against
   ``libmaxsim_amd.so``.
@@ -32,7 +32,7 @@ ARCH = os.environ.get("MAXSIM_AMD_ARCH", "gfx950")
 
 HIP_SOURCES = ["maxsim_fwd.hip", "maxsim_kloop.hip", "maxsim_bwd.hip", "maxsim_pack.hip",
                "maxsim_ce.hip", "maxsim_check.hip", "maxsim_norm.hip", "maxsim_unit.hip",
-               "maxsim_adamw.hip", "maxsim_capi.hip"]
+               "maxsim_adamw.hip", "maxsim_gradnorm.hip", "maxsim_embed.hip", "maxsim_capi.hip"]
 TORCH_SOURCES = ["torch_binding.cpp", "torch_training.cpp"]
 LIB = PKG / "libmaxsim_amd.so"  # the two libraries, where they are loaded from
 TORCH_LIB = PKG / "_maxsim_amd_torch.so"

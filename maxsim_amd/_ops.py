@@ -14,10 +14,10 @@ are the fused training loss behind
 :func:`maxsim_amd.score_contrastive_cross_entropy`.  ``maxsim_check_padded``,
 ``maxsim_check_packed`` and ``maxsim_check_contrastive`` queue a device-side
 check of a call's offsets, ids or lengths and return the words that
-``maxsim_check_wait`` waits for.  ``maxsim_layer_norm``,
+``maxsim_check_wait`` waits for.  ``maxsim_embed_tokens``, ``maxsim_layer_norm``,
 ``maxsim_normalize_embeddings``, ``maxsim_pack_normalized`` (differentiable in
-C++), ``maxsim_adamw_step`` and their parts are behind
-:mod:`maxsim_amd.training`.
+C++), ``maxsim_clip_factor``, ``maxsim_clip_grad_norm``, ``maxsim_adamw_step``
+and their parts are behind :mod:`maxsim_amd.training`.
 
 Importing this module loads ``_maxsim_amd_torch.so`` (which pulls in
 ``libmaxsim_amd.so``).  There is no fallback: if the native build is missing
@@ -187,8 +187,34 @@ def _(dy, x, lengths, offsets, eps):
 
 @torch.library.register_fake("maxsim_amd::maxsim_adamw_step")
 def _(params, grads, exp_avgs, exp_avg_sqs, scales, masters, lr, lr_tensor, beta1, beta2, eps,
-      weight_decay, step, step_tensor, seed):
+      weight_decay, step, step_tensor, seed, grad_scale=None):
     return None
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_embed_tokens")
+def _(weight, ids, lengths, scale, padding_idx, dtype):
+    return weight.new_empty((*ids.shape, weight.shape[1]), dtype=dtype or weight.dtype)
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_embed_tokens_forward")
+def _(weight, ids, lengths, scale, padding_idx, dtype):
+    return (weight.new_empty((*ids.shape, weight.shape[1]), dtype=dtype or weight.dtype),
+            _i32(weight, (ids.numel(),)))
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_embed_tokens_backward")
+def _(dy, rows, vocab, scale, weight_dtype):
+    return dy.new_empty((vocab, dy.shape[-1]), dtype=weight_dtype)
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_clip_factor")
+def _(grads, max_norm, eps):
+    return _f32(grads[0], ()), _f32(grads[0], ())
+
+
+@torch.library.register_fake("maxsim_amd::maxsim_clip_grad_norm")
+def _(grads, max_norm, eps):
+    return _f32(grads[0], ())
 
 
 @torch.library.register_fake("maxsim_amd::maxsim_adamw_state_values")

@@ -29,7 +29,7 @@
 
 #include "maxsim_host.h"
 #include "maxsim_rows.h"
-#include "../../include/maxsim_amd_training.h"
+#include "../../include/maxsim_amd_encoder.h"
 
 namespace maxsim {
 
@@ -71,6 +71,7 @@ template <int BITS, bool MASTER> struct AdamArgs {
   // read on the device where given: the learning rate, and the step count
   const float* lr_at;
   const int64_t* step_at;
+  const float* grad_scale;  // what gradients are multiplied by; NULL: 1
   float weight_decay;
   double beta1, beta2;
   uint64_t seed;
@@ -225,6 +226,7 @@ __device__ __forceinline__ uint2 top_bytes(const uint32_t (&q)[8]) {
 struct AdamStep {
   float decay, size, root;  // lr weight_decay, lr / c1, 1 / sqrt(c2)
   uint32_t key;
+  float grad_scale;
 };
 
 // Tensor k's elements from base on.  The quotient is a product with the
@@ -256,6 +258,10 @@ __device__ __forceinline__ void adam_chunk(const AdamArgs<BITS, MASTER>& a, int 
   } else {
     load8<F32, FULL>(a.m[k], i, n, m);
     load8<F32, FULL>(a.v[k], i, n, v);
+  }
+  if (a.grad_scale) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] *= h.grad_scale;
   }
   uint32_t big_m = 0, big_v = 0;
 #pragma unroll
@@ -327,7 +333,7 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs<BITS, MAST
     c1 = c[0], c2 = c[1];
     key = dither_key(a.seed, (uint64_t)step);
   }
-  const AdamStep h{decay, lr / c1, 1.0f / sqrtf(c2), key};
+  const AdamStep h{decay, lr / c1, 1.0f / sqrtf(c2), key, a.grad_scale ? *a.grad_scale : 1.0f};
   const int64_t base = (int64_t)(chunk - a.first[k]) * kChunkElems;
   if (base + kChunkElems <= a.n[k]) adam_chunk<P, Gr, BITS, MASTER, true>(a, k, h, base);
   else adam_chunk<P, Gr, BITS, MASTER, false>(a, k, h, base);
@@ -367,6 +373,17 @@ int maxsim_amd_adamw_step(maxsim_dtype param_dtype, maxsim_dtype grad_dtype, int
                           const float* lr_on_device, double beta1, double beta2, double eps,
                           double weight_decay, int64_t step, const int64_t* step_on_device,
                           uint64_t seed, void* stream) {
+  return maxsim_amd_adamw_step_scaled(param_dtype, grad_dtype, state_bits, tensors, count, nullptr,
+                                      lr, lr_on_device, beta1, beta2, eps, weight_decay, step,
+                                      step_on_device, seed, stream);
+}
+
+int maxsim_amd_adamw_step_scaled(maxsim_dtype param_dtype, maxsim_dtype grad_dtype, int state_bits,
+                                 const maxsim_adamw_tensor* tensors, int64_t count,
+                                 const float* grad_scale, double lr, const float* lr_on_device,
+                                 double beta1, double beta2, double eps, double weight_decay,
+                                 int64_t step, const int64_t* step_on_device, uint64_t seed,
+                                 void* stream) {
   clear_error();
   if (int e = check_dtype(param_dtype)) return e;
   if (int e = check_dtype(grad_dtype)) return e;
@@ -411,7 +428,7 @@ int maxsim_amd_adamw_step(maxsim_dtype param_dtype, maxsim_dtype grad_dtype, int
     a.c1 = (float)(1.0 - std::pow(beta1, (double)step));
     a.c2 = (float)(1.0 - std::pow(beta2, (double)step));
     a.key = dither_key(seed, (uint64_t)step);
-    a.lr_at = lr_on_device, a.step_at = step_on_device;
+    a.lr_at = lr_on_device, a.step_at = step_on_device, a.grad_scale = grad_scale;
     a.beta1 = beta1, a.beta2 = beta2, a.seed = seed;
     uint32_t chunks = 0;
     auto launch = [&] {

@@ -1,0 +1,262 @@
+// The norm of many gradients together, the factor that clips them to a limit,
+// and clipping in place.
+//
+//   norm = sqrt(sum_i |g_i|^2),  factor = min(1, max_norm / (norm + eps))
+//
+// Memory-bound: every gradient is read once (and written once where it is
+// clipped).  A launch takes up to kTensors tensors by their addresses in its
+// arguments and cuts each into chunks, one per workgroup, that finds its
+// tensor as adamw_kernel does.  Squares are added in 64 bits: no gradient is
+// too large or too small for them, and their order matters to no digit that
+// is kept.  Each chunk's sum is stored, and one workgroup adds them up: no
+// atomics, the same bits every time, and nothing to clear before a call.
+#include <cmath>
+
+#include "maxsim_host.h"
+#include "maxsim_rows.h"
+#include "../../include/maxsim_amd_encoder.h"
+
+namespace maxsim {
+
+constexpr int kGradThreads = 256;
+constexpr int kGradUnroll = 8;                // chunks of 16 bytes in flight per thread
+constexpr int kGradTurns = 2;
+constexpr int64_t kGradBytes = (int64_t)kGradThreads * 16 * kGradUnroll * kGradTurns;  // of a workgroup
+constexpr int64_t kGradMaxChunks = UINT32_MAX / kGradThreads;  // of a launch: threads in 32 bits
+constexpr int kJoinThreads = 1024;
+
+struct GradArgs {
+  static constexpr int kTensors = (4096 - 128) / 20;
+  void* p[kTensors];
+  uint64_t n[kTensors];      // 4 * elements + type
+  uint32_t first[kTensors];  // number of the tensor's first chunk
+  int count;
+  double* sums;         // of the launch's chunks
+  const float* factor;  // clipping in place
+};
+static_assert(sizeof(GradArgs) <= 4096, "kernel arguments");
+
+// The last tensor that starts at or before this chunk.
+__device__ __forceinline__ int tensor_of(const GradArgs& a, uint32_t chunk) {
+  const int lane = threadIdx.x & 63;
+  int k = -1;
+#pragma unroll
+  for (int i = 0; i < GradArgs::kTensors; i += 64)
+    k += __popcll(__ballot(i + lane < a.count && a.first[min(i + lane, a.count - 1)] <= chunk));
+  return k;
+}
+
+// Sum over the workgroup in thread 0, lanes and then waves in one order.
+template <int THREADS>
+__device__ __forceinline__ double block_sum(double s) {
+  __shared__ double waves[THREADS / 64];
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) s += __shfl_xor(s, off, 64);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = waves[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) s += waves[w];
+  return s;
+}
+
+// Squares of elements [at, end) of p.
+template <typename T>
+__device__ __forceinline__ double squares(const void* p, int64_t at, int64_t end) {
+  constexpr int V = kVec<T>;
+  const auto* g = static_cast<const typename T::storage*>(p);
+  double s[2] = {0.0, 0.0};
+  int64_t i = at + threadIdx.x * V;
+  constexpr int64_t step = kGradThreads * V;
+  for (; i + (kGradUnroll - 1) * step + V <= end; i += kGradUnroll * step) {
+    Chunk<T> c[kGradUnroll];
+#pragma unroll
+    for (int u = 0; u < kGradUnroll; ++u) c[u] = load_any<Chunk<T>>(g + i + u * step);
+#pragma unroll
+    for (int u = 0; u < kGradUnroll; ++u) {
+      float f[V];
+      unpack<T>(c[u], f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[e & 1] = fma((double)f[e], (double)f[e], s[e & 1]);
+    }
+  }
+  for (; i < end; i += step) {
+    if (i + V <= end) {
+      float f[V];
+      unpack<T>(load_any<Chunk<T>>(g + i), f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[e & 1] = fma((double)f[e], (double)f[e], s[e & 1]);
+    } else {
+      for (int64_t e = i; e < end; ++e) {
+        const double d = to_float<T>(g[e]);
+        s[0] = fma(d, d, s[0]);
+      }
+    }
+  }
+  return s[0] + s[1];
+}
+
+__global__ __launch_bounds__(kGradThreads) void grad_squares_kernel(GradArgs a) {
+  const int k = tensor_of(a, blockIdx.x);
+  const int64_t n = (int64_t)(a.n[k] >> 2);
+  const int type = (int)(a.n[k] & 3);
+  const int64_t each = kGradBytes / (type == MAXSIM_FLOAT32 ? 4 : 2);
+  const int64_t at = (int64_t)(blockIdx.x - a.first[k]) * each, end = min(at + each, n);
+  double s;
+  if (type == MAXSIM_FLOAT32) s = squares<F32>(a.p[k], at, end);
+  else if (type == MAXSIM_FLOAT16) s = squares<F16>(a.p[k], at, end);
+  else s = squares<BF16>(a.p[k], at, end);
+  s = block_sum<kGradThreads>(s);
+  if (threadIdx.x == 0) a.sums[blockIdx.x] = s;
+}
+
+__global__ __launch_bounds__(kJoinThreads) void grad_norm_kernel(const double* __restrict__ sums,
+                                                                 int64_t count, double max_norm,
+                                                                 double eps, float* norm,
+                                                                 float* factor) {
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < count; i += kJoinThreads) s += sums[i];
+  s = block_sum<kJoinThreads>(s);
+  if (threadIdx.x != 0) return;
+  const double root = sqrt(s);
+  *norm = (float)root;
+  if (!factor) return;
+  const double f = max_norm / (root + eps);
+  *factor = f > 1.0 ? 1.0f : (float)f;  // NaN stays
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_chunk(void* p, int64_t at, int64_t end, float factor) {
+  constexpr int V = kVec<T>;
+  auto* g = static_cast<typename T::storage*>(p);
+  constexpr int64_t step = kGradThreads * V;
+  int64_t i = at + threadIdx.x * V;
+  auto scaled = [&](const Chunk<T>& c) {
+    float f[V];
+    unpack<T>(c, f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] *= factor;
+    return pack<T>(f);
+  };
+  for (; i + (kGradUnroll - 1) * step + V <= end; i += kGradUnroll * step) {
+    Chunk<T> c[kGradUnroll];
+#pragma unroll
+    for (int u = 0; u < kGradUnroll; ++u) c[u] = load_any<Chunk<T>>(g + i + u * step);
+#pragma unroll
+    for (int u = 0; u < kGradUnroll; ++u) store_any(g + i + u * step, scaled(c[u]));
+  }
+  for (; i < end; i += step) {
+    if (i + V <= end) {
+      store_any(g + i, scaled(load_any<Chunk<T>>(g + i)));
+    } else {
+      for (int64_t e = i; e < end; ++e) g[e] = from_float<T>(to_float<T>(g[e]) * factor);
+    }
+  }
+}
+
+__global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(GradArgs a) {
+  const float factor = *a.factor;
+  if (factor == 1.0f) return;  // every element stays what it is
+  const int k = tensor_of(a, blockIdx.x);
+  const int64_t n = (int64_t)(a.n[k] >> 2);
+  const int type = (int)(a.n[k] & 3);
+  const int64_t each = kGradBytes / (type == MAXSIM_FLOAT32 ? 4 : 2);
+  const int64_t at = (int64_t)(blockIdx.x - a.first[k]) * each, end = min(at + each, n);
+  if (type == MAXSIM_FLOAT32) scale_chunk<F32>(a.p[k], at, end, factor);
+  else if (type == MAXSIM_FLOAT16) scale_chunk<F16>(a.p[k], at, end, factor);
+  else scale_chunk<BF16>(a.p[k], at, end, factor);
+}
+
+static int64_t grad_chunks(const maxsim_grad_tensor& t) {
+  const int64_t each = kGradBytes / (t.dtype == MAXSIM_FLOAT32 ? 4 : 2);
+  return t.numel / each + (t.numel % each != 0);
+}
+
+static int check_grads(const maxsim_grad_tensor* tensors, int64_t count) {
+  if (count < 0 || (count > 0 && !tensors)) return fail(MAXSIM_ERR_INVALID, "no tensors");
+  for (int64_t i = 0; i < count; ++i) {
+    if (int e = check_dtype(tensors[i].dtype)) return e;
+    if (tensors[i].numel < 0) return fail(MAXSIM_ERR_INVALID, "negative size");
+    if (tensors[i].numel > 0 && !tensors[i].grad)
+      return fail(MAXSIM_ERR_INVALID, "null pointer argument");
+    if (grad_chunks(tensors[i]) > kGradMaxChunks)
+      return fail(MAXSIM_ERR_UNSUPPORTED, "tensor too large for one launch");
+  }
+  return MAXSIM_OK;
+}
+
+// Calls launch(arguments, chunks) for as many tensors as an argument list holds.
+template <typename F>
+static int for_grads(const maxsim_grad_tensor* tensors, int64_t count, F&& launch) {
+  GradArgs a{};
+  uint32_t chunks = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const maxsim_grad_tensor& t = tensors[i];
+    if (t.numel == 0) continue;
+    const uint32_t more = (uint32_t)grad_chunks(t);
+    if (a.count == GradArgs::kTensors || (uint64_t)chunks + more > (uint64_t)kGradMaxChunks) {
+      if (int e = launch(a, chunks)) return e;
+      a.count = 0, chunks = 0;
+    }
+    const int k = a.count++;
+    a.p[k] = t.grad, a.n[k] = (uint64_t)t.numel * 4 + (uint64_t)t.dtype, a.first[k] = chunks;
+    chunks += more;
+  }
+  return a.count > 0 ? launch(a, chunks) : MAXSIM_OK;
+}
+
+}  // namespace maxsim
+
+using namespace maxsim;
+
+extern "C" {
+
+size_t maxsim_amd_grad_norm_workspace_size(const maxsim_grad_tensor* tensors, int64_t count) {
+  if (check_grads(tensors, count) != MAXSIM_OK) return 0;
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < count; ++i) chunks += grad_chunks(tensors[i]);
+  return (size_t)chunks * sizeof(double);
+}
+
+int maxsim_amd_grad_norm(const maxsim_grad_tensor* tensors, int64_t count, double max_norm,
+                         double eps, float* norm, float* factor, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int e = check_grads(tensors, count)) return e;
+  if (!norm) return fail(MAXSIM_ERR_INVALID, "null pointer argument");
+  if (factor && (!(max_norm >= 0.0) || !(eps >= 0.0)))
+    return fail(MAXSIM_ERR_INVALID, "max_norm and eps must be >= 0");
+  int64_t all = 0;
+  for (int64_t i = 0; i < count; ++i) all += grad_chunks(tensors[i]);
+  if (all > 0 && (!workspace || workspace_bytes < (size_t)all * sizeof(double)))
+    return fail(MAXSIM_ERR_INVALID, "workspace too small: %zu bytes, %zu needed", workspace_bytes,
+                (size_t)all * sizeof(double));
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  double* sums = static_cast<double*>(workspace);
+  int64_t at = 0;
+  const int rc = for_grads(tensors, count, [&](GradArgs& a, uint32_t chunks) {
+    a.sums = sums + at;
+    at += chunks;
+    hipLaunchKernelGGL(grad_squares_kernel, dim3(chunks), dim3(kGradThreads), 0, st, a);
+    return check_launch("grad_squares_kernel");
+  });
+  if (rc != MAXSIM_OK) return rc;
+  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kJoinThreads), 0, st, sums, all, max_norm, eps,
+                     norm, factor);
+  return check_launch("grad_norm_kernel");
+}
+
+int maxsim_amd_scale_grads(const maxsim_grad_tensor* tensors, int64_t count, const float* factor,
+                           void* stream) {
+  clear_error();
+  if (int e = check_grads(tensors, count)) return e;
+  if (!factor) return fail(MAXSIM_ERR_INVALID, "null pointer argument");
+  return for_grads(tensors, count, [&](GradArgs& a, uint32_t chunks) {
+    a.factor = factor;
+    hipLaunchKernelGGL(grad_scale_kernel, dim3(chunks), dim3(kGradThreads), 0,
+                       static_cast<hipStream_t>(stream), a);
+    return check_launch("grad_scale_kernel");
+  });
+}
+
+}  // extern "C"

@@ -1,5 +1,6 @@
-// Torch binding of the operators around the scoring kernels (layer norm, unit
-// rows, AdamW) over the C ABI of include/maxsim_amd_training.h.
+// Torch binding of the operators around the scoring kernels (token embeddings,
+// layer norm, unit rows, the gradients' norm, AdamW) over the C ABI of
+// include/maxsim_amd_training.h and include/maxsim_amd_encoder.h.
 //
 // The differentiable ones are C++ autograd functions: their backward runs on
 // the engine's thread without the interpreter, and both directions go through
@@ -15,12 +16,13 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <cmath>
 #include <map>
 #include <optional>
 #include <tuple>
 #include <vector>
 
-#include "../../include/maxsim_amd_training.h"
+#include "../../include/maxsim_amd_encoder.h"
 #include "torch_common.h"
 
 namespace {
@@ -361,6 +363,114 @@ Tensor maxsim_pack_normalized_backward(const Tensor& dy, const Tensor& x, const 
   return unit_backward(dy, x, lengths_of(lengths), offsets, dy.size(0), eps);
 }
 
+// ---- token embeddings ----------------------------------------------------------
+
+struct Embed {
+  Tensor weight, ids;
+  Lengths lengths;
+  int64_t vocab, dim, stride, sequences, length;
+  maxsim_dtype weight_dtype, dtype;
+  at::ScalarType type;
+  std::vector<int64_t> sizes;  // of the result
+};
+
+Embed prep_embed(const Tensor& weight, const Tensor& ids, const optional<Tensor>& lengths,
+                 double scale, int64_t padding_idx, optional<at::ScalarType> dtype) {
+  Embed e;
+  e.weight_dtype = dtype_of(weight, "weight");
+  TORCH_CHECK_VALUE(weight.dim() == 2, "weight must be 2-D [vocab, dim]; got ", weight.sizes());
+  e.vocab = weight.size(0), e.dim = weight.size(1);
+  TORCH_CHECK_VALUE(e.dim > 0, "dim must be > 0; got ", e.dim);
+  TORCH_CHECK_TYPE(ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong,
+                   "ids must be int32 or int64; got ", ids.scalar_type());
+  e.type = dtype.value_or(weight.scalar_type());
+  TORCH_CHECK_TYPE(e.type == weight.scalar_type() ||
+                       (weight.scalar_type() == at::kFloat &&
+                        (e.type == at::kHalf || e.type == at::kBFloat16)),
+                   "dtype must be weight's, or float16 or bfloat16 of a float32 weight; got ",
+                   e.type, " of ", weight.scalar_type());
+  e.dtype = e.type == at::kFloat ? MAXSIM_FLOAT32 : e.type == at::kHalf ? MAXSIM_FLOAT16
+                                                                        : MAXSIM_BFLOAT16;
+  TORCH_CHECK_VALUE(std::isfinite((float)scale), "scale must be finite; got ", scale);
+  TORCH_CHECK_VALUE(padding_idx >= -1 && padding_idx < std::max<int64_t>(e.vocab, 1),
+                    "padding_idx must be a row of weight; got ", padding_idx);
+  check_hip(weight, "weight");
+  check_same_device(ids, "ids", weight, "weight");
+  if (lengths.has_value()) {
+    TORCH_CHECK_VALUE(ids.dim() == 2, "ids must be 2-D [N, L] where lengths are given; got ",
+                      ids.sizes());
+    check_lengths(*lengths);
+    TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == ids.size(0),
+                      "lengths must have shape [N=", ids.size(0), "]; got ", lengths->sizes());
+    check_same_device(*lengths, "lengths", weight, "weight");
+    e.sequences = ids.size(0), e.length = ids.size(1);
+  } else {
+    e.sequences = ids.numel(), e.length = 1;
+  }
+  // rows may lie anywhere, their elements side by side
+  e.weight = e.dim > 1 && weight.stride(1) != 1 ? weight.contiguous() : weight;
+  e.stride = e.weight.stride(0);
+  e.ids = ids.contiguous();
+  e.lengths = lengths_of(lengths);
+  e.sizes = ids.sizes().vec();
+  e.sizes.push_back(e.dim);
+  return e;
+}
+
+Tensor run_embed(const Embed& e, double scale, int64_t padding_idx, int32_t* rows) {
+  Tensor y = empty_like_on(e.weight, e.sizes, e.type);
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(e.weight.device());
+  check_status(maxsim_amd_embed_forward(
+      e.weight_dtype, e.dtype, e.weight.data_ptr(), e.vocab, e.dim, e.stride, e.ids.data_ptr(),
+      e.ids.scalar_type() == at::kLong, e.sequences, e.length, e.lengths.data, e.lengths.is64,
+      (float)scale, padding_idx, y.data_ptr(), rows, current_stream(e.weight)));
+  return y;
+}
+
+// padding_idx: -1 for none.
+Tensor maxsim_embed_tokens(const Tensor& weight, const Tensor& ids,
+                           const optional<Tensor>& lengths, double scale, int64_t padding_idx,
+                           optional<at::ScalarType> dtype) {
+  return run_embed(prep_embed(weight, ids, lengths, scale, padding_idx, dtype), scale, padding_idx,
+                   nullptr);
+}
+
+// With what the backward needs: each token's row of weight, -1 where it has none.
+std::tuple<Tensor, Tensor> maxsim_embed_tokens_forward(const Tensor& weight, const Tensor& ids,
+                                                       const optional<Tensor>& lengths,
+                                                       double scale, int64_t padding_idx,
+                                                       optional<at::ScalarType> dtype) {
+  const Embed e = prep_embed(weight, ids, lengths, scale, padding_idx, dtype);
+  Tensor rows = empty_like_on(weight, {e.ids.numel()}, at::kInt);
+  return {run_embed(e, scale, padding_idx, rows.data_ptr<int32_t>()), rows};
+}
+
+Tensor maxsim_embed_tokens_backward(const Tensor& dy, const Tensor& rows, int64_t vocab,
+                                    double scale, at::ScalarType weight_dtype) {
+  const maxsim_dtype dt = dtype_of(dy, "dy");
+  check_hip(dy, "dy");
+  TORCH_CHECK_VALUE(dy.dim() >= 1 && dy.size(-1) > 0 && vocab >= 0,
+                    "dy must be [..., dim] and vocab >= 0; got ", dy.sizes(), " and ", vocab);
+  const int64_t dim = dy.size(-1);
+  TORCH_CHECK(rows.scalar_type() == at::kInt && rows.is_contiguous() &&
+                  rows.numel() * dim == dy.numel(),
+              "rows must be contiguous int32, one for each row of dy");
+  check_same_device(rows, "rows", dy, "dy");
+  TORCH_CHECK_TYPE(weight_dtype == dy.scalar_type() || weight_dtype == at::kFloat,
+                   "weight_dtype must be dy's or float32; got ", weight_dtype);
+  const int64_t tokens = rows.numel();
+  const Rows r = rows_of(dy, 0);
+  Tensor dw = empty_like_on(dy, {vocab, dim}, weight_dtype);
+  const size_t bytes = maxsim_amd_embed_backward_workspace_size(dt, tokens, vocab, dim);
+  Tensor ws = empty_like_on(dy, {(int64_t)bytes}, at::kByte);
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
+  check_status(maxsim_amd_embed_backward(dtype_of(dw, "weight"), dt, r.t.data_ptr(),
+                                         r.inner_stride, rows.data_ptr<int32_t>(), tokens, vocab,
+                                         dim, (float)scale, dw.data_ptr(), ws.data_ptr(), bytes,
+                                         current_stream(dy)));
+  return dw;
+}
+
 // ---- autograd ----------------------------------------------------------------
 
 // An operator of this library through the dispatcher, looked up once.
@@ -511,6 +621,40 @@ Tensor pack_normalized_autograd(const Tensor& x, const Tensor& lengths, const Te
   return MAXSIM_CALL(maxsim_pack_normalized, x, lengths, offsets, packed_rows, eps);
 }
 
+struct EmbedFn : torch::autograd::Function<EmbedFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids,
+                        const optional<Tensor>& lengths, double scale, int64_t padding_idx,
+                        optional<at::ScalarType> dtype) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [y, rows] =
+        MAXSIM_CALL(maxsim_embed_tokens_forward, weight, ids, lengths, scale, padding_idx, dtype);
+    ctx->save_for_backward({rows});
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["dtype"] = (int64_t)weight.scalar_type();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto run = [&] {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      return MAXSIM_CALL(maxsim_embed_tokens_backward, grads[0], saved[0],
+                         ctx->saved_data["vocab"].toInt(), ctx->saved_data["scale"].toDouble(),
+                         (at::ScalarType)ctx->saved_data["dtype"].toInt());
+    };
+    return backward_results({run()}, 6, grads[0], saved[0], std::nullopt);
+  }
+};
+
+Tensor embed_autograd(const Tensor& weight, const Tensor& ids, const optional<Tensor>& lengths,
+                      double scale, int64_t padding_idx, optional<at::ScalarType> dtype) {
+  refuse_tangents("embed_tokens", weight);
+  if (at::GradMode::is_enabled() && wants(weight))
+    return EmbedFn::apply(weight, ids, lengths, scale, padding_idx, dtype);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return MAXSIM_CALL(maxsim_embed_tokens, weight, ids, lengths, scale, padding_idx, dtype);
+}
+
 // ---- AdamW -------------------------------------------------------------------
 
 // The two tensors have their elements in the same order in memory.
@@ -590,7 +734,8 @@ void maxsim_adamw_step(at::TensorList params, at::TensorList grads, at::TensorLi
                        at::TensorList exp_avg_sqs, at::TensorList scales, at::TensorList masters,
                        double lr, const optional<Tensor>& lr_tensor, double beta1, double beta2,
                        double eps, double weight_decay, int64_t step,
-                       const optional<Tensor>& step_tensor, int64_t seed) {
+                       const optional<Tensor>& step_tensor, int64_t seed,
+                       const optional<Tensor>& grad_scale) {
   const size_t n = params.size();
   TORCH_CHECK_VALUE(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n &&
                         (scales.empty() || scales.size() == n) &&
@@ -609,6 +754,7 @@ void maxsim_adamw_step(at::TensorList params, at::TensorList grads, at::TensorLi
   if (n == 0) return;
   const Tensor* lr_at = device_scalar(lr_tensor, "lr", at::kFloat, params[0]);
   const Tensor* step_at = device_scalar(step_tensor, "step", at::kLong, params[0]);
+  const Tensor* scale_at = device_scalar(grad_scale, "grad_scale", at::kFloat, params[0]);
   const bool eight = !scales.empty();
   const at::ScalarType state = eight ? at::kByte : at::kFloat;
 
@@ -696,13 +842,95 @@ void maxsim_adamw_step(at::TensorList params, at::TensorList grads, at::TensorLi
   check_places(places);
   c10::hip::HIPGuardMasqueradingAsCUDA guard(params[0].device());
   for (const auto& [types, tensors] : groups)
-    check_status(maxsim_amd_adamw_step(
-        types.first, types.second, eight ? 8 : 32, tensors.data(), (int64_t)tensors.size(), lr,
+    check_status(maxsim_amd_adamw_step_scaled(
+        types.first, types.second, eight ? 8 : 32, tensors.data(), (int64_t)tensors.size(),
+        scale_at ? scale_at->data_ptr<float>() : nullptr, lr,
         lr_at ? lr_at->data_ptr<float>() : nullptr, beta1, beta2, eps, weight_decay, step,
         step_at ? step_at->data_ptr<int64_t>() : nullptr, (uint64_t)seed,
         current_stream(params[0])));
   for (const at::TensorList& l : {params, exp_avgs, exp_avg_sqs, scales, masters})
     for (const Tensor& t : l) touched(t);
+}
+
+// ---- the gradients' norm -------------------------------------------------------
+
+struct Grads {
+  std::vector<maxsim_grad_tensor> list;
+  std::vector<Tensor> copies;
+};
+
+// in_place: the tensors themselves are written, so that each covers its memory
+// and shares it with no other.
+Grads prep_grads(at::TensorList grads, bool in_place) {
+  Grads g;
+  g.list.reserve(grads.size());
+  std::vector<Place> places;
+  if (in_place) places.reserve(grads.size());
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& t = grads[i];
+    TORCH_CHECK_TYPE(t.layout() == at::kStrided, "grads[", i, "] must be dense");
+    const maxsim_dtype dt = dtype_of(t, "grads");
+    TORCH_CHECK(t.device() == grads[0].device(),
+                "all tensors must be on the same device; grads[0] is on ", grads[0].device(),
+                " but grads[", i, "] is on ", t.device());
+    check_hip(t, "grads");
+    const bool dense = t.is_non_overlapping_and_dense();
+    TORCH_CHECK_VALUE(dense || !in_place, "grads[", i,
+                      "] must cover its memory without gaps or overlaps");
+    if (!dense) g.copies.push_back(t.contiguous());
+    const Tensor& from = dense ? t : g.copies.back();
+    const int64_t numel = from.numel();
+    g.list.push_back({from.data_ptr(), numel, dt});
+    if (in_place && numel > 0) {
+      const auto begin = reinterpret_cast<uintptr_t>(from.data_ptr());
+      places.push_back({begin, begin + (uintptr_t)numel * from.element_size(), 0, (uint32_t)i});
+    }
+  }
+  if (!std::is_sorted(places.begin(), places.end())) std::sort(places.begin(), places.end());
+  for (size_t i = 1; i < places.size(); ++i)
+    TORCH_CHECK_VALUE(places[i - 1].end <= places[i].begin, "grads[", places[i - 1].index,
+                      "] and grads[", places[i].index, "] share memory");
+  return g;
+}
+
+void check_clip(double max_norm, double eps) {
+  TORCH_CHECK_VALUE(max_norm >= 0.0, "max_norm must be >= 0; got ", max_norm);
+  TORCH_CHECK_VALUE(eps >= 0.0 && eps < 1e30, "eps must be finite and >= 0; got ", eps);
+}
+
+// Norm and factor of what prep_grads gave.
+std::tuple<Tensor, Tensor> run_grad_norm(const Grads& g, const Tensor& like, double max_norm,
+                                         double eps) {
+  Tensor norm = empty_like_on(like, {}, at::kFloat), factor = empty_like_on(like, {}, at::kFloat);
+  const int64_t count = (int64_t)g.list.size();
+  const size_t bytes = maxsim_amd_grad_norm_workspace_size(g.list.data(), count);
+  Tensor ws = empty_like_on(like, {(int64_t)bytes}, at::kByte);
+  check_status(maxsim_amd_grad_norm(g.list.data(), count, max_norm, eps, norm.data_ptr<float>(),
+                                    factor.data_ptr<float>(), ws.data_ptr(), bytes,
+                                    current_stream(like)));
+  return {norm, factor};
+}
+
+std::tuple<Tensor, Tensor> maxsim_clip_factor(at::TensorList grads, double max_norm, double eps) {
+  check_clip(max_norm, eps);
+  TORCH_CHECK_VALUE(!grads.empty(), "needs at least one gradient");
+  at::AutoDispatchBelowADInplaceOrView below;  // a gradient's copy records nothing
+  const Grads g = prep_grads(grads, false);
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(grads[0].device());
+  return run_grad_norm(g, grads[0], max_norm, eps);
+}
+
+Tensor maxsim_clip_grad_norm(at::TensorList grads, double max_norm, double eps) {
+  check_clip(max_norm, eps);
+  TORCH_CHECK_VALUE(!grads.empty(), "needs at least one gradient");
+  at::AutoDispatchBelowADInplaceOrView below;
+  const Grads g = prep_grads(grads, true);
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(grads[0].device());
+  auto [norm, factor] = run_grad_norm(g, grads[0], max_norm, eps);
+  check_status(maxsim_amd_scale_grads(g.list.data(), (int64_t)g.list.size(),
+                                      factor.data_ptr<float>(), current_stream(grads[0])));
+  for (const Tensor& t : grads) touched(t);
+  return norm;
 }
 
 // The values of 8-bit states, in bf16 (which holds them exactly).
@@ -753,7 +981,15 @@ TORCH_LIBRARY_FRAGMENT(maxsim_amd, m) {
   m.def("maxsim_adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, "
         "Tensor(c!)[] exp_avg_sqs, Tensor(d!)[] scales, Tensor(e!)[] masters, float lr, "
         "Tensor? lr_tensor, float beta1, float beta2, float eps, float weight_decay, int step, "
-        "Tensor? step_tensor, int seed) -> ()");
+        "Tensor? step_tensor, int seed, Tensor? grad_scale=None) -> ()");
+  m.def("maxsim_embed_tokens(Tensor weight, Tensor ids, Tensor? lengths, float scale, "
+        "int padding_idx, ScalarType? dtype) -> Tensor");
+  m.def("maxsim_embed_tokens_forward(Tensor weight, Tensor ids, Tensor? lengths, float scale, "
+        "int padding_idx, ScalarType? dtype) -> (Tensor, Tensor)");
+  m.def("maxsim_embed_tokens_backward(Tensor dy, Tensor rows, int vocab, float scale, "
+        "ScalarType weight_dtype) -> Tensor");
+  m.def("maxsim_clip_factor(Tensor[] grads, float max_norm, float eps) -> (Tensor, Tensor)");
+  m.def("maxsim_clip_grad_norm(Tensor(a!)[] grads, float max_norm, float eps) -> Tensor");
   m.def("maxsim_adamw_state_values(Tensor exp_avg, Tensor exp_avg_sq, Tensor scales) "
         "-> (Tensor, Tensor)");
 }
@@ -769,17 +1005,27 @@ TORCH_LIBRARY_IMPL(maxsim_amd, CUDA, m) {
   m.impl("maxsim_pack_normalized_backward", &maxsim_pack_normalized_backward);
   m.impl("maxsim_adamw_step", &maxsim_adamw_step);
   m.impl("maxsim_adamw_state_values", &maxsim_adamw_state_values);
+  m.impl("maxsim_embed_tokens", &maxsim_embed_tokens);
+  m.impl("maxsim_embed_tokens_forward", &maxsim_embed_tokens_forward);
+  m.impl("maxsim_embed_tokens_backward", &maxsim_embed_tokens_backward);
+  m.impl("maxsim_clip_factor", &maxsim_clip_factor);
+  m.impl("maxsim_clip_grad_norm", &maxsim_clip_grad_norm);
 }
 
 // a sparse gradient comes here to be refused by name
 TORCH_LIBRARY_IMPL(maxsim_amd, SparseCUDA, m) {
   m.impl("maxsim_adamw_step", &maxsim_adamw_step);
+  m.impl("maxsim_clip_factor", &maxsim_clip_factor);
+  m.impl("maxsim_clip_grad_norm", &maxsim_clip_grad_norm);
 }
 
 TORCH_LIBRARY_IMPL(maxsim_amd, AutogradCUDA, m) {
   m.impl("maxsim_layer_norm", &layer_norm_autograd);
   m.impl("maxsim_normalize_embeddings", &normalize_autograd);
   m.impl("maxsim_pack_normalized", &pack_normalized_autograd);
+  m.impl("maxsim_embed_tokens", &embed_autograd);
   // nothing to record, and its hundreds of tensors need not be looked at for it
   m.impl("maxsim_adamw_step", torch::CppFunction::makeFallthrough());
+  m.impl("maxsim_clip_factor", torch::CppFunction::makeFallthrough());
+  m.impl("maxsim_clip_grad_norm", torch::CppFunction::makeFallthrough());
 }

@@ -1,16 +1,23 @@
-"""What lies around the scores in training and indexing: from an encoder's
-hidden states to scored token embeddings, and the step that trains both.
+"""What lies around the scores in training and indexing: from token ids and an
+encoder's hidden states to scored token embeddings, and the step that trains
+both.
 
+* :func:`embed_tokens` -- token ids looked up in an embedding table,
+  differentiable.
 * :func:`layer_norm` -- layer norm over the last axis, differentiable.
 * :func:`normalize_embeddings` -- token embeddings of unit length, those of
   padding 0; :func:`pack_normalized_documents` -- the same, packed into the
   inputs of the contrastive functions.  Differentiable.
+* :func:`grad_norm`, :func:`clip_grad_norm` and :func:`clip_factor` -- the norm
+  of all gradients together, clipping in place, and the factor that a step
+  takes gradients clipped by.
 * :func:`adamw_step` and :class:`AdamW` -- the AdamW step over many tensors in
-  a few launches, with states in 32 or 8 bits.
+  a few launches, with states in 32 or 8 bits, on clipped gradients.
 
 The reference leaves these to torch (its training example, README.md:160-205).
-Here they are hand-written HIP kernels behind ``include/maxsim_amd_training.h``:
-one pass over memory each, sums in fp32, 16-bit results rounded once.
+Here they are hand-written HIP kernels behind ``include/maxsim_amd_training.h``
+and ``include/maxsim_amd_encoder.h``: one pass over memory each, sums in fp32
+(the gradients' norm in 64 bits), 16-bit results rounded once.
 Differentiable means first derivatives in reverse mode: the gradients have no
 derivatives of their own and forward-mode tangents are not carried (both raise).
 All are exported from :mod:`maxsim_amd`.
@@ -34,6 +41,42 @@ def _require_hip(name: str, t: torch.Tensor) -> None:
     # dispatcher's error names no argument
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a HIP (torch 'cuda') tensor; got {t.device}")
+
+
+# ---------------------------------------------------------------------------
+# Token embeddings
+# ---------------------------------------------------------------------------
+def embed_tokens(weight, ids, lengths=None, *, scale: float = 1.0, padding_idx=None,
+                 dtype=None) -> torch.Tensor:
+    """``scale * weight[ids]``: the embedding of each token.
+
+    Args:
+        weight: ``[vocab, dim]`` fp32 / fp16 / bf16, dim up to 16384.  Rows may
+            be any distance apart; other layouts are copied first.
+        ids: int32/int64 of any shape.  An id outside ``[0, vocab)`` gives a
+            row of NaN and no gradient; nothing waits for the device to look.
+        lengths: ``[N]`` int32/int64 for ids ``[N, L]``: tokens at or past a
+            sequence's length become 0, have no gradient, and their ids are
+            never read.  Lengths outside ``[0, L]`` are clamped.
+        scale: multiplied in fp32 before the one rounding.
+        padding_idx: a row that is looked up like any other and gets no
+            gradient (negative ones count from the end).
+        dtype: of the result: weight's (None), or fp16 / bf16 of an fp32
+            weight.
+
+    Returns:
+        ``[*ids.shape, dim]``, differentiable with respect to weight.  The
+        gradient is dense, in weight's dtype: fp32 sums over the tokens of a
+        row, in an order that the ids alone decide, rounded once.  It takes up
+        to 2^31 - 1 tokens."""
+    _require_hip("weight", weight)
+    if padding_idx is not None:
+        rows = weight.shape[0]
+        if not -rows <= padding_idx < rows:
+            raise ValueError(f"padding_idx must be a row of weight [{rows}, ...]; got {padding_idx}")
+        padding_idx = padding_idx % rows
+    return ops.maxsim_embed_tokens(weight, ids, lengths, scale,
+                                   -1 if padding_idx is None else padding_idx, dtype)
 
 
 # ---------------------------------------------------------------------------
@@ -109,11 +152,66 @@ def pack_normalized_documents(doc_emb, doc_lengths, *,
 
 
 # ---------------------------------------------------------------------------
+# The norm of all gradients, and clipping
+# ---------------------------------------------------------------------------
+def _grad_list(grads) -> list:
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if grads:
+        _require_hip("grads", grads[0])
+    return grads
+
+
+def clip_factor(grads, max_norm: float, *, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The norm of all gradients together, and what clips them to ``max_norm``::
+
+        norm = sqrt(sum of all squares)      factor = min(1, max_norm / (norm + eps))
+
+    Args:
+        grads: fp32 / fp16 / bf16 tensors on one device (any of the types
+            together), or a single one.
+        max_norm: >= 0; infinite: the factor is 1 for every finite norm.
+
+    Returns:
+        Two fp32 tensors of one element on the gradients' device; nothing waits
+        for it.  Squares are added in 64 bits, in an order that the sizes alone
+        decide: gradients of any finite size have a norm (infinite in fp32
+        above its largest number; the factor still knows it).  A gradient that
+        is not finite makes the norm inf or NaN and the factor 0 or NaN.
+
+    The factor is :func:`adamw_step`'s ``grad_scale``: clipping then costs no
+    pass over the gradients of its own."""
+    grads = _grad_list(grads)
+    if not grads:
+        return torch.zeros(()), torch.ones(())
+    return ops.maxsim_clip_factor(grads, max_norm, eps)
+
+
+def grad_norm(grads) -> torch.Tensor:
+    """The norm of all gradients together: :func:`clip_factor`'s first result."""
+    return clip_factor(grads, math.inf)[0]
+
+
+def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6) -> torch.Tensor:
+    """Multiplies all gradients by :func:`clip_factor`'s factor, in place, and
+    returns their norm before that, as ``torch.nn.utils.clip_grad_norm_`` does
+    for parameters.
+
+    The gradients (``[p.grad for p in parameters if p.grad is not None]``) are
+    each dense in memory, in any order of their axes, and share none of it
+    (ValueError).  Products are rounded once.  Nothing is written where the
+    norm is within the limit."""
+    grads = _grad_list(grads)
+    if not grads:
+        return torch.zeros(())
+    return ops.maxsim_clip_grad_norm(grads, max_norm, eps)
+
+
+# ---------------------------------------------------------------------------
 # AdamW
 # ---------------------------------------------------------------------------
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.9, 0.999),
                eps: float = 1e-8, weight_decay: float = 1e-2, scales=None, masters=None,
-               seed: int = 0) -> None:
+               seed: int = 0, grad_scale=None) -> None:
     """One AdamW step (decoupled weight decay) over lists of tensors, in place::
 
         m = beta1 m + (1 - beta1) g        v = beta2 v + (1 - beta2) g^2
@@ -141,6 +239,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
         seed: of the random rounding of 8-bit states, which depends on
             (seed, step, position of the element in the lists) alone; its low
             32 bits count.
+        grad_scale: an fp32 tensor of one element on the device that every
+            gradient is multiplied by on its way in (:func:`clip_factor`'s
+            factor); the gradients stay as they are.  None: 1.
 
     8-bit states keep 4 significant bits per element and a power-of-two scale
     per 256; they are rounded up or down at random in proportion, so that the
@@ -159,7 +260,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     ops.maxsim_adamw_step(
         params, grads, exp_avgs, exp_avg_sqs, scales, masters,
         0.0 if lr_tensor is not None else lr, lr_tensor, betas[0], betas[1], eps, weight_decay,
-        1 if step_tensor is not None else step, step_tensor, seed)
+        1 if step_tensor is not None else step, step_tensor, seed, grad_scale)
 
 
 def adamw_state_values(exp_avg, exp_avg_sq, scales) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -195,6 +296,11 @@ class AdamW(torch.optim.Optimizer):
             that (made at the parameter's first step; the parameter itself is
             then only written).
         seed: of the random rounding of 8-bit states.
+        max_norm: clip the gradients of all groups together to this norm on
+            their way into the step (:func:`clip_factor`; they stay as they
+            are, and are on one device).  ``grad_norm`` is their norm in the
+            last step, a tensor on the device.  None: no clipping.  Not part of
+            the state dict.
 
     State of a parameter: ``step`` (an int), ``exp_avg``, ``exp_avg_sq``, and
     ``scales`` / ``master`` where they apply.  ``state_dict`` round trips keep
@@ -205,7 +311,10 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, min_8bit_size: int = 4096,
-                 master_weights: bool = False, seed: int = 0):
+                 master_weights: bool = False, seed: int = 0, max_norm=None):
+        if max_norm is not None and not max_norm >= 0.0:
+            raise ValueError(f"max_norm must be >= 0; got {max_norm}")
+        self.max_norm = max_norm
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
                                       weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_size=min_8bit_size,
@@ -215,6 +324,23 @@ class AdamW(torch.optim.Optimizer):
         """As torch's; a group's own options are checked like the defaults."""
         _check_options({**self.defaults, **param_group})
         super().add_param_group(param_group)
+
+    max_norm = None
+    grad_norm = None
+
+    def __getstate__(self) -> dict:
+        return {**super().__getstate__(), "max_norm": self.max_norm}
+
+    def _clip(self):
+        """What multiplies the gradients of a step; None: nothing does."""
+        if self.max_norm is None:
+            return None
+        grads = [p.grad for group in self.param_groups for p in group["params"]
+                 if p.grad is not None]
+        if any(g.is_sparse for g in grads):
+            raise RuntimeError("AdamW does not support sparse gradients")
+        self.grad_norm, factor = clip_factor(grads, self.max_norm)
+        return factor
 
     def _new_state(self, p, group) -> dict:
         eight = group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]
@@ -238,6 +364,7 @@ class AdamW(torch.optim.Optimizer):
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step() counts its steps on the host and cannot be captured; "
                                "use adamw_step with a step tensor")
+        factor = self._clip()
         for at, group in enumerate(self.param_groups):
             # one call per device, step count and kind of state
             calls: dict = {}
@@ -261,7 +388,7 @@ class AdamW(torch.optim.Optimizer):
                            weight_decay=group["weight_decay"],
                            scales=[s["scales"] for s in states] if eight else None,
                            masters=[s["master"] for s in states] if master else None,
-                           seed=group["seed"] + at)
+                           seed=group["seed"] + at, grad_scale=factor)
                 for s in states:
                     s["step"] = step + 1
         return loss

@@ -180,3 +180,52 @@ def decode(codes, e, signed):
     if signed:
         x = np.where(q > 127, -x, x)
     return np.where(e == 255, np.nan, x).reshape(-1)[:n]
+
+
+# ---------------------------------------------------------------------------
+# Token embeddings
+# ---------------------------------------------------------------------------
+def embed(weight, ids, lengths, scale):
+    """weight [V, D], ids [N, L] -> [N, L, D]: NaN for ids outside, 0 at and
+    past a sequence's length (lengths None: nowhere)."""
+    n, length = ids.shape
+    y = np.full((n, length, weight.shape[1]), np.nan)
+    known = (ids >= 0) & (ids < weight.shape[0])
+    y[known] = weight[ids[known]] * scale
+    if lengths is not None:
+        y[np.arange(length) >= np.asarray(lengths)[:, None]] = 0
+    return y
+
+
+def embed_rows(vocab, ids, lengths, padding):
+    """Each token's row of the table for its gradient, -1: none."""
+    rows = np.where((ids >= 0) & (ids < vocab), ids, -1)
+    if padding is not None:
+        rows[rows == padding] = -1
+    if lengths is not None:
+        rows[np.arange(ids.shape[1]) >= np.asarray(lengths)[:, None]] = -1
+    return rows.reshape(-1)
+
+
+def embed_backward(dy, rows, vocab, scale):
+    """dweight [V, D] of dy [T, D], and the bound of its error before it is
+    rounded: a sum of k fp32 numbers, in whatever order, is off by k - 1
+    roundings of partial sums at most, and the scale (its own rounding and the
+    product's) by two more."""
+    dw, size = np.zeros((vocab, dy.shape[1])), np.zeros((vocab, dy.shape[1]))
+    real = rows >= 0
+    np.add.at(dw, rows[real], dy[real])
+    np.add.at(size, rows[real], np.abs(dy[real]))
+    count = np.bincount(rows[real], minlength=vocab)[:, None]
+    return dw * scale, abs(scale) * (count + 2) * U32 * size
+
+
+# ---------------------------------------------------------------------------
+# The norm of all gradients
+# ---------------------------------------------------------------------------
+def grad_norm(grads):
+    return np.sqrt(sum(np.square(g).sum() for g in grads))
+
+
+def clip_factor(norm, max_norm, eps):
+    return min(1.0, max_norm / (norm + eps))
