@@ -48,10 +48,21 @@ def _check(weight, ids, lengths=None, scale=1.0, padding=None, dtype=None, dy=No
     (dw,) = torch.autograd.grad(y, leaf, dy)
     assert dw.dtype == weight.dtype and dw.shape == weight.shape
     rows = oracle.embed_rows(vocab, flat, lens, padding)
-    exact, bound = oracle.embed_backward(f64(dy).reshape(-1, dim), rows, vocab,
-                                         float(np.float32(scale)))
+    exact, bound = _gradient(dy.reshape(-1, dim), rows, vocab, float(np.float32(scale)))
     assert_within(dw, exact, bound, "dweight")
     return y.detach(), dw
+
+
+def _gradient(dy, rows, vocab, scale):
+    """oracle.embed_backward; large ones with its sums on the device, in 64 bits."""
+    if dy.numel() < 1 << 20:
+        return oracle.embed_backward(f64(dy), rows, vocab, scale)
+    real = torch.from_numpy(rows >= 0).cuda()
+    at, d = torch.from_numpy(rows).cuda()[real], dy[real].double()
+    sums = [torch.zeros(vocab, dy.shape[1], dtype=torch.float64, device="cuda").index_add_(0, at, x)
+            for x in (d, d.abs())]
+    count = np.bincount(rows[rows >= 0], minlength=vocab)[:, None]
+    return f64(sums[0]) * scale, abs(scale) * (count + 2) * 2.0 ** -24 * f64(sums[1])
 
 
 WIDTHS = [1, 2, 3, 7, 8, 60, 64, 77, 128, 129, 250, 256, 300, 301, 384, 389, 500, 512, 768, 770, 1024,
@@ -61,10 +72,11 @@ WIDTHS = [1, 2, 3, 7, 8, 60, 64, 77, 128, 129, 250, 256, 300, 301, 384, 389, 500
 @pytest.mark.parametrize("kind", KINDS, ids=str)
 @pytest.mark.parametrize("dim", WIDTHS)
 def test_widths(dim, kind):
+    # one launch in LDS, and the sort of many
     gen = torch.Generator().manual_seed(dim)
-    tokens = 700 if dim <= 1024 else 90
     weight = rand(gen, 37, dim, dtype=kind[0])
-    _check(weight, _ids(gen, 37, tokens), dtype=kind[1], gen=gen)
+    _check(weight, _ids(gen, 37, 700 if dim <= 1024 else 90), dtype=kind[1], gen=gen)
+    _check(weight, _ids(gen, 37, 4097), dtype=kind[1], gen=gen)
 
 
 @pytest.mark.parametrize("vocab", [1, 2, 3, 127, 128, 255, 256, 257, 512, 513, 1000, 32000, 131072,
@@ -72,17 +84,20 @@ def test_widths(dim, kind):
 def test_tables(vocab):
     gen = torch.Generator().manual_seed(vocab)
     weight = rand(gen, vocab, 24, dtype=torch.bfloat16)
-    _check(weight, _ids(gen, vocab, 3001), gen=gen)
+    for tokens in (100, 3001, 4097, 20000):
+        _check(weight, _ids(gen, vocab, tokens), gen=gen)
 
 
-def test_a_table_of_more_rows_than_a_pass_marks():
-    # more than 2^26 rows: 19 high bits, three passes and two rounds of marks
-    gen = torch.Generator().manual_seed(0)
-    vocab = 2 ** 26 + 5
+@pytest.mark.parametrize("tokens", [300, 4096, 5000])
+@pytest.mark.parametrize("bits", [16, 17, 24, 25, 26, 28, 29])
+def test_tables_of_many_rows(bits, tokens):
+    # one to four passes of the sorts, and what the one in LDS has no bits for
+    gen = torch.Generator().manual_seed(bits)
+    vocab = 2 ** bits - (bits % 2) * 77
     weight = torch.zeros(vocab, 1, dtype=torch.bfloat16, device="cuda", requires_grad=True)
-    ids = torch.randint(0, vocab, (5000,), generator=gen).cuda()
-    ids[:100], ids[100:200], ids[200] = ids[300], vocab - 1, 0
-    dy = rand(gen, 5000, 1, dtype=torch.bfloat16)
+    ids = torch.randint(0, vocab, (tokens,), generator=gen).cuda()
+    ids[:100], ids[100:200], ids[200] = ids[250], vocab - 1, 0
+    dy = rand(gen, tokens, 1, dtype=torch.bfloat16)
     (dw,) = torch.autograd.grad(maxsim_amd.embed_tokens(weight, ids), weight, dy)
     unique, inverse = torch.unique(ids, return_inverse=True)
     want, bound = oracle.embed_backward(f64(dy), inverse.cpu().numpy(), len(unique), 1.0)
@@ -91,45 +106,52 @@ def test_a_table_of_more_rows_than_a_pass_marks():
     assert int(torch.count_nonzero(dw)) == 0
 
 
-@pytest.mark.parametrize("tokens", [1, 2, 7, 8, 9, 63, 64, 65, 255, 1023, 1024, 1025, 16383, 16384,
-                                    16385, 40000, 262144, 262145])
+@pytest.mark.parametrize("tokens", [1, 2, 7, 8, 9, 63, 64, 65, 255, 256, 257, 1023, 1024, 1025, 4093,
+                                    4095, 4096, 4097, 16384, 16385, 131072, 131073, 262144, 262145,
+                                    600001])
 def test_numbers_of_tokens(tokens):
     gen = torch.Generator().manual_seed(tokens)
     weight = rand(gen, 501, 16)
     _check(weight, _ids(gen, 501, tokens), scale=0.5, gen=gen)
 
 
-@pytest.mark.parametrize("tokens", [8 * 2048, 40 * 2048 + 11, 128 * 2048, 300000])
-def test_runs_around_the_boundaries(tokens):
-    # runs of one row of 63 to 66 and of 127 to 130 tokens, longer and shorter
-    # ones, each in the windows' every position
+@pytest.mark.parametrize("dim", [8, 100, 300, 600, 2100])
+@pytest.mark.parametrize("tokens", [2000, 4096, 8 * 2048, 40 * 2048 + 11, 128 * 2048, 300000])
+def test_runs_around_the_boundaries(tokens, dim):
+    # runs of one row around the windows' 8 to 128 tokens and around the 64 that
+    # are finished by one group, longer and shorter ones, in every position
+    if tokens * dim > 1 << 26:
+        dim = 8
     rng = np.random.default_rng(tokens)
     runs, left = [], tokens
     while left > 0:
-        runs.append(min(left, int(rng.choice([1, 2, 5, 7, 8, 9, 16, 62, 63, 64, 65, 66, 67, 127, 128,
-                                              129, 130, 200, 1000]))))
+        runs.append(min(left, int(rng.choice([1, 2, 5, 7, 8, 9, 15, 16, 17, 31, 32, 33, 40, 41, 62, 63, 64,
+                                              65, 66, 67, 127, 128, 129, 130, 200, 1000]))))
         left -= runs[-1]
     rows = rng.permutation(len(runs))
     ids = torch.from_numpy(rng.permutation(np.repeat(rows, runs))).cuda()
     gen = torch.Generator().manual_seed(1)
-    _check(rand(gen, len(runs), 8, dtype=torch.float16), ids, dtype=None, gen=gen)
+    _check(rand(gen, len(runs), dim, dtype=torch.float16), ids, gen=gen)
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)
 @pytest.mark.parametrize("dim", [5, 77, 768, 2560])
 def test_one_row_for_all(kind, dim):
     gen = torch.Generator().manual_seed(dim)
-    tokens = 70001 if dim < 100 else 9001
-    ids = torch.full((tokens,), 300, device="cuda")
-    _check(rand(gen, 700, dim, dtype=kind[0]), ids, dtype=kind[1], gen=gen)
+    weight = rand(gen, 700, dim, dtype=kind[0])
+    for tokens in (3, 1000, 4096, 70001 if dim < 100 else 9001):
+        ids = torch.full((tokens,), 300, device="cuda")
+        _check(weight, ids, dtype=kind[1], gen=gen)
 
 
 def test_rows_of_one_bucket():
-    # all rows alike in their low bits: one workgroup sorts them all, from memory
+    # all rows alike in their low bits: one workgroup has them all where the
+    # tokens are few, and one digit where they are many
     gen = torch.Generator().manual_seed(3)
     vocab = 200000
-    ids = torch.randint(0, vocab // 256, (20011,), generator=gen) * 256 + 17
-    _check(rand(gen, vocab, 8), ids.cuda(), gen=gen)
+    for tokens in (4096, 20011):
+        ids = torch.randint(0, vocab // 512, (tokens,), generator=gen) * 512 + 17
+        _check(rand(gen, vocab, 8), ids.cuda(), gen=gen)
 
 
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64], ids=str)
@@ -247,21 +269,27 @@ def test_layouts_of_the_gradient():
 
 def test_the_same_bits_every_time():
     gen = torch.Generator().manual_seed(12)
-    weight, ids = rand(gen, 5000, 130, dtype=torch.bfloat16), _ids(gen, 5000, 50000)
-    dy = rand(gen, 50000, 130, dtype=torch.bfloat16)
-    first = _grad(weight, ids, dy=dy)
-    for _ in range(4):
-        assert torch.equal(_grad(weight, ids, dy=dy), first)
-    assert torch.equal(_grad(weight, ids.int(), dy=dy), first)
+    for tokens in (4000, 50000):
+        weight, ids = rand(gen, 5000, 130, dtype=torch.bfloat16), _ids(gen, 5000, tokens)
+        dy = rand(gen, tokens, 130, dtype=torch.bfloat16)
+        first = _grad(weight, ids, dy=dy)
+        for _ in range(4):
+            assert torch.equal(_grad(weight, ids, dy=dy), first)
+        assert torch.equal(_grad(weight, ids.int(), dy=dy), first)
 
 
-def test_order_of_a_sum_is_the_tokens():
-    # 1, 2^24 and -2^24 in the ids' order: (1 + 2^24) - 2^24 is 0 in fp32,
-    # 2^24 - 2^24 + 1 is 1
-    for order, want in (((1.0, 2.0 ** 24, -2.0 ** 24), 0.0), ((2.0 ** 24, -2.0 ** 24, 1.0), 1.0)):
-        dy = torch.tensor(order, device="cuda")[:, None].expand(3, 8).contiguous()
-        dw = _grad(torch.zeros(9, 8, device="cuda"), torch.tensor([4, 4, 4], device="cuda"), dy=dy)
-        assert dw[4].tolist() == [want] * 8
+@pytest.mark.parametrize("others", [0, 3000, 6000])
+def test_order_of_a_sum_is_the_tokens(others):
+    # 1, 2^25 and -2^25 in the ids' order: (1 + 2^25) - 2^25 is 0 in fp32,
+    # 2^25 - 2^25 + 1 is 1
+    places = [0, 1 + others // 2, 2 + others]
+    ids = torch.arange(others + 3, device="cuda") + 20
+    ids[places] = 0
+    for order, want in (((1.0, 2.0 ** 25, -2.0 ** 25), 0.0), ((2.0 ** 25, -2.0 ** 25, 1.0), 1.0)):
+        dy = torch.zeros(others + 3, 8, device="cuda")
+        dy[places] = torch.tensor(order, device="cuda")[:, None]
+        dw = _grad(torch.zeros(others + 23, 8, device="cuda"), ids, dy=dy)
+        assert dw[0].tolist() == [want] * 8
 
 
 def test_the_comparison_sees_one_wrong_element():
