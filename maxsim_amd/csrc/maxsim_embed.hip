@@ -11,12 +11,8 @@
 // that the ids alone decide every order:
 //   embed_few_kernel   few tokens: one launch does all of it in LDS;
 //   embed_count_kernel, embed_place_kernel   a pass of the sort of many;
-//   embed_sum_kernel   groups of lanes add up `window` sorted tokens each, a
-//                      run of one row in registers, and write the finished rows;
-//                      a run of up to short_run tokens that crosses into the
-//                      next window is finished by the group it began with, of
-//                      a longer one each group leaves its part in the workspace;
-//                      more workgroups write the rows without a token;
+//   embed_sum_kernel   groups of lanes add up the tokens of one row each, of
+//                      rows with many a part; more write zeros for rows without;
 //   embed_join_kernel  adds those parts.
 #include <algorithm>
 
@@ -27,6 +23,13 @@
 namespace maxsim {
 
 // ---- forward -----------------------------------------------------------------
+
+// A result of more bytes than this goes past the caches, which then keep the
+// table (524288 tokens x 768, fp32 table, bf16 result: 217 us against 305, and
+// 579 against 617 with the layer norm that reads the result).  A smaller one is
+// mostly still there for its reader (40000 tokens: 18.7 against 20.1 us, but
+// 42.4 against 41.5 with the layer norm; 80000, 123 MB: 79 against 90).
+constexpr int64_t kCacheBytes = (int64_t)96 << 20;
 
 struct EmbedArgs {
   const void* weight;
@@ -87,9 +90,16 @@ __device__ __forceinline__ void store_piece(typename W::storage* row, int e0, in
   }
 }
 
+// 16 bytes that the caches need not keep.
+template <typename T>
+__device__ __forceinline__ void store_past_cache(typename T::storage* p, const Chunk<T>& c) {
+  typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+  __builtin_nontemporal_store(Words{c.w[0], c.w[1], c.w[2], c.w[3]}, reinterpret_cast<Words*>(p));
+}
+
 // A group of G lanes looks up U tokens, GROUPS apart: their ids (and lengths)
 // are asked for together, then their rows.
-template <typename W, typename T, int G, int K, int U>
+template <typename W, typename T, int G, int K, int U, bool PAST_CACHE>
 __global__ __launch_bounds__(row_threads(G)) void embed_kernel(EmbedArgs a) {
   constexpr int V = kVec<T>, GROUPS = row_threads(G) / G;
   const int j = threadIdx.x % G, group = threadIdx.x / G;
@@ -139,7 +149,9 @@ __global__ __launch_bounds__(row_threads(G)) void embed_kernel(EmbedArgs a) {
 #pragma unroll
       for (int e = 0; e < V; ++e)
         f[e] = known[u] ? f[e] * a.scale : real[u] ? __builtin_nanf("") : 0.0f;
-      store_chunk<T>(to, (j + k * G) * V, dim, f);
+      const int e0 = (j + k * G) * V;
+      if (PAST_CACHE && e0 + V <= dim) store_past_cache(to + e0, pack<T>(f));
+      else store_chunk<T>(to, e0, dim, f);
     }
   }
 }
@@ -189,7 +201,7 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t (&waves)[kSo
   return s;
 }
 
-// The rows of the table that some workgroups look after: those without a token
+// A stretch of the table that a workgroup looks after: rows without a token
 // become 0.
 struct ZeroArgs {
   void* dweight;
@@ -454,6 +466,7 @@ struct SortArgs {
   int shift, bits;
   uint32_t* counts;  // [workgroups][kDigits]
   uint32_t* total;   // entries in all, which the first pass writes
+  uint32_t* begun;   // which it clears, for the sums
 };
 
 // Calls f(entry, whether there is one) for the entries of a wave's share of the
@@ -534,7 +547,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(SortArgs a) {
       for (uint32_t i = threadIdx.x; i < kSortThreads; i += digits)
         all += sums[0][i], before += sums[1][i];
     uint32_t start = sum_before(all, waves);
-    if (FIRST && blockIdx.x == 0 && threadIdx.x == kSortThreads - 1) *a.total = start + all;
+    if (FIRST && blockIdx.x == 0 && threadIdx.x == kSortThreads - 1) *a.total = start + all, *a.begun = 0;
     start += before;
     if (threadIdx.x < digits)
       for (int w = 0; w < kSortWaves; ++w) {
@@ -558,21 +571,27 @@ __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(SortArgs a) {
 
 // ---- backward: the sums of many ------------------------------------------------
 
-constexpr int kHalo = 64;           // entries on either side of a workgroup's that it looks at
-constexpr int kWindowEntries = 1024;  // most entries of a workgroup's windows
+// A run is a row's sorted tokens.  A workgroup has `span` sorted tokens, whose
+// runs its groups of lanes add up one by one, whichever is free the next: a run
+// of up to `short_run` tokens where it begins, of a longer one the part in each
+// window (spans are whole windows).  Parts of a run that reaches into other
+// windows are left in the workspace.  More workgroups write zeros.
+constexpr int kMaxShortRun = 64, kMaxWindow = 64, kMaxSpan = 512;
 
 struct SumArgs {
   const void* dy;
   int64_t dy_row;  // stride in elements
   int dim;
   const Entry* sorted;
-  uint32_t tokens;
   const uint32_t* total;
-  uint32_t window, short_run, groups;  // groups: workgroups that add up
+  uint32_t span, window;  // powers of two
+  uint32_t short_run;
+  uint32_t spans;         // workgroups that add up
   float scale;
-  float* parts;      // [windows][2][part_dim]: of a run from before, of one that goes on
+  float* parts;     // [windows][2][part_dim]: of a run from before, of one that begins here
   int part_dim;
-  uint32_t* begins;  // [windows] whether a long run begins here and goes on
+  uint2* begins;    // windows where a run begins that goes on, and its row, in any order
+  uint32_t* begun;  // their number
   ZeroArgs zero;
 };
 
@@ -592,98 +611,163 @@ __device__ __forceinline__ uint32_t first_of(const Entry* sorted, uint32_t total
   return lo;
 }
 
+// The same by one lane, among entries [lo, hi).
+__device__ __forceinline__ uint32_t first_among(const Entry* sorted, uint32_t lo, uint32_t hi,
+                                                uint64_t row) {
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (sorted[mid].row < row) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// acc = the sum of the rows of dy that token_of(first) to token_of(last - 1)
+// name, in that order, U rows in flight.
+template <typename T, int G, int K, int U, typename F>
+__device__ __forceinline__ void sum_rows(const SumArgs& a, uint32_t first, uint32_t last,
+                                         F&& token_of, float (&acc)[K][kVec<T>]) {
+  constexpr int V = kVec<T>;
+  constexpr bool SHORT = takes_short(G);
+  const int j = threadIdx.x % G;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[k][e] = 0.0f;
+  for (uint32_t i = first; i < last; i += U) {
+    Chunk<T> raw[U][K];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      // past the last, the last again: its lines are on their way
+      const auto* row = static_cast<const typename T::storage*>(a.dy) +
+                        (int64_t)token_of(min(i + u, last - 1)) * a.dy_row;
+#pragma unroll
+      for (int k = 0; k < K; ++k) raw[u][k] = load_chunk<T, SHORT>(row, (j + k * G) * V, a.dim);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool has = i + u < last;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float f[V];
+        place_chunk<T, SHORT>(raw[u][k], (j + k * G) * V, a.dim);
+        unpack<T>(raw[u][k], f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[k][e] += has ? f[e] : 0.0f;
+      }
+    }
+  }
+}
+
 template <typename T, typename W, int G, int K, int U>
 __global__ __launch_bounds__(row_threads(G)) void embed_sum_kernel(SumArgs a) {
-  using S = typename T::storage;
-  constexpr int V = kVec<T>, THREADS = row_threads(G), GROUPS = THREADS / G;
-  constexpr bool SHORT = takes_short(G);
-  constexpr int L = G < 64 ? G : 64;  // lanes that look at entries together
+  constexpr int V = kVec<T>, THREADS = row_threads(G);
   __shared__ union {
-    Entry entries[kWindowEntries + 2 * (kHalo + 1)];
+    struct {
+      Entry entries[kMaxSpan + 2 * kMaxShortRun];
+      uint32_t list[kMaxSpan], used, next;
+    } span;
     struct { uint32_t bounds[2], has[kZeroRows / 32]; } zero;
   } lds;
   const uint32_t total = *a.total;
-  if (blockIdx.x >= a.groups) {
-    const uint32_t first = (blockIdx.x - a.groups) * a.zero.rows;
-    if (threadIdx.x < kZeroRows / 32) lds.zero.has[threadIdx.x] = 0;
+
+  if (blockIdx.x >= a.spans) {
+    const uint32_t first = (blockIdx.x - a.spans) * a.zero.rows;
+    for (int i = threadIdx.x; i < kZeroRows / 32; i += THREADS) lds.zero.has[i] = 0;
     if (threadIdx.x < 128) {
       const int which = threadIdx.x >> 6;
       const uint32_t i = first_of(a.sorted, total, (uint64_t)first + which * a.zero.rows);
       if ((threadIdx.x & 63) == 0) lds.zero.bounds[which] = i;
     }
     __syncthreads();
-    const uint32_t end = lds.zero.bounds[1];
-    for (uint32_t i = lds.zero.bounds[0] + threadIdx.x; i < end; i += THREADS) {
-      const uint32_t r = a.sorted[i].row - first;
-      atomicOr(&lds.zero.has[r / 32], 1u << (r & 31));
+    // from entries that are few, or by a search for each row: a frequent one's
+    // are as many as they like (524288 tokens: the launch 200 us without it)
+    const uint32_t lo = lds.zero.bounds[0], hi = lds.zero.bounds[1];
+    const uint32_t rows = min(a.zero.rows, a.zero.vocab - first);
+    const bool search = hi - lo > 4 * THREADS;
+    for (uint32_t t = threadIdx.x; t < (search ? rows : hi - lo); t += THREADS) {
+      const uint32_t i = search ? first_among(a.sorted, lo, hi, (uint64_t)first + t) : lo + t;
+      const uint32_t r = i < hi ? a.sorted[i].row - first : rows;
+      if (r < rows) atomicOr(&lds.zero.has[r / 32], 1u << (r & 31));
     }
     __syncthreads();
     zero_rows(a.zero, first, lds.zero.has);
     return;
   }
 
-  const int j = threadIdx.x % G, group = threadIdx.x / G;
-  const int dim = a.dim;
-  // the windows' entries and those around them; kNoRow where there are none
-  const int64_t base = (int64_t)blockIdx.x * GROUPS * a.window - (kHalo + 1);
-  if (base + kHalo + 1 >= total) return;
-  const int count_all = GROUPS * (int)a.window + 2 * (kHalo + 1);
-  for (int t = threadIdx.x; t < count_all; t += THREADS) {
-    const int64_t i = base + t;
-    lds.entries[t] = i >= 0 && i < total ? a.sorted[i] : Entry{kNoRow, 0};
+  // the span's entries and those around them; kNoRow where there are none
+  const int64_t base = (int64_t)blockIdx.x * a.span;
+  if (base >= total) return;
+  const int span = (int)a.span, short_run = (int)a.short_run;
+  for (int t = threadIdx.x; t < span + 2 * short_run; t += THREADS) {
+    const int64_t i = base - short_run + t;
+    lds.span.entries[t] = i >= 0 && i < total ? a.sorted[i] : Entry{kNoRow, 0};
+  }
+  if (threadIdx.x == 0) lds.span.used = lds.span.next = 0;
+  __syncthreads();
+  const Entry* entries = lds.span.entries + short_run;
+  // What is to be added up: from entry t on where a run begins with it, or
+  // where a window does inside of a long run.  In any order: none has to do
+  // with another.
+  const int n = (int)min((int64_t)span, (int64_t)total - base), window = (int)a.window;
+  for (int t = threadIdx.x; t < n; t += THREADS) {
+    const uint32_t row = entries[t].row;
+    const bool starts = entries[t - 1].row != row, edge = (t & (window - 1)) == 0;
+    if (!starts && !edge) continue;
+    int start = t;  // of the run, or short_run before t where it is further
+    if (!starts) {
+      int lo = t - short_run;
+      while (lo < start) {
+        const int mid = (lo + start) >> 1;
+        if (entries[mid].row == row) start = mid;
+        else lo = mid + 1;
+      }
+    }
+    const bool is_long = start == t - short_run || entries[start + short_run].row == row;
+    if (!is_long && !starts) continue;
+    // its end, or the window's that a long run reaches past
+    int lo = t + 1, hi = is_long ? min((t | (window - 1)) + 1, n) : t + short_run;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (entries[mid].row == row) lo = mid + 1;
+      else hi = mid;
+    }
+    lds.span.list[atomicAdd(&lds.span.used, 1u)] = (uint32_t)t | (uint32_t)hi << 16;
   }
   __syncthreads();
-  // from here on entries are counted from the workgroup's first, minus the halo
-  const Entry* entries = lds.entries;
-  const uint32_t window = blockIdx.x * GROUPS + group;
-  const int first = kHalo + 1 + group * (int)a.window, last_of_all = (int)min((int64_t)total - base, (int64_t)count_all);
-  if (first >= last_of_all) return;
-  const int i0 = first, i1 = min(first + (int)a.window, last_of_all);
-  const int short_run = (int)a.short_run;
-
-  // Entries of `row` among the short_run from `at` on, or before it.
-  auto count = [&](uint32_t row, int at, int step) {
-    int n = 0;
-    const int shift = (threadIdx.x & 63) / L * L;
-    for (int t = 0; t < short_run; t += L) {
-      const int k = t + (int)(threadIdx.x % L);
-      const bool same = k < short_run && entries[at + step * k].row == row;
-      const uint64_t all = __ballot(same) >> shift;
-      n += (int)__popcll(L == 64 ? all : all & (((uint64_t)1 << L) - 1));
+  const uint32_t used = lds.span.used;
+  const int j = threadIdx.x % G;
+  for (;;) {
+    uint32_t i = 0;
+    if constexpr (G <= 64) {
+      if (j == 0) i = atomicAdd(&lds.span.next, 1u);
+      i = (uint32_t)__shfl((int)i, (int)(threadIdx.x & 63) / G * G, 64);
+    } else {
+      i = lds.span.next;
+      __syncthreads();
+      if (threadIdx.x == 0) lds.span.next = i + 1;
+      __syncthreads();
     }
-    return n;
-  };
-  int at = i0, stop = i1;
-  bool joins = false, goes_on = false;  // the first run is a long one's next part; so is the last's
-  if (const uint32_t row = entries[i0].row; entries[i0 - 1].row == row) {
-    const int back = count(row, i0 - 1, -1);
-    if (back == short_run || entries[i0 - back + short_run].row == row) joins = true;
-    else at = i0 + count(row, i0, 1);  // whose group has it
-  }
-  if (const uint32_t row = entries[i1 - 1].row; at < i1 && i1 < last_of_all && entries[i1].row == row) {
-    const int back = count(row, i1 - 1, -1);
-    if (back == short_run || entries[i1 - back + short_run].row == row) goes_on = true;
-    else stop = i1 + count(row, i1, 1);
-  }
-
-  float acc[K][V];
-  auto clear = [&] {
+    if (i >= used) break;
+    const int lo = lds.span.list[i] & 0xffff, hi = lds.span.list[i] >> 16;
+    float acc[K][V];
+    sum_rows<T, G, K, U>(a, (uint32_t)lo, (uint32_t)hi,
+                         [&](uint32_t i) { return entries[i].token; }, acc);
+    const uint32_t row = entries[lo].row;
+    const bool from_before = entries[lo - 1].row == row;
+    const bool goes_on = entries[hi].row == row;  // only a long one's part ends inside of it
+    if (!from_before && !goes_on) {
+      auto* to = static_cast<typename W::storage*>(a.zero.dweight) + (int64_t)row * a.dim;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+      for (int k = 0; k < K; ++k) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[k][e] = 0.0f;
-  };
-  auto write_row = [&](uint32_t row) {
-    auto* to = static_cast<typename W::storage*>(a.zero.dweight) + (int64_t)row * dim;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) acc[k][e] *= a.scale;
-      store_piece<W, V>(to, (j + k * G) * V, dim, acc[k]);
+        for (int e = 0; e < V; ++e) acc[k][e] *= a.scale;
+        store_piece<W, V>(to, (j + k * G) * V, a.dim, acc[k]);
+      }
+      continue;
     }
-  };
-  auto write_part = [&](int which) {
-    float* to = a.parts + ((int64_t)window * 2 + which) * a.part_dim;
+    const uint32_t number = (uint32_t)((base + lo) / window);
+    float* to = a.parts + ((int64_t)number * 2 + (from_before ? 0 : 1)) * a.part_dim;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int e0 = (j + k * G) * V;
@@ -692,116 +776,62 @@ __global__ __launch_bounds__(row_threads(G)) void embed_sum_kernel(SumArgs a) {
         if (e0 + e < a.part_dim)
           store_any(to + e0 + e, make_float4(acc[k][e], acc[k][e + 1], acc[k][e + 2], acc[k][e + 3]));
     }
-  };
-  clear();
-  uint32_t row = at < stop ? entries[at].row : 0;
-  bool part = joins;
-  for (int i = at; i < stop; i += U) {
-    Chunk<T> raw[U][K];
-    uint32_t rows[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const Entry e = entries[min(i + u, stop - 1)];
-      rows[u] = e.row;
-      const S* from = static_cast<const S*>(a.dy) + (int64_t)e.token * a.dy_row;
-#pragma unroll
-      for (int k = 0; k < K; ++k) raw[u][k] = load_chunk<T, SHORT>(from, (j + k * G) * V, dim);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u >= stop) break;
-      if (rows[u] != row) {
-        if (part) write_part(0);
-        else write_row(row);
-        part = false;
-        row = rows[u];
-        clear();
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float f[V];
-        place_chunk<T, SHORT>(raw[u][k], (j + k * G) * V, dim);
-        unpack<T>(raw[u][k], f);
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[k][e] += f[e];
-      }
-    }
+    if (!from_before && j == 0) a.begins[atomicAdd(a.begun, 1u)] = make_uint2(number, row);
   }
-  if (at < stop) {
-    if (part) write_part(0);
-    else if (goes_on) write_part(1);
-    else write_row(row);
-  }
-  if (j == 0) a.begins[window] = goes_on && !part;
 }
 
-// Adds up the parts of the long runs that begin in a workgroup's share of the
-// windows and go on.  Threads share a row's columns, four each, and where
-// there are more threads than that, the parts.
-constexpr int kJoinThreads = 512, kJoinUnroll = 8, kJoinWindows = 512;
+// Adds up the parts of the runs that go on from the window that they begin in,
+// a workgroup a run and kJoinColumns of its columns; a thread has four of them,
+// and of the parts a share.
+constexpr int kJoinThreads = 512, kJoinUnroll = 8, kJoinColumns = 256;
 template <typename W>
-__global__ __launch_bounds__(kJoinThreads) void embed_join_kernel(SumArgs a, uint32_t share) {
-  __shared__ uint32_t list[kJoinWindows], found;
+__global__ __launch_bounds__(kJoinThreads) void embed_join_kernel(SumArgs a) {
   __shared__ float4 sums[kJoinThreads];
-  const uint32_t total = *a.total;
-  const uint32_t windows = (uint32_t)(((uint64_t)total + a.window - 1) / a.window);
-  const uint64_t first = (uint64_t)blockIdx.x * share;
-  if (first >= windows) return;
-  // the runs' windows, in whatever order: none has to do with another
-  if (threadIdx.x == 0) found = 0;
-  __syncthreads();
-  const uint64_t w = first + threadIdx.x;
-  if (threadIdx.x < share && w < windows && a.begins[w]) list[atomicAdd(&found, 1u)] = (uint32_t)w;
-  __syncthreads();
-  const int columns = (a.dim + 3) / 4;
-  const int across = min(columns, kJoinThreads), shares = kJoinThreads / across;
-  const int column = threadIdx.x % across, mine = threadIdx.x / across;
-  for (uint32_t r = 0; r < found; ++r) {
-    const uint32_t window = list[r];
-    const uint64_t begin = (uint64_t)window * a.window;
-    const uint32_t row = a.sorted[begin + a.window - 1].row;
+  const uint32_t runs = *a.begun, total = *a.total;
+  constexpr int across = kJoinColumns / 4, shares = kJoinThreads / across;
+  const int mine = threadIdx.x / across;
+  const int e0 = blockIdx.y * kJoinColumns + threadIdx.x % across * 4;
+  const bool has = e0 < a.dim;
+  for (uint32_t r = blockIdx.x; r < runs; r += gridDim.x) {
+    const uint2 run = a.begins[r];
+    const uint64_t begin = (uint64_t)run.x * a.window;
     // the windows after it that the run reaches into
     uint32_t more = 0;
     for (;;) {
       const uint64_t i = begin + (uint64_t)(more + 1 + (threadIdx.x & 63)) * a.window;
-      const uint64_t same = __ballot(i < total && a.sorted[min(i, (uint64_t)total - 1)].row == row);
+      const uint64_t same = __ballot(i < total && a.sorted[min(i, (uint64_t)total - 1)].row == run.y);
       more += (uint32_t)__popcll(same);
       if (~same) break;
     }
     const uint32_t take = (more + shares - 1) / shares;
-    const uint32_t lo = min(mine * take, more), hi = mine < shares ? min(lo + take, more) : lo;
-    auto* out = static_cast<typename W::storage*>(a.zero.dweight) + (int64_t)row * a.dim;
-    for (int c0 = 0; c0 < columns; c0 += across) {
-      const int e0 = (c0 + column) * 4;
-      const bool has = e0 < a.dim;
-      const float* p = a.parts + (int64_t)window * 2 * a.part_dim + e0;
-      float4 s = make_float4(0, 0, 0, 0);
-      if (has && mine == 0) s = load_any<float4>(p + a.part_dim);
-      for (uint32_t k = lo; has && k < hi; k += kJoinUnroll) {
-        float4 v[kJoinUnroll];
+    const uint32_t lo = min(mine * take, more), hi = min(lo + take, more);
+    const float* p = a.parts + (int64_t)run.x * 2 * a.part_dim + e0;
+    float4 s = make_float4(0, 0, 0, 0);
+    if (has && mine == 0) s = load_any<float4>(p + a.part_dim);
+    for (uint32_t k = lo; has && k < hi; k += kJoinUnroll) {
+      float4 v[kJoinUnroll];
 #pragma unroll
-        for (int u = 0; u < kJoinUnroll; ++u)
-          v[u] = load_any<float4>(p + (int64_t)min(k + u + 1, hi) * 2 * a.part_dim);
+      for (int u = 0; u < kJoinUnroll; ++u)
+        v[u] = load_any<float4>(p + (int64_t)min(k + u + 1, hi) * 2 * a.part_dim);
 #pragma unroll
-        for (int u = 0; u < kJoinUnroll; ++u)
-          if (k + u < hi) s.x += v[u].x, s.y += v[u].y, s.z += v[u].z, s.w += v[u].w;
+      for (int u = 0; u < kJoinUnroll; ++u)
+        if (k + u < hi) s.x += v[u].x, s.y += v[u].y, s.z += v[u].z, s.w += v[u].w;
+    }
+    sums[threadIdx.x] = s;
+    __syncthreads();
+    if (mine == 0 && has) {
+#pragma unroll
+      for (int i = 1; i < shares; ++i) {
+        const float4 v = sums[i * across + threadIdx.x];
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
       }
-      if (shares > 1) {
-        sums[threadIdx.x] = s;
-        __syncthreads();
-        if (mine == 0)
-          for (int i = 1; i < shares; ++i) {
-            const float4 v = sums[i * across + column];
-            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-          }
-        __syncthreads();
-      }
-      if (!has || mine != 0) continue;
+      auto* out = static_cast<typename W::storage*>(a.zero.dweight) + (int64_t)run.y * a.dim;
       const float f[4] = {s.x * a.scale, s.y * a.scale, s.z * a.scale, s.w * a.scale};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (e0 + e < a.dim) out[e0 + e] = from_float<W>(f[e]);
     }
+    __syncthreads();
   }
 }
 
@@ -828,31 +858,39 @@ static int row_groups(maxsim_dtype dtype, int64_t dim) {
 
 struct EmbedLayout {
   int64_t windows;
-  uint32_t window;  // tokens of one
-  int groups;       // windows of a workgroup
-  uint32_t run;     // tokens of a workgroup of the sort
+  uint32_t window, span, short_run;  // tokens
+  uint32_t run;           // tokens of a workgroup of the sort
   int part_dim;
   size_t sorted, other, counts, begins, parts, bytes;  // offsets, and all
 };
 static EmbedLayout embed_layout(maxsim_dtype dtype, int64_t tokens, int64_t vocab, int64_t dim) {
   EmbedLayout l{};
   if (few_tokens(tokens, vocab)) return l;
-  l.groups = row_groups(dtype, dim);
-  // enough windows to fill the chip, long enough that few runs cross into the next
-  const int64_t most = std::min(kWindowEntries / l.groups, 128);
-  l.window = (uint32_t)std::min<int64_t>(std::max<int64_t>(tokens / 2048, 8), most);
+  // a group of lanes has up to 32 tokens, fewer where that leaves CUs idle
+  const uint32_t groups = (uint32_t)row_groups(dtype, dim);
+  uint32_t share = 32;
+  while (share > 2 && tokens / share < 8192) share /= 2;
+  l.span = std::min<uint32_t>(std::max<uint32_t>(groups * share, 8), kMaxSpan);
+  l.window = std::min<uint32_t>(l.span, kMaxWindow);
+  // what the others have long done when a group ends with it
+  l.short_run = std::min<uint32_t>(std::max<uint32_t>(2 * share, 16), kMaxShortRun);
   l.windows = (tokens + l.window - 1) / l.window;
   l.part_dim = (int)((dim + 7) / 8 * 8);
   const int64_t each = (tokens + kSortGroups - 1) / kSortGroups;
   l.run = (uint32_t)((each + kSortThreads - 1) / kSortThreads * kSortThreads);
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  l.sorted = 256;  // the total first
+  l.sorted = 256;  // two numbers first
   l.other = l.sorted + up((size_t)tokens * sizeof(Entry));
   l.counts = l.other + up((size_t)tokens * sizeof(Entry));
   l.begins = l.counts + (size_t)kSortGroups * kDigits * sizeof(uint32_t);
-  l.parts = l.begins + up((size_t)l.windows * sizeof(uint32_t));
+  l.parts = l.begins + up((size_t)l.windows * sizeof(uint2));
   l.bytes = l.parts + (size_t)l.windows * 2 * l.part_dim * sizeof(float);
   return l;
+}
+
+static ZeroArgs zero_args(void* dweight, int64_t vocab, int64_t row_bytes, int element) {
+  const int64_t rows = std::min<int64_t>(std::max<int64_t>(kZeroBytes / row_bytes, 1), kZeroRows);
+  return ZeroArgs{dweight, row_bytes, (uint32_t)vocab, (uint32_t)rows, element};
 }
 
 static int check_embed(maxsim_dtype weight_dtype, maxsim_dtype dtype, int64_t vocab, int64_t dim) {
@@ -899,6 +937,7 @@ int maxsim_amd_embed_forward(maxsim_dtype weight_dtype, maxsim_dtype dtype, cons
   const EmbedArgs all{weight, weight_stride, vocab, (int)dim, ids, ids64, sequences,
                       sequences * length, 0, (uint32_t)length, lengths, lengths64,
                       padding_idx < 0 ? -1 : padding_idx, scale, y, rows};
+  const bool past_cache = all.tokens * dim * (dtype == MAXSIM_FLOAT32 ? 4 : 2) > kCacheBytes;
   return with_embed_types(weight_dtype, dtype, [&](auto w, auto t) {
     using W = decltype(w);
     using T = decltype(t);
@@ -910,8 +949,12 @@ int maxsim_amd_embed_forward(maxsim_dtype weight_dtype, maxsim_dtype dtype, cons
       EmbedArgs a = all;
       for (; a.begin < a.tokens && rc == MAXSIM_OK; a.begin += most * each) {
         const int64_t blocks = std::min<int64_t>((a.tokens - a.begin + each - 1) / each, most);
-        hipLaunchKernelGGL((embed_kernel<W, T, G, K, U>), dim3((unsigned)blocks), dim3(threads), 0,
-                           static_cast<hipStream_t>(stream), a);
+        if (past_cache)
+          hipLaunchKernelGGL((embed_kernel<W, T, G, K, U, true>), dim3((unsigned)blocks),
+                             dim3(threads), 0, static_cast<hipStream_t>(stream), a);
+        else
+          hipLaunchKernelGGL((embed_kernel<W, T, G, K, U, false>), dim3((unsigned)blocks),
+                             dim3(threads), 0, static_cast<hipStream_t>(stream), a);
         rc = check_launch("embed_kernel");
       }
     });
@@ -946,12 +989,9 @@ int maxsim_amd_embed_backward(maxsim_dtype weight_dtype, maxsim_dtype dtype, con
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int element = weight_dtype == MAXSIM_FLOAT32 ? 4 : 2;
   const int bits = bits_of((uint64_t)vocab);
-  ZeroArgs zero{dweight, dim * element, (uint32_t)vocab, 0, element};
-  zero.rows = (uint32_t)std::min<int64_t>(std::max<int64_t>(kZeroBytes / zero.row_bytes, 1),
-                                          kZeroRows);
-  const int64_t zero_groups = (vocab + zero.rows - 1) / zero.rows;
-
   if (few_tokens(tokens, vocab)) {
+    const ZeroArgs zero = zero_args(dweight, vocab, dim * element, element);
+    const int64_t zero_groups = (vocab + zero.rows - 1) / zero.rows;
     FewArgs few{rows, dy, dy_stride, (uint32_t)tokens, (int)dim, std::min(bits, kBucketBits), 0, 0,
                 scale, zero};
     few.high_bits = bits - few.bucket_bits;
@@ -966,8 +1006,10 @@ int maxsim_amd_embed_backward(maxsim_dtype weight_dtype, maxsim_dtype dtype, con
     });
   }
 
-  const int64_t sum_groups = (l.windows + l.groups - 1) / l.groups;
-  if (sum_groups + zero_groups > UINT32_MAX / 1024)
+  const ZeroArgs zero = zero_args(dweight, vocab, dim * element, element);
+  const int64_t spans = (tokens + l.span - 1) / l.span;
+  const int64_t blocks = spans + (vocab + zero.rows - 1) / zero.rows;
+  if (blocks > UINT32_MAX / 1024)
     return fail(MAXSIM_ERR_UNSUPPORTED, "table or gradient too large for one launch");
   char* ws = static_cast<char*>(workspace);
   uint32_t* total = reinterpret_cast<uint32_t*>(ws);
@@ -975,7 +1017,7 @@ int maxsim_amd_embed_backward(maxsim_dtype weight_dtype, maxsim_dtype dtype, con
   Entry* other = reinterpret_cast<Entry*>(ws + l.other);
   const int passes = std::max((bits + kDigitBits - 1) / kDigitBits, 1);
   SortArgs sort{rows, nullptr, passes & 1 ? sorted : other, (uint32_t)tokens, (uint32_t)vocab, l.run,
-                0, (bits + passes - 1) / passes, reinterpret_cast<uint32_t*>(ws + l.counts), total};
+                0, (bits + passes - 1) / passes, reinterpret_cast<uint32_t*>(ws + l.counts), total, total + 1};
   const dim3 runs((unsigned)((tokens + l.run - 1) / l.run));
   for (int p = 0; p < passes; ++p) {
     if (p == 0) {
@@ -991,26 +1033,26 @@ int maxsim_amd_embed_backward(maxsim_dtype weight_dtype, maxsim_dtype dtype, con
     }
     if (int e = check_launch("embed_place_kernel")) return e;
   }
-  const SumArgs sum{dy, dy_stride, (int)dim, sorted, (uint32_t)tokens, total, l.window,
-                    std::min<uint32_t>(l.window, kHalo), (uint32_t)sum_groups, scale,
+  const SumArgs sum{dy, dy_stride, (int)dim, sorted, total, l.span, l.window, l.short_run,
+                    (uint32_t)spans, scale,
                     reinterpret_cast<float*>(ws + l.parts), l.part_dim,
-                    reinterpret_cast<uint32_t*>(ws + l.begins), zero};
+                    reinterpret_cast<uint2*>(ws + l.begins), total + 1, zero};
   return with_embed_types(weight_dtype, dtype, [&](auto w, auto t) {
     using W = decltype(w);
     using T = decltype(t);
     int rc = MAXSIM_OK;
     with_shape<kVec<T>>(dim, [&](auto s) {
       constexpr int G = decltype(s)::G, K = decltype(s)::K;
-      constexpr int U = K >= 3 ? 4 : 8;
+      constexpr int U = 2;
       hipLaunchKernelGGL((embed_sum_kernel<T, W, G, K, U>),
-                         dim3((unsigned)(sum_groups + zero_groups)), dim3(row_threads(G)), 0, st,
-                         sum);
+                         dim3((unsigned)blocks), dim3(row_threads(G)), 0, st, sum);
       rc = check_launch("embed_sum_kernel");
     });
     if (rc != MAXSIM_OK) return rc;
-    const uint32_t share = (uint32_t)std::min<int64_t>((l.windows + 511) / 512, kJoinWindows);
-    hipLaunchKernelGGL(embed_join_kernel<W>, dim3((unsigned)((l.windows + share - 1) / share)),
-                       dim3(kJoinThreads), 0, st, sum, share);
+    const unsigned blocks = (unsigned)((dim + kJoinColumns - 1) / kJoinColumns);
+    hipLaunchKernelGGL(embed_join_kernel<W>,
+                       dim3((unsigned)std::min<int64_t>(l.windows, 4096 / blocks), blocks),
+                       dim3(kJoinThreads), 0, st, sum);
     return check_launch("embed_join_kernel");
   });
 }
