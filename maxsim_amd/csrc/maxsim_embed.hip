@@ -452,9 +452,13 @@ __global__ __launch_bounds__(kSortThreads) void embed_few_kernel(FewArgs a) {
 // Stable passes by kDigitBits of the row each, from the lowest.  The workgroups
 // of a pass each have a run of the entries; embed_count_kernel counts a run's
 // digits, embed_place_kernel adds up what the others counted and moves its run.
+// Where the entries are few, each workgroup counts all of them itself, which
+// saves the launches (18283 tokens, two passes: the gradient 34.7 us against
+// 38.5; 30000: 47.4 against 41.0).
 constexpr int kDigitBits = 9;
 constexpr int kDigits = 1 << kDigitBits;
 constexpr int kSortGroups = 128;  // most workgroups of a pass
+constexpr int kCountAll = 20480;  // entries that every workgroup counts
 static_assert(kSortThreads % kDigits == 0, "threads share the digits' sums evenly");
 
 struct SortArgs {
@@ -514,7 +518,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_count_kernel(SortArgs a) {
   a.counts[(size_t)blockIdx.x * kDigits + threadIdx.x] = s;
 }
 
-template <bool FIRST>
+template <bool FIRST, bool COUNTED>
 __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(SortArgs a) {
   __shared__ uint32_t counts[kSortWaves][kDigits];
   __shared__ uint32_t sums[2][kSortThreads], waves[kSortWaves];
@@ -522,8 +526,40 @@ __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(SortArgs a) {
   const uint32_t digits = 1u << a.bits, mask = digits - 1;
   const uint32_t n = FIRST ? a.tokens : *a.total;
   count_share<FIRST>(a, n, counts[wave]);
-  // of a digit: all entries, and those of the runs before; several threads each
-  {
+  // of a digit: all entries, and those of the runs before
+  if constexpr (!COUNTED) {
+    for (uint32_t i = threadIdx.x; i < digits; i += kSortThreads) sums[0][i] = sums[1][i] = 0;
+    __syncthreads();
+    const uint32_t begin = blockIdx.x * a.run;
+    constexpr int U = 8;
+    for (uint32_t i0 = 0; i0 < n; i0 += kSortThreads * U) {
+      uint32_t row[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t i = min(i0 + u * kSortThreads + threadIdx.x, n - 1);
+        row[u] = FIRST ? (uint32_t)a.rows[i] : a.in[i].row;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t i = i0 + u * kSortThreads + threadIdx.x;
+        if (i < n && row[u] < a.vocab) atomicAdd(&sums[i < begin][row[u] >> a.shift & mask], 1u);
+      }
+    }
+    __syncthreads();
+    const uint32_t before = threadIdx.x < digits ? sums[1][threadIdx.x] : 0;
+    const uint32_t all = threadIdx.x < digits ? sums[0][threadIdx.x] + before : 0;
+    uint32_t start = sum_before(all, waves);
+    if (FIRST && blockIdx.x == 0 && threadIdx.x == kSortThreads - 1)
+      *a.total = start + all, *a.begun = 0;
+    start += before;
+    if (threadIdx.x < digits)
+      for (int w = 0; w < kSortWaves; ++w) {
+        const uint32_t c = counts[w][threadIdx.x];
+        counts[w][threadIdx.x] = start;
+        start += c;
+      }
+  } else {
+    // several threads each
     const uint32_t d = threadIdx.x & mask, part = threadIdx.x >> a.bits;
     const uint32_t parts = kSortThreads >> a.bits, groups = gridDim.x;
     uint32_t all = 0, before = 0;
@@ -990,7 +1026,9 @@ int maxsim_amd_embed_backward(maxsim_dtype weight_dtype, maxsim_dtype dtype, con
   const int element = weight_dtype == MAXSIM_FLOAT32 ? 4 : 2;
   const int bits = bits_of((uint64_t)vocab);
   if (few_tokens(tokens, vocab)) {
-    const ZeroArgs zero = zero_args(dweight, vocab, dim * element, element);
+    ZeroArgs zero = zero_args(dweight, vocab, dim * element, element);
+    // one such workgroup per CU, beside one with a bucket
+    zero.rows = std::max(zero.rows, (uint32_t)std::min<int64_t>((vocab + 255) / 256, kZeroRows));
     const int64_t zero_groups = (vocab + zero.rows - 1) / zero.rows;
     FewArgs few{rows, dy, dy_stride, (uint32_t)tokens, (int)dim, std::min(bits, kBucketBits), 0, 0,
                 scale, zero};
@@ -1019,18 +1057,26 @@ int maxsim_amd_embed_backward(maxsim_dtype weight_dtype, maxsim_dtype dtype, con
   SortArgs sort{rows, nullptr, passes & 1 ? sorted : other, (uint32_t)tokens, (uint32_t)vocab, l.run,
                 0, (bits + passes - 1) / passes, reinterpret_cast<uint32_t*>(ws + l.counts), total, total + 1};
   const dim3 runs((unsigned)((tokens + l.run - 1) / l.run));
+  const bool counted = tokens > kCountAll;
   for (int p = 0; p < passes; ++p) {
-    if (p == 0) {
-      hipLaunchKernelGGL(embed_count_kernel<true>, runs, dim3(kSortThreads), 0, st, sort);
-      hipLaunchKernelGGL(embed_place_kernel<true>, runs, dim3(kSortThreads), 0, st, sort);
-    } else {
+    if (p > 0) {
       sort.in = sort.out;
       sort.out = sort.out == sorted ? other : sorted;
       sort.shift += sort.bits;
       sort.bits = std::min(sort.bits, bits - sort.shift);
-      hipLaunchKernelGGL(embed_count_kernel<false>, runs, dim3(kSortThreads), 0, st, sort);
-      hipLaunchKernelGGL(embed_place_kernel<false>, runs, dim3(kSortThreads), 0, st, sort);
     }
+    auto launch = [&](auto first) {
+      constexpr bool FIRST = decltype(first)::value;
+      const dim3 threads(kSortThreads);
+      if (counted) {
+        hipLaunchKernelGGL(embed_count_kernel<FIRST>, runs, threads, 0, st, sort);
+        hipLaunchKernelGGL((embed_place_kernel<FIRST, true>), runs, threads, 0, st, sort);
+      } else {
+        hipLaunchKernelGGL((embed_place_kernel<FIRST, false>), runs, threads, 0, st, sort);
+      }
+    };
+    if (p == 0) launch(std::true_type{});
+    else launch(std::false_type{});
     if (int e = check_launch("embed_place_kernel")) return e;
   }
   const SumArgs sum{dy, dy_stride, (int)dim, sorted, total, l.span, l.window, l.short_run,
