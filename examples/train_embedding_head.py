@@ -75,12 +75,13 @@ class Batches:
 
 
 def train(steps=200, batch=64, lq=32, ld=180, hidden=768, dim=128, dtype=torch.bfloat16,
-          state_bits=8, lr=2e-3, temperature=0.5, seed=0, report=20):
+          state_bits=8, lr=2e-3, temperature=0.5, seed=0, report=20, max_norm=None):
     """Returns the losses of all steps."""
     torch.manual_seed(seed)
     head = EmbeddingHead(hidden, dim, dtype).cuda()
     optimizer = maxsim_amd.AdamW(head.parameters(), lr=lr, weight_decay=0.01,
-                                 state_bits=state_bits, master_weights=dtype != torch.float32)
+                                 state_bits=state_bits, master_weights=dtype != torch.float32,
+                                 max_norm=max_norm)
     data = Batches(batch, lq, ld, hidden, dtype, seed)
     losses = []
     # one GPU per process: backward on this thread saves the hand-over to the
@@ -111,9 +112,12 @@ def main() -> None:
     parser.add_argument("--dtype", choices=("bf16", "f16", "f32"), default="bf16")
     parser.add_argument("--state-bits", type=int, choices=(8, 32), default=8)
     parser.add_argument("--lr", type=float, default=2e-3)
+    parser.add_argument("--max-norm", type=float, default=None,
+                        help="clip the gradients' norm on their way into the step")
     args = parser.parse_args()
     dtype = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}[args.dtype]
-    train(args.steps, args.batch, dtype=dtype, state_bits=args.state_bits, lr=args.lr)
+    train(args.steps, args.batch, dtype=dtype, state_bits=args.state_bits, lr=args.lr,
+          max_norm=args.max_norm)
 
 
 if __name__ == "__main__":
