@@ -28,8 +28,11 @@ namespace maxsim {
 // table (524288 tokens x 768, fp32 table, bf16 result: 217 us against 305, and
 // 579 against 617 with the layer norm that reads the result).  A smaller one is
 // mostly still there for its reader (40000 tokens: 18.7 against 20.1 us, but
-// 42.4 against 41.5 with the layer norm; 80000, 123 MB: 79 against 90).
-constexpr int64_t kCacheBytes = (int64_t)96 << 20;
+// 42.4 against 41.5 with the layer norm; 80000, 123 MB: 79 against 90).  Rows
+// that share lines with their neighbours leave pieces of lines behind, which
+// costs short ones more than it gives (256000 x 304 bf16: 44 us against 35, x 301
+// fp32 99 and 99, x 1038 bf16 137 against 199).
+constexpr int64_t kCacheBytes = (int64_t)96 << 20, kCacheRow = 2048;
 
 struct EmbedArgs {
   const void* weight;
@@ -521,14 +524,17 @@ __global__ __launch_bounds__(kSortThreads) void embed_count_kernel(SortArgs a) {
 template <bool FIRST, bool COUNTED>
 __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(SortArgs a) {
   __shared__ uint32_t counts[kSortWaves][kDigits];
-  __shared__ uint32_t sums[2][kSortThreads], waves[kSortWaves];
+  __shared__ uint32_t sums[COUNTED ? 2 * kSortThreads : kDigits], waves[kSortWaves];
   const int wave = threadIdx.x >> 6;
   const uint32_t digits = 1u << a.bits, mask = digits - 1;
   const uint32_t n = FIRST ? a.tokens : *a.total;
   count_share<FIRST>(a, n, counts[wave]);
   // of a digit: all entries, and those of the runs before
+  uint32_t all = 0, before = 0;
   if constexpr (!COUNTED) {
-    for (uint32_t i = threadIdx.x; i < digits; i += kSortThreads) sums[0][i] = sums[1][i] = 0;
+    // the former in the low half of a word, the latter in the high
+    static_assert(kCountAll < 65536, "counts of 16 bits");
+    if (threadIdx.x < digits) sums[threadIdx.x] = 0;
     __syncthreads();
     const uint32_t begin = blockIdx.x * a.run;
     constexpr int U = 8;
@@ -542,27 +548,18 @@ __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(SortArgs a) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const uint32_t i = i0 + u * kSortThreads + threadIdx.x;
-        if (i < n && row[u] < a.vocab) atomicAdd(&sums[i < begin][row[u] >> a.shift & mask], 1u);
+        if (i < n && row[u] < a.vocab)
+          atomicAdd(&sums[row[u] >> a.shift & mask], i < begin ? 0x10001u : 1u);
       }
     }
     __syncthreads();
-    const uint32_t before = threadIdx.x < digits ? sums[1][threadIdx.x] : 0;
-    const uint32_t all = threadIdx.x < digits ? sums[0][threadIdx.x] + before : 0;
-    uint32_t start = sum_before(all, waves);
-    if (FIRST && blockIdx.x == 0 && threadIdx.x == kSortThreads - 1)
-      *a.total = start + all, *a.begun = 0;
-    start += before;
     if (threadIdx.x < digits)
-      for (int w = 0; w < kSortWaves; ++w) {
-        const uint32_t c = counts[w][threadIdx.x];
-        counts[w][threadIdx.x] = start;
-        start += c;
-      }
+      all = sums[threadIdx.x] & 0xffff, before = sums[threadIdx.x] >> 16;
   } else {
     // several threads each
     const uint32_t d = threadIdx.x & mask, part = threadIdx.x >> a.bits;
-    const uint32_t parts = kSortThreads >> a.bits, groups = gridDim.x;
-    uint32_t all = 0, before = 0;
+    const uint32_t parts = min((uint32_t)kSortThreads >> a.bits, 16u);
+    const uint32_t groups = part < parts ? gridDim.x : 0;
     constexpr int U = 8;
     for (uint32_t g0 = part; g0 < groups; g0 += parts * U) {
       uint32_t c[U];
@@ -576,22 +573,23 @@ __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(SortArgs a) {
         before += g < blockIdx.x ? c[u] : 0;
       }
     }
-    sums[0][threadIdx.x] = all, sums[1][threadIdx.x] = before;
+    sums[threadIdx.x] = all, sums[kSortThreads + threadIdx.x] = before;
     __syncthreads();
     all = before = 0;
     if (threadIdx.x < digits)
-      for (uint32_t i = threadIdx.x; i < kSortThreads; i += digits)
-        all += sums[0][i], before += sums[1][i];
-    uint32_t start = sum_before(all, waves);
-    if (FIRST && blockIdx.x == 0 && threadIdx.x == kSortThreads - 1) *a.total = start + all, *a.begun = 0;
-    start += before;
-    if (threadIdx.x < digits)
-      for (int w = 0; w < kSortWaves; ++w) {
-        const uint32_t c = counts[w][threadIdx.x];
-        counts[w][threadIdx.x] = start;
-        start += c;
-      }
+      for (uint32_t i = threadIdx.x; i < digits * parts; i += digits)
+        all += sums[i], before += sums[kSortThreads + i];
   }
+  uint32_t start = sum_before(all, waves);
+  if (FIRST && blockIdx.x == 0 && threadIdx.x == kSortThreads - 1)
+    *a.total = start + all, *a.begun = 0;
+  start += before;
+  if (threadIdx.x < digits)
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = counts[w][threadIdx.x];
+      counts[w][threadIdx.x] = start;
+      start += c;
+    }
   __syncthreads();
   for_share<FIRST>(a, n, [&](Entry e, bool has) {
     const uint32_t d = e.row >> a.shift & mask;
@@ -612,7 +610,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(SortArgs a) {
 // of up to `short_run` tokens where it begins, of a longer one the part in each
 // window (spans are whole windows).  Parts of a run that reaches into other
 // windows are left in the workspace.  More workgroups write zeros.
-constexpr int kMaxShortRun = 64, kMaxWindow = 64, kMaxSpan = 512;
+constexpr int kMaxShortRun = 64, kMaxSpan = 512;
 
 struct SumArgs {
   const void* dy;
@@ -818,27 +816,31 @@ __global__ __launch_bounds__(row_threads(G)) void embed_sum_kernel(SumArgs a) {
 
 // Adds up the parts of the runs that go on from the window that they begin in,
 // a workgroup a run and kJoinColumns of its columns; a thread has four of them,
-// and of the parts a share.
+// and of the parts a share.  Where the runs are few and long, as with a table of
+// a few rows, 4 or 16 workgroups divide the columns among them and have as many
+// more shares.
 constexpr int kJoinThreads = 512, kJoinUnroll = 8, kJoinColumns = 256;
 template <typename W>
 __global__ __launch_bounds__(kJoinThreads) void embed_join_kernel(SumArgs a) {
   __shared__ float4 sums[kJoinThreads];
   const uint32_t runs = *a.begun, total = *a.total;
-  constexpr int across = kJoinColumns / 4, shares = kJoinThreads / across;
+  const uint32_t windows = total / a.window;  // of a run: windows / runs on average at most
+  const uint32_t split = runs * 16 <= gridDim.x && windows / 64 >= runs  ? 16
+                         : runs * 4 <= gridDim.x && windows / 16 >= runs ? 4
+                                                                         : 1;
+  const int across = kJoinColumns / 4 / split, shares = kJoinThreads / across;
   const int mine = threadIdx.x / across;
-  const int e0 = blockIdx.y * kJoinColumns + threadIdx.x % across * 4;
+  const int e0 = blockIdx.y * kJoinColumns +
+                 (blockIdx.x % split * across + threadIdx.x % across) * 4;
   const bool has = e0 < a.dim;
-  for (uint32_t r = blockIdx.x; r < runs; r += gridDim.x) {
+  for (uint32_t r = blockIdx.x / split; r < runs; r += gridDim.x / split) {
     const uint2 run = a.begins[r];
     const uint64_t begin = (uint64_t)run.x * a.window;
     // the windows after it that the run reaches into
-    uint32_t more = 0;
-    for (;;) {
-      const uint64_t i = begin + (uint64_t)(more + 1 + (threadIdx.x & 63)) * a.window;
-      const uint64_t same = __ballot(i < total && a.sorted[min(i, (uint64_t)total - 1)].row == run.y);
-      more += (uint32_t)__popcll(same);
-      if (~same) break;
-    }
+    const uint64_t i = begin + (uint64_t)(1 + (threadIdx.x & 63)) * a.window;
+    const uint64_t same = __ballot(i < total && a.sorted[min(i, (uint64_t)total - 1)].row == run.y);
+    uint32_t more = (uint32_t)__popcll(same);
+    if (more == 64) more = (first_of(a.sorted, total, (uint64_t)run.y + 1) - 1) / a.window - run.x;
     const uint32_t take = (more + shares - 1) / shares;
     const uint32_t lo = min(mine * take, more), hi = min(lo + take, more);
     const float* p = a.parts + (int64_t)run.x * 2 * a.part_dim + e0;
@@ -856,10 +858,14 @@ __global__ __launch_bounds__(kJoinThreads) void embed_join_kernel(SumArgs a) {
     sums[threadIdx.x] = s;
     __syncthreads();
     if (mine == 0 && has) {
+      static_assert(kJoinThreads / (kJoinColumns / 4) == 8, "shares are a multiple of 8");
+      s = make_float4(0, 0, 0, 0);
+      for (int i = 0; i < shares; i += 8) {
+        float4 v[8];
 #pragma unroll
-      for (int i = 1; i < shares; ++i) {
-        const float4 v = sums[i * across + threadIdx.x];
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        for (int u = 0; u < 8; ++u) v[u] = sums[(i + u) * across + threadIdx.x];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s.x += v[u].x, s.y += v[u].y, s.z += v[u].z, s.w += v[u].w;
       }
       auto* out = static_cast<typename W::storage*>(a.zero.dweight) + (int64_t)run.y * a.dim;
       const float f[4] = {s.x * a.scale, s.y * a.scale, s.z * a.scale, s.w * a.scale};
@@ -879,8 +885,15 @@ static int bits_of(uint64_t n) {  // that numbers below n have
   return b;
 }
 
-static bool few_tokens(int64_t tokens, int64_t vocab) {
-  return tokens <= kFewTokens && bits_of((uint64_t)vocab) <= kFewVocabBits;
+// Whether the one launch is the faster.  A workgroup of it has all tokens of a
+// row, so not where rows are few (tables of 6, 45 and 64 rows: 496, 2056 and
+// 2816 tokens at most; 3654 tokens of 6 rows 41 us against 19, 512 of 16 10 against 17)
+// or so wide that its waves share the columns alone (796 x 2560 fp32: 77 against
+// 28; 2048 x 768 bf16 of 32000 rows: 16 against 29).
+static bool few_tokens(maxsim_dtype dtype, int64_t tokens, int64_t vocab, int64_t dim) {
+  const int64_t columns = dtype == MAXSIM_FLOAT32 ? 64 * kVec<F32> : 64 * kVec<F16>;
+  return tokens <= std::min<int64_t>(256 + 40 * vocab, kFewTokens) && dim <= 4 * columns &&
+         bits_of((uint64_t)vocab) <= kFewVocabBits;
 }
 
 // Groups of lanes that hold a row in a workgroup.
@@ -901,15 +914,15 @@ struct EmbedLayout {
 };
 static EmbedLayout embed_layout(maxsim_dtype dtype, int64_t tokens, int64_t vocab, int64_t dim) {
   EmbedLayout l{};
-  if (few_tokens(tokens, vocab)) return l;
+  if (few_tokens(dtype, tokens, vocab, dim)) return l;
   // a group of lanes has up to 32 tokens, fewer where that leaves CUs idle
   const uint32_t groups = (uint32_t)row_groups(dtype, dim);
   uint32_t share = 32;
   while (share > 2 && tokens / share < 8192) share /= 2;
   l.span = std::min<uint32_t>(std::max<uint32_t>(groups * share, 8), kMaxSpan);
-  l.window = std::min<uint32_t>(l.span, kMaxWindow);
   // what the others have long done when a group ends with it
   l.short_run = std::min<uint32_t>(std::max<uint32_t>(2 * share, 16), kMaxShortRun);
+  l.window = std::min(l.span, l.short_run);
   l.windows = (tokens + l.window - 1) / l.window;
   l.part_dim = (int)((dim + 7) / 8 * 8);
   const int64_t each = (tokens + kSortGroups - 1) / kSortGroups;
@@ -973,7 +986,9 @@ int maxsim_amd_embed_forward(maxsim_dtype weight_dtype, maxsim_dtype dtype, cons
   const EmbedArgs all{weight, weight_stride, vocab, (int)dim, ids, ids64, sequences,
                       sequences * length, 0, (uint32_t)length, lengths, lengths64,
                       padding_idx < 0 ? -1 : padding_idx, scale, y, rows};
-  const bool past_cache = all.tokens * dim * (dtype == MAXSIM_FLOAT32 ? 4 : 2) > kCacheBytes;
+  const int64_t row_bytes = dim * (dtype == MAXSIM_FLOAT32 ? 4 : 2);
+  const bool past_cache = all.tokens * row_bytes > kCacheBytes &&
+                          (row_bytes % 64 == 0 || row_bytes >= kCacheRow);
   return with_embed_types(weight_dtype, dtype, [&](auto w, auto t) {
     using W = decltype(w);
     using T = decltype(t);
@@ -1025,7 +1040,7 @@ int maxsim_amd_embed_backward(maxsim_dtype weight_dtype, maxsim_dtype dtype, con
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int element = weight_dtype == MAXSIM_FLOAT32 ? 4 : 2;
   const int bits = bits_of((uint64_t)vocab);
-  if (few_tokens(tokens, vocab)) {
+  if (few_tokens(dtype, tokens, vocab, dim)) {
     ZeroArgs zero = zero_args(dweight, vocab, dim * element, element);
     // one such workgroup per CU, beside one with a bucket
     zero.rows = std::max(zero.rows, (uint32_t)std::min<int64_t>((vocab + 255) / 256, kZeroRows));

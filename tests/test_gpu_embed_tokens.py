@@ -59,8 +59,11 @@ def _gradient(dy, rows, vocab, scale):
         return oracle.embed_backward(f64(dy), rows, vocab, scale)
     real = torch.from_numpy(rows >= 0).cuda()
     at, d = torch.from_numpy(rows).cuda()[real], dy[real].double()
-    sums = [torch.zeros(vocab, dy.shape[1], dtype=torch.float64, device="cuda").index_add_(0, at, x)
-            for x in (d, d.abs())]
+    if vocab <= 64:  # few rows: atomics would wait for each other
+        sums = [torch.stack([x[at == v].sum(0) for v in range(vocab)]) for x in (d, d.abs())]
+    else:
+        sums = [torch.zeros(vocab, dy.shape[1], dtype=torch.float64, device="cuda").index_add_(0, at, x)
+                for x in (d, d.abs())]
     count = np.bincount(rows[rows >= 0], minlength=vocab)[:, None]
     return f64(sums[0]) * scale, abs(scale) * (count + 2) * 2.0 ** -24 * f64(sums[1])
 
@@ -152,6 +155,34 @@ def test_rows_of_one_bucket():
     for tokens in (4096, 20011):
         ids = torch.randint(0, vocab // 512, (tokens,), generator=gen) * 512 + 17
         _check(rand(gen, vocab, 8), ids.cuda(), gen=gen)
+
+
+@pytest.mark.parametrize("vocab,tokens", [(1, 296), (1, 297), (2, 336), (2, 337), (6, 496), (6, 497),
+                                          (96, 4096), (96, 4097), (500, 20480), (500, 20481)])
+@pytest.mark.parametrize("dim", [64, 512, 1024, 1025, 2048, 2049])
+def test_where_the_launches_change(vocab, tokens, dim):
+    gen = torch.Generator().manual_seed(tokens)
+    for dtype in (torch.bfloat16, torch.float32):
+        _check(rand(gen, vocab, dim, dtype=dtype), _ids(gen, vocab, tokens), gen=gen)
+
+
+@pytest.mark.parametrize("vocab,tokens,dim", [(2, 300001, 64), (3, 70000, 72), (40, 131073, 8),
+                                              (1, 100000, 300)])
+def test_long_runs(vocab, tokens, dim):
+    gen = torch.Generator().manual_seed(tokens)
+    _check(rand(gen, vocab, dim, dtype=torch.bfloat16), _ids(gen, vocab, tokens), gen=gen)
+
+
+@pytest.mark.parametrize("dim", [300, 304, 320, 1030])
+def test_results_past_the_caches(dim):
+    # more than 96 MiB, in rows that are whole lines and that are not
+    gen = torch.Generator().manual_seed(dim)
+    tokens = (100 << 20) // (2 * dim) + 3
+    weight = rand(gen, 1000, dim, dtype=torch.float16)
+    ids = _ids(gen, 1000, tokens)
+    lens = torch.tensor([tokens - 70], device="cuda")
+    y = maxsim_amd.embed_tokens(weight, ids[None], lens, scale=0.5)[0]
+    assert torch.equal(y[:-70], weight[ids[:-70]] * 0.5) and not y[-70:].any()
 
 
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64], ids=str)
