@@ -59,7 +59,7 @@ typedef struct {
   maxsim_dtype dtype;
 } maxsim_grad_tensor;
 
-/* Bytes of workspace of the norm (partial sums). */
+/* Bytes of workspace of the norm and of clipping (partial sums). */
 size_t maxsim_amd_grad_norm_workspace_size(const maxsim_grad_tensor* tensors, int64_t count);
 
 /* norm = the root of the sum of all squares of `count` tensors (host array,
@@ -70,10 +70,11 @@ int maxsim_amd_grad_norm(const maxsim_grad_tensor* tensors, int64_t count, doubl
                          double eps, float* norm, float* factor, void* workspace,
                          size_t workspace_bytes, void* stream);
 
-/* Every element times *factor (on the device), rounded once, in place; nothing
+/* The same, and every element times the factor, rounded once, in place; nothing
  * is moved where the factor is 1.  No two tensors overlap. */
-int maxsim_amd_scale_grads(const maxsim_grad_tensor* tensors, int64_t count, const float* factor,
-                           void* stream);
+int maxsim_amd_clip_grads(const maxsim_grad_tensor* tensors, int64_t count, double max_norm,
+                          double eps, float* norm, float* factor, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 /* ---- AdamW on scaled gradients ------------------------------------------- */
 

@@ -898,16 +898,16 @@ void check_clip(double max_norm, double eps) {
   TORCH_CHECK_VALUE(eps >= 0.0 && eps < 1e30, "eps must be finite and >= 0; got ", eps);
 }
 
-// Norm and factor of what prep_grads gave.
+// Norm and factor of what prep_grads gave; clip: which is then clipped.
 std::tuple<Tensor, Tensor> run_grad_norm(const Grads& g, const Tensor& like, double max_norm,
-                                         double eps) {
+                                         double eps, bool clip) {
   Tensor norm = empty_like_on(like, {}, at::kFloat), factor = empty_like_on(like, {}, at::kFloat);
   const int64_t count = (int64_t)g.list.size();
   const size_t bytes = maxsim_amd_grad_norm_workspace_size(g.list.data(), count);
   Tensor ws = empty_like_on(like, {(int64_t)bytes}, at::kByte);
-  check_status(maxsim_amd_grad_norm(g.list.data(), count, max_norm, eps, norm.data_ptr<float>(),
-                                    factor.data_ptr<float>(), ws.data_ptr(), bytes,
-                                    current_stream(like)));
+  check_status((clip ? maxsim_amd_clip_grads : maxsim_amd_grad_norm)(
+      g.list.data(), count, max_norm, eps, norm.data_ptr<float>(), factor.data_ptr<float>(),
+      ws.data_ptr(), bytes, current_stream(like)));
   return {norm, factor};
 }
 
@@ -917,7 +917,7 @@ std::tuple<Tensor, Tensor> maxsim_clip_factor(at::TensorList grads, double max_n
   at::AutoDispatchBelowADInplaceOrView below;  // a gradient's copy records nothing
   const Grads g = prep_grads(grads, false);
   c10::hip::HIPGuardMasqueradingAsCUDA guard(grads[0].device());
-  return run_grad_norm(g, grads[0], max_norm, eps);
+  return run_grad_norm(g, grads[0], max_norm, eps, false);
 }
 
 Tensor maxsim_clip_grad_norm(at::TensorList grads, double max_norm, double eps) {
@@ -926,9 +926,7 @@ Tensor maxsim_clip_grad_norm(at::TensorList grads, double max_norm, double eps) 
   at::AutoDispatchBelowADInplaceOrView below;
   const Grads g = prep_grads(grads, true);
   c10::hip::HIPGuardMasqueradingAsCUDA guard(grads[0].device());
-  auto [norm, factor] = run_grad_norm(g, grads[0], max_norm, eps);
-  check_status(maxsim_amd_scale_grads(g.list.data(), (int64_t)g.list.size(),
-                                      factor.data_ptr<float>(), current_stream(grads[0])));
+  const Tensor norm = std::get<0>(run_grad_norm(g, grads[0], max_norm, eps, true));
   for (const Tensor& t : grads) touched(t);
   return norm;
 }

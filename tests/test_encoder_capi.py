@@ -67,7 +67,7 @@ def test_embed_backward_refusals(lib):
     assert size(BF16, 2 ** 31, 9, 64) == 0 and size(9, 100, 9, 64) == 0
     need = size(BF16, 10000, 9, 64)
     assert need >= 10000 * 16
-    assert size(BF16, 4096, 9, 64) == 0  # few tokens need none
+    assert size(BF16, 600, 9, 64) == 0 == size(BF16, 4096, 96, 64)  # few tokens need none
     fn = lib.maxsim_amd_embed_backward
     fn.argtypes = [INT, INT, P, I64, P, I64, I64, I64, F, P, P, SIZE, P]
 
@@ -90,8 +90,8 @@ def test_gradient_list_refusals(lib):
     size.restype, size.argtypes = SIZE, [P, I64]
     norm = lib.maxsim_amd_grad_norm
     norm.argtypes = [P, I64, D, D, P, P, P, SIZE, P]
-    scale = lib.maxsim_amd_scale_grads
-    scale.argtypes = [P, I64, P, P]
+    clip = lib.maxsim_amd_clip_grads
+    clip.argtypes = norm.argtypes
     good = (Grad * 2)(Grad(ONE, 5, F32), Grad(ONE, 10 ** 6, BF16))
     need = size(good, 2)
     assert need % 8 == 0 and 8 * 2 <= need <= 8 * 1000
@@ -99,10 +99,9 @@ def test_gradient_list_refusals(lib):
     for bad, text in ((Grad(ONE, 5, 7), b"dtype"), (Grad(ONE, -1, F32), b"negative"),
                       (Grad(None, 1, F32), b"null")):
         one = (Grad * 1)(bad)
-        assert norm(one, 1, 1.0, 0.0, ONE, ONE, ONE, 64, None) == INVALID
-        assert text in lib.maxsim_amd_last_error()
-        assert scale(one, 1, ONE, None) == INVALID
-        assert text in lib.maxsim_amd_last_error()
+        for fn in (norm, clip):
+            assert fn(one, 1, 1.0, 0.0, ONE, ONE, ONE, 64, None) == INVALID
+            assert text in lib.maxsim_amd_last_error()
     for args, text in (((None, 2, 1.0, 0.0, ONE, ONE, ONE, need), b"no tensors"),
                        ((good, -1, 1.0, 0.0, ONE, ONE, ONE, need), b"no tensors"),
                        ((good, 2, 1.0, 0.0, None, ONE, ONE, need), b"null"),
@@ -111,12 +110,12 @@ def test_gradient_list_refusals(lib):
                        ((good, 2, 1.0, -1.0, ONE, ONE, ONE, need), b"max_norm"),
                        ((good, 2, 1.0, 0.0, ONE, ONE, None, need), b"workspace"),
                        ((good, 2, 1.0, 0.0, ONE, ONE, ONE, need - 1), b"workspace")):
-        assert norm(*args, None) == INVALID, text
-        assert text in lib.maxsim_amd_last_error()
-    assert scale(good, 2, None, None) == INVALID
-    assert scale(None, 0, ONE, None) == OK
+        for fn in (norm, clip):
+            assert fn(*args, None) == INVALID, text
+            assert text in lib.maxsim_amd_last_error()
+    assert clip(good, 2, 1.0, 0.0, ONE, None, ONE, need, None) == INVALID
     large = (Grad * 1)(Grad(ONE, 2 ** 50, F32))
-    assert scale(large, 1, ONE, None) == UNSUPPORTED
+    assert clip(large, 1, 1.0, 0.0, ONE, ONE, ONE, need, None) == UNSUPPORTED
 
 
 def test_scaled_step_refusals(lib):

@@ -90,7 +90,9 @@ def test_the_limit():
 
 
 @pytest.mark.parametrize("dtypes", [[t] for t in DTYPES] + [DTYPES], ids=str)
-@pytest.mark.parametrize("sizes", [[1], SIZES, [0, 5, 0], [11] * 399 + [70001]],
+@pytest.mark.parametrize("sizes", [[1], SIZES, [0, 5, 0], [11] * 399 + [70001], [3000] * 198,
+                                   [3000] * 199, [256 * 2048], [256 * 2048 + 1], [0] * 200 + [7],
+                                   [2100000], [4300000]],
                          ids=lambda s: f"{len(s)}x{s[0]}")
 def test_clipping(sizes, dtypes):
     grads = _list(sizes, dtypes, seed=1)
