@@ -20,6 +20,10 @@ from maxsim_amd import (  # noqa: F401  (re-exported)
     _pack_padded,
     adamw_state_values,
     adamw_step,
+    clip_factor,
+    clip_grad_norm,
+    embed_tokens,
+    grad_norm,
     host_checks,
     layer_norm,
     maxsim_reference,

@@ -245,6 +245,7 @@ constexpr int kTokenBits = 12, kFewTokens = 1 << kTokenBits;
 constexpr int kBucketBits = 8;   // low bits of a row: a workgroup per CU
 constexpr int kFewVocabBits = 32 - kTokenBits + kBucketBits;
 constexpr int kFewDigitBits = 8; // high bits that a pass sorts by
+constexpr int kFewBlocks = 4;    // of 64 chunks of 16 bytes: a row at most
 constexpr int kWaveIds = kFewTokens / kSortWaves;
 static_assert(kWaveIds == 64 * 4, "four ids per lane");
 
@@ -371,82 +372,71 @@ __global__ __launch_bounds__(kSortThreads) void embed_few_kernel(FewArgs a) {
     __syncthreads();
   }
 
-  // Sums: waves share the columns, kColumns each, and where there are more
-  // waves than that, the sorted tokens.  A run that began in an earlier wave's
-  // share is left in LDS for that wave.
-  const int blocks = (a.dim + kColumns - 1) / kColumns;
-  const int across = min(blocks, kSortWaves), shares = kSortWaves / across;
+  // Sums: waves share the columns, kColumns each (kFewBlocks of those at most),
+  // and the sorted tokens.  A run that began in an earlier wave's share is left
+  // in LDS for that wave.
+  const int across = (a.dim + kColumns - 1) / kColumns, shares = kSortWaves / across;
   const int share = wave / across;
   const uint32_t take = (m + shares - 1) / shares;
   const uint32_t begin = share < shares ? min(share * take, m) : m, end = min(begin + take, m);
   auto row_at = [&](uint32_t i) { return sorted[i] >> kTokenBits; };
   const bool joins = begin > 0 && begin < end && row_at(begin) == row_at(begin - 1);
   const bool goes_on = begin < end && end < m && row_at(end) == row_at(end - 1);
-  for (int round = 0; round * across < blocks; ++round) {
-    const int block = round * across + wave % across;
-    const int e0 = block * kColumns + lane * V;
-    const bool active = block < blocks && begin < end;
-    float acc[V];
+  const int e0 = wave % across * kColumns + lane * V;
+  float acc[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0.0f;
-    auto write_row = [&](uint32_t row) {
-      auto* out = static_cast<typename W::storage*>(a.zero.dweight) +
-                  (int64_t)(row << a.bucket_bits | bucket) * a.dim;
+  for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+  auto write_row = [&](uint32_t row) {
+    auto* out = static_cast<typename W::storage*>(a.zero.dweight) +
+                (int64_t)(row << a.bucket_bits | bucket) * a.dim;
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] *= a.scale;
-      store_piece<W, V>(out, e0, a.dim, acc);
-    };
-    bool part = joins;
-    uint32_t row = active ? row_at(begin) : 0;
-    if (active) {
-      for (uint32_t i = begin; i < end; i += U) {
-        Chunk<T> raw[U];
-        uint32_t entry[U];
+    for (int e = 0; e < V; ++e) acc[e] *= a.scale;
+    store_piece<W, V>(out, e0, a.dim, acc);
+  };
+  auto leave_part = [&] {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          entry[u] = sorted[min(i + u, end - 1)];
-          const S* dy = static_cast<const S*>(a.dy) + (entry[u] & (kFewTokens - 1)) * a.dy_row;
-          raw[u] = load_pieces<T>(dy, e0, a.dim);
-        }
+    for (int e = 0; e < V; ++e) lds.parts[wave][lane * V + e] = acc[e];
+  };
+  bool part = joins;
+  uint32_t row = begin < end ? row_at(begin) : 0;
+  for (uint32_t i = begin; i < end; i += U) {
+    Chunk<T> raw[U];
+    uint32_t entry[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (i + u >= end) break;
-          if (entry[u] >> kTokenBits != row) {
-            if (part) {
-#pragma unroll
-              for (int e = 0; e < V; ++e) lds.parts[wave][lane * V + e] = acc[e];
-            } else {
-              write_row(row);
-            }
-            part = false;
-            row = entry[u] >> kTokenBits;
-#pragma unroll
-            for (int e = 0; e < V; ++e) acc[e] = 0.0f;
-          }
-          float f[V];
-          unpack<T>(raw[u], f);
-#pragma unroll
-          for (int e = 0; e < V; ++e) acc[e] += f[e];
-        }
-      }
-      if (part) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) lds.parts[wave][lane * V + e] = acc[e];
-      } else if (!goes_on) {
-        write_row(row);
-      }
+    for (int u = 0; u < U; ++u) {
+      entry[u] = sorted[min(i + u, end - 1)];
+      const S* dy = static_cast<const S*>(a.dy) + (entry[u] & (kFewTokens - 1)) * a.dy_row;
+      raw[u] = load_pieces<T>(dy, e0, a.dim);
     }
-    __syncthreads();
-    if (active && goes_on && !part) {
-      for (int s = share + 1; s < shares; ++s) {
-        if (s * take >= m || row_at(s * take) != row) break;
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          acc[e] += lds.parts[s * across + wave % across][lane * V + e];
+    for (int u = 0; u < U; ++u) {
+      if (i + u >= end) break;
+      if (entry[u] >> kTokenBits != row) {
+        if (part) leave_part();
+        else write_row(row);
+        part = false;
+        row = entry[u] >> kTokenBits;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = 0.0f;
       }
-      write_row(row);
+      float f[V];
+      unpack<T>(raw[u], f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += f[e];
     }
-    __syncthreads();
+  }
+  if (begin < end) {
+    if (part) leave_part();
+    else if (!goes_on) write_row(row);
+  }
+  __syncthreads();
+  if (goes_on && !part) {
+    for (int s = share + 1; s < shares; ++s) {
+      if (s * take >= m || row_at(s * take) != row) break;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += lds.parts[s * across + wave % across][lane * V + e];
+    }
+    write_row(row);
   }
 }
 
@@ -892,7 +882,7 @@ static int bits_of(uint64_t n) {  // that numbers below n have
 // 28; 2048 x 768 bf16 of 32000 rows: 16 against 29).
 static bool few_tokens(maxsim_dtype dtype, int64_t tokens, int64_t vocab, int64_t dim) {
   const int64_t columns = dtype == MAXSIM_FLOAT32 ? 64 * kVec<F32> : 64 * kVec<F16>;
-  return tokens <= std::min<int64_t>(256 + 40 * vocab, kFewTokens) && dim <= 4 * columns &&
+  return tokens <= std::min<int64_t>(256 + 40 * vocab, kFewTokens) && dim <= kFewBlocks * columns &&
          bits_of((uint64_t)vocab) <= kFewVocabBits;
 }
 

@@ -125,3 +125,33 @@ def test_scaled_step_refusals(lib):
     assert fn(F32, F32, 16, None, 0, ONE, 1e-3, None, 0.9, 0.999, 1e-8, 0.0, 1, None, 0,
               None) == INVALID
     assert b"state_bits" in lib.maxsim_amd_last_error()
+
+
+def test_the_operators_are_exported():
+    import maxsim
+    import maxsim_amd
+    from maxsim_amd import training
+
+    for name in ("embed_tokens", "grad_norm", "clip_factor", "clip_grad_norm"):
+        assert getattr(maxsim, name) is getattr(maxsim_amd, name) is getattr(training, name)
+        assert name not in maxsim_amd.__all__  # which stays the reference's list
+
+
+def test_host_tensors_are_refused():
+    import torch
+
+    import maxsim_amd
+
+    table, ids = torch.zeros(4, 8), torch.zeros(3, dtype=torch.int64)
+    for call in (lambda: maxsim_amd.embed_tokens(table, ids), lambda: maxsim_amd.grad_norm([table]),
+                 lambda: maxsim_amd.clip_grad_norm(table, 1.0),
+                 lambda: maxsim_amd.clip_factor([table], 1.0)):
+        with pytest.raises(RuntimeError, match="HIP"):
+            call()
+    for padding in (4, -5):
+        with pytest.raises((RuntimeError, ValueError)):
+            maxsim_amd.embed_tokens(table, ids, padding_idx=padding)
+    assert float(maxsim_amd.grad_norm([])) == 0.0
+    for value in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_norm"):
+            maxsim_amd.AdamW([torch.nn.Parameter(table)], max_norm=value)

@@ -287,15 +287,57 @@ def test_layouts_of_the_table():
             assert torch.equal(got[1], want[1])
 
 
-def test_layouts_of_the_gradient():
+@pytest.mark.parametrize("n", [30, 130])
+def test_layouts_of_the_gradient(n):
     gen = torch.Generator().manual_seed(11)
-    weight, ids = rand(gen, 60, 77, dtype=torch.float16), _ids(gen, 60, 30, 40)
-    wide = rand(gen, 30, 40, 90, dtype=torch.float16)
-    for dy in (wide[..., 3:80], wide[:, :1, :77].expand(30, 40, 77), wide[0, 0, :77].expand(30, 40, 77),
-               rand(gen, 77, 40, 30, dtype=torch.float16).permute(2, 1, 0),
-               rand(gen, 40, 30, 77, dtype=torch.float16).transpose(0, 1)):
+    weight, ids = rand(gen, 160, 77, dtype=torch.float16), _ids(gen, 160, n, 40)
+    wide = rand(gen, n, 40, 90, dtype=torch.float16)
+    for dy in (wide[..., 3:80], wide[:, :1, :77].expand(n, 40, 77), wide[0, 0, :77].expand(n, 40, 77),
+               rand(gen, 77, 40, n, dtype=torch.float16).permute(2, 1, 0),
+               rand(gen, 40, n, 77, dtype=torch.float16).transpose(0, 1)):
         got = _check(weight, ids, dy=dy)[1]
         assert torch.equal(got, _grad(weight, ids, dy=dy.contiguous()))
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("tokens", [1000, 9000])
+def test_what_is_not_finite_stays_in_its_row(tokens, value):
+    gen = torch.Generator().manual_seed(tokens)
+    weight, ids = rand(gen, 300, 130), _ids(gen, 300, tokens)
+    dy = rand(gen, tokens, 130)
+    clean = _grad(weight, ids, dy=dy)
+    for at in (0, tokens // 2, tokens - 1):
+        bad = dy.clone()
+        bad[at, 5] = value
+        got = _grad(weight, ids, dy=bad)
+        row = int(ids[at])
+        assert not torch.isfinite(got[row, 5])
+        got[row, 5] = clean[row, 5]
+        assert torch.equal(got, clean)
+    # and what the table holds in the rows that are looked up
+    weight[7] = value
+    y = maxsim_amd.embed_tokens(weight, ids)
+    assert torch.equal(torch.isfinite(y).all(1), ids != 7)
+
+
+@pytest.mark.parametrize("vocab", [3, 300, 70001])
+@pytest.mark.parametrize("tokens", [200, 4000, 9000, 50000])
+def test_rows_outside_the_table_in_the_backward(tokens, vocab):
+    # through the operator: its rows may hold anything
+    from maxsim_amd._ops import ops
+
+    gen = torch.Generator().manual_seed(tokens)
+    rows = torch.randint(-3, vocab + 3, (tokens,), generator=gen)
+    rows[torch.randint(0, tokens, (9,), generator=gen)] = 2 ** 31 - 1
+    rows[torch.randint(0, tokens, (9,), generator=gen)] = -2 ** 31
+    dy = rand(gen, tokens, 24)
+    got = ops.maxsim_embed_tokens_backward(dy, rows.int().cuda(), vocab, 2.0, torch.float32)
+    known = np.where((rows >= 0) & (rows < vocab), rows, -1)
+    exact, bound = oracle.embed_backward(f64(dy), known, vocab, 2.0)
+    assert_within(got, exact, bound)
+    none = ops.maxsim_embed_tokens_backward(dy, torch.full((tokens,), -1, dtype=torch.int32, device="cuda"),
+                                            vocab, 2.0, torch.float32)
+    assert not none.any()
 
 
 def test_the_same_bits_every_time():
