@@ -71,7 +71,7 @@ template <int BITS, bool MASTER> struct AdamArgs {
   // read on the device where given: the learning rate, and the step count
   const float* lr_at;
   const int64_t* step_at;
-  const float* grad_scale;  // what gradients are multiplied by; NULL: 1
+  const float* grad_scale;  // what gradients are multiplied by, if they are
   float weight_decay;
   double beta1, beta2;
   uint64_t seed;
@@ -226,16 +226,17 @@ __device__ __forceinline__ uint2 top_bytes(const uint32_t (&q)[8]) {
 struct AdamStep {
   float decay, size, root;  // lr weight_decay, lr / c1, 1 / sqrt(c2)
   uint32_t key;
-  float grad_scale;
 };
 
 // Tensor k's elements from base on.  The quotient is a product with the
 // hardware's reciprocal (1 ulp): the update is off by a few 1e-7 of itself,
 // and exact roots and quotients made the step bound by arithmetic (bf16 with
 // 8-bit states, 66 M parameters: 190 us against 155).
-template <typename P, typename Gr, int BITS, bool MASTER, bool FULL>
+// SCALED: gradients are multiplied by *a.grad_scale, in fp32 (a test of the
+// pointer in one kernel for both cost the 8-bit step 3 %: 227 us against 220).
+template <typename P, typename Gr, int BITS, bool MASTER, bool SCALED, bool FULL>
 __device__ __forceinline__ void adam_chunk(const AdamArgs<BITS, MASTER>& a, int k,
-                                           const AdamStep& h, int64_t base) {
+                                           const AdamStep& h, float scale, int64_t base) {
 #pragma clang fp contract(off)
   const int64_t n = a.n[k];
   const int64_t i = base + threadIdx.x * kLaneElems;
@@ -259,9 +260,9 @@ __device__ __forceinline__ void adam_chunk(const AdamArgs<BITS, MASTER>& a, int 
     load8<F32, FULL>(a.m[k], i, n, m);
     load8<F32, FULL>(a.v[k], i, n, v);
   }
-  if (a.grad_scale) {
+  if constexpr (SCALED) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) g[e] *= h.grad_scale;
+    for (int e = 0; e < 8; ++e) g[e] *= scale;
   }
   uint32_t big_m = 0, big_v = 0;
 #pragma unroll
@@ -311,7 +312,7 @@ __device__ __forceinline__ void adam_chunk(const AdamArgs<BITS, MASTER>& a, int 
   }
 }
 
-template <typename P, typename Gr, int BITS, bool MASTER>
+template <typename P, typename Gr, int BITS, bool MASTER, bool SCALED>
 __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs<BITS, MASTER> a) {
   // the last tensor that starts at or before this chunk: one load per wave
   // instead of a chain of them
@@ -333,10 +334,11 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs<BITS, MAST
     c1 = c[0], c2 = c[1];
     key = dither_key(a.seed, (uint64_t)step);
   }
-  const AdamStep h{decay, lr / c1, 1.0f / sqrtf(c2), key, a.grad_scale ? *a.grad_scale : 1.0f};
+  const AdamStep h{decay, lr / c1, 1.0f / sqrtf(c2), key};
+  const float scale = SCALED ? *a.grad_scale : 1.0f;
   const int64_t base = (int64_t)(chunk - a.first[k]) * kChunkElems;
-  if (base + kChunkElems <= a.n[k]) adam_chunk<P, Gr, BITS, MASTER, true>(a, k, h, base);
-  else adam_chunk<P, Gr, BITS, MASTER, false>(a, k, h, base);
+  if (base + kChunkElems <= a.n[k]) adam_chunk<P, Gr, BITS, MASTER, SCALED, true>(a, k, h, scale, base);
+  else adam_chunk<P, Gr, BITS, MASTER, SCALED, false>(a, k, h, scale, base);
 }
 
 // The values of 8-bit states in bf16, which holds their 4 significant bits.
@@ -432,9 +434,14 @@ int maxsim_amd_adamw_step_scaled(maxsim_dtype param_dtype, maxsim_dtype grad_dty
     a.beta1 = beta1, a.beta2 = beta2, a.seed = seed;
     uint32_t chunks = 0;
     auto launch = [&] {
-      hipLaunchKernelGGL((adamw_kernel<decltype(p), decltype(g), BITS, MASTER>), dim3(chunks),
-                         dim3(kAdamThreads), BITS == 32 ? kReservedLds : 0,
-                         static_cast<hipStream_t>(stream), a);
+      auto go = [&](auto scaled) {
+        hipLaunchKernelGGL(
+            (adamw_kernel<decltype(p), decltype(g), BITS, MASTER, decltype(scaled)::value>),
+            dim3(chunks), dim3(kAdamThreads), BITS == 32 ? kReservedLds : 0,
+            static_cast<hipStream_t>(stream), a);
+      };
+      if (grad_scale) go(std::true_type{});
+      else go(std::false_type{});
       a.count = 0, chunks = 0;
       return check_launch("adamw_kernel");
     };
