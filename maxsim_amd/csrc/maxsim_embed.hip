@@ -241,13 +241,13 @@ __device__ __forceinline__ void zero_rows(const ZeroArgs& a, uint32_t first, con
 // dy; more workgroups write the rows without a token.  An entry is a number:
 // the high bits above a token's kTokenBits, so that order of rows and then of
 // tokens is the order of the numbers.
-constexpr int kTokenBits = 12, kFewTokens = 1 << kTokenBits;
+constexpr int kTokenBits = 11, kFewTokens = 1 << kTokenBits;
 constexpr int kBucketBits = 8;   // low bits of a row: a workgroup per CU
 constexpr int kFewVocabBits = 32 - kTokenBits + kBucketBits;
 constexpr int kFewDigitBits = 8; // high bits that a pass sorts by
 constexpr int kFewBlocks = 4;    // of 64 chunks of 16 bytes: a row at most
 constexpr int kWaveIds = kFewTokens / kSortWaves;
-static_assert(kWaveIds == 64 * 4, "four ids per lane");
+static_assert(kWaveIds == 64 * 2, "two ids per lane");
 
 struct FewArgs {
   const int32_t* rows;
@@ -260,15 +260,15 @@ struct FewArgs {
   ZeroArgs zero;
 };
 
-// Four ids in a row; past the end there is no row.
+// Two ids in a row; past the end there is no row.
 __device__ __forceinline__ void load_rows(const int32_t* rows, uint32_t i, uint32_t n,
-                                          uint32_t (&key)[4]) {
-  if (i + 4 <= n) {
-    const uint4 q = load_any<uint4>(rows + i);
-    key[0] = q.x, key[1] = q.y, key[2] = q.z, key[3] = q.w;
+                                          uint32_t (&key)[2]) {
+  if (i + 2 <= n) {
+    const uint2 q = load_any<uint2>(rows + i);
+    key[0] = q.x, key[1] = q.y;
   } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) key[e] = i + e < n ? (uint32_t)rows[i + e] : kNoRow;
+    key[0] = i < n ? (uint32_t)rows[i] : kNoRow;
+    key[1] = kNoRow;
   }
 }
 
@@ -287,8 +287,8 @@ __global__ __launch_bounds__(kSortThreads) void embed_few_kernel(FewArgs a) {
   __shared__ uint32_t sorted[kFewTokens];
   __shared__ uint32_t found[kSortWaves], waves[kSortWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t key[4];
-  const uint32_t i0 = wave * kWaveIds + lane * 4;
+  uint32_t key[2];
+  const uint32_t i0 = wave * kWaveIds + lane * 2;
   load_rows(a.rows, i0, a.tokens, key);
 
   if (blockIdx.x >= a.buckets) {
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_few_kernel(FewArgs a) {
     if (threadIdx.x < kZeroRows / 32) lds.has[threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 2; ++e) {
       const uint32_t r = key[e] - first;
       if (key[e] < a.zero.vocab && r < a.zero.rows) atomicOr(&lds.has[r / 32], 1u << (r & 31));
     }
@@ -308,16 +308,16 @@ __global__ __launch_bounds__(kSortThreads) void embed_few_kernel(FewArgs a) {
   // the wave's own, in order, to its part of the list
   const uint32_t bucket = blockIdx.x, low = (1u << a.bucket_bits) - 1;
   uint32_t* list = lds.sort.list + wave * kWaveIds;
-  uint64_t own[4];
+  uint64_t own[2];
   uint32_t at = 0, mine = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < 2; ++e) {
     own[e] = __ballot(key[e] < a.zero.vocab && (key[e] & low) == bucket);
     at += set_before(own[e]);
     mine += (uint32_t)__popcll(own[e]);
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
+  for (int e = 0; e < 2; ++e)
     if (own[e] >> lane & 1) list[at++] = key[e] >> a.bucket_bits << kTokenBits | (i0 + e);
   if (lane == 0) found[wave] = mine;
   __syncthreads();
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_few_kernel(FewArgs a) {
     for (int u = 0; u < U; ++u) {
       entry[u] = sorted[min(i + u, end - 1)];
       const S* dy = static_cast<const S*>(a.dy) + (entry[u] & (kFewTokens - 1)) * a.dy_row;
-      raw[u] = load_pieces<T>(dy, e0, a.dim);
+      raw[u] = load_chunk<T, true>(dy, e0, a.dim);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -420,6 +420,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_few_kernel(FewArgs a) {
         for (int e = 0; e < V; ++e) acc[e] = 0.0f;
       }
       float f[V];
+      place_chunk<T, true>(raw[u], e0, a.dim);
       unpack<T>(raw[u], f);
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[e] += f[e];
@@ -876,10 +877,11 @@ static int bits_of(uint64_t n) {  // that numbers below n have
 }
 
 // Whether the one launch is the faster.  A workgroup of it has all tokens of a
-// row, so not where rows are few (tables of 6, 45 and 64 rows: 496, 2056 and
-// 2816 tokens at most; 3654 tokens of 6 rows 41 us against 19, 512 of 16 10 against 17)
-// or so wide that its waves share the columns alone (796 x 2560 fp32: 77 against
-// 28; 2048 x 768 bf16 of 32000 rows: 16 against 29).
+// row, so not where rows are few (a table of 6 rows: 496 tokens at most; 3654 of
+// 6 rows 41 us against 19, 512 of 16 10 against 17) or so wide that its waves
+// share the columns alone (796 x 2560 fp32: 77 against 28; 2048 x 768 bf16 of
+// 32000 rows: 14 against 29).  4096 tokens would be 19 against 31, but 153
+// against 38 if all are of one row; the limit of 2048 leaves 78 against 31 there.
 static bool few_tokens(maxsim_dtype dtype, int64_t tokens, int64_t vocab, int64_t dim) {
   const int64_t columns = dtype == MAXSIM_FLOAT32 ? 64 * kVec<F32> : 64 * kVec<F16>;
   return tokens <= std::min<int64_t>(256 + 40 * vocab, kFewTokens) && dim <= kFewBlocks * columns &&

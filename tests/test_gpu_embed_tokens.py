@@ -158,6 +158,7 @@ def test_rows_of_one_bucket():
 
 
 @pytest.mark.parametrize("vocab,tokens", [(1, 296), (1, 297), (2, 336), (2, 337), (6, 496), (6, 497),
+                                          (44, 2016), (44, 2017), (45, 2048), (45, 2049),
                                           (96, 4096), (96, 4097), (500, 20480), (500, 20481)])
 @pytest.mark.parametrize("dim", [64, 512, 1024, 1025, 2048, 2049])
 def test_where_the_launches_change(vocab, tokens, dim):
