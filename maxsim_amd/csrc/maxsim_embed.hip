@@ -882,7 +882,10 @@ static int bits_of(uint64_t n) {  // that numbers below n have
 // share the columns alone (796 x 2560 fp32: 77 against 28; 2048 x 768 bf16 of
 // 32000 rows: 14 against 29).  4096 tokens would be 19 against 31, but 153
 // against 38 if all are of one row; the limit of 2048 leaves 78 against 31 there.
+// No tokens at all are the zeros alone, of rows of any width and number: nothing
+// is sorted, and the other path's shares would be empty.
 static bool few_tokens(maxsim_dtype dtype, int64_t tokens, int64_t vocab, int64_t dim) {
+  if (tokens == 0) return true;
   const int64_t columns = dtype == MAXSIM_FLOAT32 ? 64 * kVec<F32> : 64 * kVec<F16>;
   return tokens <= std::min<int64_t>(256 + 40 * vocab, kFewTokens) && dim <= kFewBlocks * columns &&
          bits_of((uint64_t)vocab) <= kFewVocabBits;
