@@ -487,11 +487,18 @@ bool wants(const optional<Tensor>& t) { return t.has_value() && t->requires_grad
 
 // No function here carries forward-mode tangents, and one that is dropped on
 // the way would count as 0.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool tangents_count() { return c10::AutogradState::get_tls_state().get_fw_grad_mode(); }
 void refuse_tangents(const char* name, const Tensor& a, const optional<Tensor>& b = std::nullopt,
                      const optional<Tensor>& c = std::nullopt) {
-  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-  const auto has = [](const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); };
-  TORCH_CHECK_NOT_IMPLEMENTED(!has(a) && !(b.has_value() && has(*b)) && !(c.has_value() && has(*c)),
+  if (!tangents_count()) return;
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(a) && !(b.has_value() && has_tangent(*b)) &&
+                                  !(c.has_value() && has_tangent(*c)),
+                              "maxsim_amd: ", name, " has no derivative in forward mode");
+}
+void refuse_tangents(const char* name, at::TensorList tensors) {
+  if (!tangents_count()) return;
+  TORCH_CHECK_NOT_IMPLEMENTED(std::none_of(tensors.begin(), tensors.end(), has_tangent),
                               "maxsim_amd: ", name, " has no derivative in forward mode");
 }
 
@@ -931,6 +938,20 @@ Tensor maxsim_clip_grad_norm(at::TensorList grads, double max_norm, double eps) 
   return norm;
 }
 
+// The norm, the factor and clipping record nothing in reverse mode: they are
+// for gradients, which seldom have any of their own.
+std::tuple<Tensor, Tensor> clip_factor_autograd(at::TensorList grads, double max_norm, double eps) {
+  refuse_tangents("clip_factor", grads);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return MAXSIM_CALL(maxsim_clip_factor, grads, max_norm, eps);
+}
+
+Tensor clip_grad_norm_autograd(at::TensorList grads, double max_norm, double eps) {
+  refuse_tangents("clip_grad_norm", grads);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return MAXSIM_CALL(maxsim_clip_grad_norm, grads, max_norm, eps);
+}
+
 // The values of 8-bit states, in bf16 (which holds them exactly).
 std::tuple<Tensor, Tensor> maxsim_adamw_state_values(const Tensor& exp_avg,
                                                      const Tensor& exp_avg_sq,
@@ -1022,8 +1043,8 @@ TORCH_LIBRARY_IMPL(maxsim_amd, AutogradCUDA, m) {
   m.impl("maxsim_normalize_embeddings", &normalize_autograd);
   m.impl("maxsim_pack_normalized", &pack_normalized_autograd);
   m.impl("maxsim_embed_tokens", &embed_autograd);
+  m.impl("maxsim_clip_factor", &clip_factor_autograd);
+  m.impl("maxsim_clip_grad_norm", &clip_grad_norm_autograd);
   // nothing to record, and its hundreds of tensors need not be looked at for it
   m.impl("maxsim_adamw_step", torch::CppFunction::makeFallthrough());
-  m.impl("maxsim_clip_factor", torch::CppFunction::makeFallthrough());
-  m.impl("maxsim_clip_grad_norm", torch::CppFunction::makeFallthrough());
 }

@@ -20,6 +20,8 @@ and ``include/maxsim_amd_encoder.h``: one pass over memory each, sums in fp32
 (the gradients' norm in 64 bits), 16-bit results rounded once.
 Differentiable means first derivatives in reverse mode: the gradients have no
 derivatives of their own and forward-mode tangents are not carried (both raise).
+The gradients' norm, the factor and clipping record nothing in reverse mode, as
+``torch.nn.utils``' do not; a tangent raises there too.
 All are exported from :mod:`maxsim_amd`.
 """
 
@@ -177,6 +179,8 @@ def clip_factor(grads, max_norm: float, *, eps: float = 1e-6) -> Tuple[torch.Ten
         decide: gradients of any finite size have a norm (infinite in fp32
         above its largest number; the factor still knows it).  A gradient that
         is not finite makes the norm inf or NaN and the factor 0 or NaN.
+        Neither has a gradient: to what is computed from them they are
+        constants, also where the gradients were made with ``create_graph``.
 
     The factor is :func:`adamw_step`'s ``grad_scale``: clipping then costs no
     pass over the gradients of its own."""
@@ -199,7 +203,8 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6) -> torch.Tensor
     The gradients (``[p.grad for p in parameters if p.grad is not None]``) are
     each dense in memory, in any order of their axes, and share none of it
     (ValueError).  Products are rounded once.  Nothing is written where the
-    norm is within the limit."""
+    norm is within the limit.  No graph records it: gradients made with
+    ``create_graph`` are differentiated as if they had not been clipped."""
     grads = _grad_list(grads)
     if not grads:
         return torch.zeros(())

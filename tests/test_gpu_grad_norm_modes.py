@@ -1,0 +1,52 @@
+"""The gradients' norm, the factor and clipping under torch's transforms: refused
+where a derivative or a batch would be dropped, and nothing clipped then."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import maxsim_amd
+
+from ._training_helpers import rand
+
+pytestmark = pytest.mark.gpu
+
+
+def _grads(seed):
+    gen = torch.Generator().manual_seed(seed)
+    return [rand(gen, 40, 7), rand(gen, 70001, dtype=torch.bfloat16), rand(gen, 3, 4, 5)]
+
+
+def test_tangents_are_refused_before_anything_is_written():
+    grads = _grads(0)
+    before = [g.clone() for g in grads]
+    for at, f in enumerate((lambda t: maxsim_amd.grad_norm([t, *grads]),
+                            lambda t: maxsim_amd.clip_factor([*grads, t], 0.01)[1],
+                            lambda t: maxsim_amd.clip_grad_norm([*grads, t], 0.01))):
+        x = rand(torch.Generator().manual_seed(at), 33)
+        kept = x.clone()
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            torch.func.jvp(f, (x,), (x,))
+        assert torch.equal(x, kept)
+    assert all(torch.equal(g, b) for g, b in zip(grads, before))
+
+
+def test_batches_are_refused():
+    x = rand(torch.Generator().manual_seed(3), 3, 50)
+    for f in (lambda t: maxsim_amd.grad_norm([t]), lambda t: maxsim_amd.clip_grad_norm([t], 1.0)):
+        with pytest.raises(RuntimeError, match="[Bb]atching rule"):
+            torch.vmap(f)(x)
+
+
+def test_gradients_with_a_graph():
+    # documented: the norm is a constant, the clipped values are what is read
+    p = rand(torch.Generator().manual_seed(4), 50).requires_grad_(True)
+    (g,) = torch.autograd.grad(p.square().sum(), p, create_graph=True)
+    want = maxsim_amd.clip_factor([g.detach().clone()], 0.5)
+    norm, factor = maxsim_amd.clip_factor([g], 0.5)
+    assert not norm.requires_grad and not factor.requires_grad
+    assert torch.equal(norm, want[0]) and torch.equal(factor, want[1])
+    kept = g.detach().clone()
+    assert torch.equal(maxsim_amd.clip_grad_norm([g], 0.5), norm)
+    assert torch.equal(g.detach(), kept * factor)
