@@ -65,7 +65,8 @@ size_t maxsim_amd_grad_norm_workspace_size(const maxsim_grad_tensor* tensors, in
 /* norm = the root of the sum of all squares of `count` tensors (host array,
  * read before the call returns), summed in 64 bits: gradients of any finite
  * size have one, in an order that the sizes alone decide.
- * factor (or NULL) = min(1, max_norm / (norm + eps)), NaN for a NaN norm. */
+ * factor (or NULL) = min(1, max_norm / (norm + eps)), 1 where norm + eps is 0,
+ * NaN for a NaN norm. */
 int maxsim_amd_grad_norm(const maxsim_grad_tensor* tensors, int64_t count, double max_norm,
                          double eps, float* norm, float* factor, void* workspace,
                          size_t workspace_bytes, void* stream);

@@ -1,7 +1,7 @@
 // The norm of many gradients together, the factor that clips them to a limit,
 // and clipping in place.
 //
-//   norm = sqrt(sum_i |g_i|^2),  factor = min(1, max_norm / (norm + eps))
+//   norm = sqrt(sum_i |g_i|^2),  factor = min(1, max_norm / (norm + eps)), 1 for 0 / 0
 //
 // Memory-bound: every gradient is read once (and written once where it is
 // clipped).  A launch takes up to kTensors tensors by their addresses in its
@@ -126,7 +126,8 @@ __global__ __launch_bounds__(kGradThreads) void grad_squares_kernel(GradArgs a) 
 }
 
 __device__ __forceinline__ float clip_factor(double norm, double max_norm, double eps) {
-  const double f = max_norm / (norm + eps);
+  // gradients of zeros are within a limit of 0 too
+  const double f = norm + eps == 0.0 ? 1.0 : max_norm / (norm + eps);
   return f > 1.0 ? 1.0f : (float)f;  // NaN stays
 }
 __device__ __forceinline__ void write_norm(double s, double max_norm, double eps, float* norm,

@@ -172,6 +172,7 @@ def clip_factor(grads, max_norm: float, *, eps: float = 1e-6) -> Tuple[torch.Ten
         grads: fp32 / fp16 / bf16 tensors on one device (any of the types
             together), or a single one.
         max_norm: >= 0; infinite: the factor is 1 for every finite norm.
+        eps: >= 0; where norm and eps are both 0, the factor is 1.
 
     Returns:
         Two fp32 tensors of one element on the gradients' device; nothing waits

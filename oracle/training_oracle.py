@@ -228,4 +228,4 @@ def grad_norm(grads):
 
 
 def clip_factor(norm, max_norm, eps):
-    return min(1.0, max_norm / (norm + eps))
+    return 1.0 if norm + eps == 0 else min(1.0, max_norm / (norm + eps))
