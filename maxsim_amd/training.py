@@ -163,6 +163,13 @@ def _grad_list(grads) -> list:
     return grads
 
 
+def _scalar_of_none(value: float, device=None) -> torch.Tensor:
+    """A result of no gradients at all: on the GPU that is in use if there is one."""
+    if device is None:
+        device = "cuda" if torch.cuda.is_available() else "cpu"
+    return torch.full((), value, dtype=torch.float32, device=device)
+
+
 def clip_factor(grads, max_norm: float, *, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
     """The norm of all gradients together, and what clips them to ``max_norm``::
 
@@ -175,11 +182,12 @@ def clip_factor(grads, max_norm: float, *, eps: float = 1e-6) -> Tuple[torch.Ten
         eps: >= 0; where norm and eps are both 0, the factor is 1.
 
     Returns:
-        Two fp32 tensors of one element on the gradients' device; nothing waits
-        for it.  Squares are added in 64 bits, in an order that the sizes alone
-        decide: gradients of any finite size have a norm (infinite in fp32
-        above its largest number; the factor still knows it).  A gradient that
-        is not finite makes the norm inf or NaN and the factor 0 or NaN.
+        Two fp32 tensors of one element on the gradients' device (no gradients:
+        0 and 1 on the current one); nothing waits for it.  Squares are added
+        in 64 bits, in an order that the sizes alone decide: gradients of any
+        finite size have a norm (infinite in fp32 above its largest number; the
+        factor still knows it).  A gradient that is not finite makes the norm
+        inf or NaN and the factor 0 or NaN.
         Neither has a gradient: to what is computed from them they are
         constants, also where the gradients were made with ``create_graph``.
 
@@ -187,7 +195,7 @@ def clip_factor(grads, max_norm: float, *, eps: float = 1e-6) -> Tuple[torch.Ten
     pass over the gradients of its own."""
     grads = _grad_list(grads)
     if not grads:
-        return torch.zeros(()), torch.ones(())
+        return _scalar_of_none(0.0), _scalar_of_none(1.0)
     return ops.maxsim_clip_factor(grads, max_norm, eps)
 
 
@@ -208,7 +216,7 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6) -> torch.Tensor
     ``create_graph`` are differentiated as if they had not been clipped."""
     grads = _grad_list(grads)
     if not grads:
-        return torch.zeros(())
+        return _scalar_of_none(0.0)
     return ops.maxsim_clip_grad_norm(grads, max_norm, eps)
 
 
@@ -305,8 +313,8 @@ class AdamW(torch.optim.Optimizer):
         max_norm: clip the gradients of all groups together to this norm on
             their way into the step (:func:`clip_factor`; they stay as they
             are, and are on one device).  ``grad_norm`` is their norm in the
-            last step, a tensor on the device.  None: no clipping.  Not part of
-            the state dict.
+            last step, a tensor on the device (0 where no parameter had a
+            gradient).  None: no clipping.  Not part of the state dict.
 
     State of a parameter: ``step`` (an int), ``exp_avg``, ``exp_avg_sq``, and
     ``scales`` / ``master`` where they apply.  ``state_dict`` round trips keep
@@ -345,6 +353,10 @@ class AdamW(torch.optim.Optimizer):
                  if p.grad is not None]
         if any(g.is_sparse for g in grads):
             raise RuntimeError("AdamW does not support sparse gradients")
+        if not grads:
+            devices = (p.device for group in self.param_groups for p in group["params"])
+            self.grad_norm = _scalar_of_none(0.0, next(devices, None))
+            return None
         self.grad_norm, factor = clip_factor(grads, self.max_norm)
         return factor
 

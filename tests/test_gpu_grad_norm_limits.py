@@ -45,3 +45,28 @@ def test_a_step_on_gradients_of_zeros():
     _, factor = maxsim_amd.clip_factor([g], 0.0, eps=0.0)
     maxsim_amd.adamw_step([p], [g], [m], [v], step=1, weight_decay=0.0, grad_scale=factor)
     assert bool((p == 1).all()) and not m.any() and not v.any()
+
+
+def test_no_gradients_have_a_norm_on_the_device():
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float64)
+    try:
+        norm, factor = maxsim_amd.clip_factor([], 1.0)
+        results = [norm, maxsim_amd.grad_norm([]), maxsim_amd.clip_grad_norm((), 1.0), factor]
+    finally:
+        torch.set_default_dtype(before)
+    for t, want in zip(results, (0.0, 0.0, 0.0, 1.0)):
+        assert t.is_cuda and t.dtype == torch.float32 and t.shape == () and float(t) == want
+
+
+def test_the_optimizer_without_gradients_has_its_norm_on_the_device():
+    p = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    opt = maxsim_amd.AdamW([p], max_norm=1.0)
+    opt.step()
+    assert opt.grad_norm.is_cuda and opt.grad_norm.dtype == torch.float32
+    assert float(opt.grad_norm) == 0.0 and bool((p == 1).all())
+    p.grad = torch.full_like(p, 2.0)
+    opt.step()
+    kept, p.grad = p.detach().clone(), None
+    opt.step()  # the norm is the last step's, not the one before
+    assert float(opt.grad_norm) == 0.0 and torch.equal(p, kept)
