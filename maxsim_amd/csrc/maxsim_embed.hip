@@ -891,13 +891,18 @@ static bool few_tokens(maxsim_dtype dtype, int64_t tokens, int64_t vocab, int64_
          bits_of((uint64_t)vocab) <= kFewVocabBits;
 }
 
-// Groups of lanes that hold a row in a workgroup.
-static int row_groups(maxsim_dtype dtype, int64_t dim) {
-  int groups = 1;
-  auto of = [&](auto s) { groups = row_threads(decltype(s)::G) / decltype(s)::G; };
+// Threads of a workgroup that adds up rows, and the groups of lanes in it that
+// hold a row each.
+struct RowGroups { int threads, groups; };
+static RowGroups row_groups(maxsim_dtype dtype, int64_t dim) {
+  RowGroups r{};
+  auto of = [&](auto s) {
+    constexpr int G = decltype(s)::G;
+    r = {row_threads(G), row_threads(G) / G};
+  };
   if (dtype == MAXSIM_FLOAT32) with_shape<kVec<F32>>(dim, of);
   else with_shape<kVec<F16>>(dim, of);
-  return groups;
+  return r;
 }
 
 struct EmbedLayout {
@@ -911,7 +916,7 @@ static EmbedLayout embed_layout(maxsim_dtype dtype, int64_t tokens, int64_t voca
   EmbedLayout l{};
   if (few_tokens(dtype, tokens, vocab, dim)) return l;
   // a group of lanes has up to 32 tokens, fewer where that leaves CUs idle
-  const uint32_t groups = (uint32_t)row_groups(dtype, dim);
+  const uint32_t groups = (uint32_t)row_groups(dtype, dim).groups;
   uint32_t share = 32;
   while (share > 2 && tokens / share < 8192) share /= 2;
   l.span = std::min<uint32_t>(std::max<uint32_t>(groups * share, 8), kMaxSpan);
@@ -1057,7 +1062,8 @@ int maxsim_amd_embed_backward(maxsim_dtype weight_dtype, maxsim_dtype dtype, con
   const ZeroArgs zero = zero_args(dweight, vocab, dim * element, element);
   const int64_t spans = (tokens + l.span - 1) / l.span;
   const int64_t blocks = spans + (vocab + zero.rows - 1) / zero.rows;
-  if (blocks > UINT32_MAX / 1024)
+  // a launch's threads fit 32 bits, those of 2^31 - 1 tokens of narrow rows too
+  if (blocks > UINT32_MAX / row_groups(dtype, dim).threads)
     return fail(MAXSIM_ERR_UNSUPPORTED, "table or gradient too large for one launch");
   char* ws = static_cast<char*>(workspace);
   uint32_t* total = reinterpret_cast<uint32_t*>(ws);
