@@ -50,3 +50,28 @@ def test_gradients_with_a_graph():
     kept = g.detach().clone()
     assert torch.equal(maxsim_amd.clip_grad_norm([g], 0.5), norm)
     assert torch.equal(g.detach(), kept * factor)
+
+
+@pytest.mark.parametrize("dynamic", [None, True])
+def test_compiled(dynamic):
+    torch._dynamo.reset()
+    compiled = lambda f: torch.compile(f, backend="aot_eager", fullgraph=True, dynamic=dynamic)
+
+    def clip(a, b, c):
+        return maxsim_amd.clip_grad_norm([a, b, c], 0.5), a * 2  # reads what was clipped
+
+    def step(p, g, m, v, at):
+        norm, factor = maxsim_amd.clip_factor([g], 0.5)
+        maxsim_amd.adamw_step([p], [g], [m], [v], step=at, grad_scale=factor)
+        return norm, factor
+
+    fast, fast_step = compiled(clip), compiled(step)
+    for seed in (5, 6):
+        x, y = _grads(seed), _grads(seed)
+        assert all(torch.equal(a, b) for a, b in zip(fast(*x), clip(*y)))
+        assert all(torch.equal(a, b) for a, b in zip(x, y))
+        x, y = ([rand(torch.Generator().manual_seed(seed), 500 + seed) for _ in range(2)] +
+                [torch.zeros(500 + seed, device="cuda") for _ in range(2)] +
+                [torch.ones(1, dtype=torch.int64, device="cuda")] for _ in range(2))
+        assert all(torch.equal(a, b) for a, b in zip(fast_step(*x), step(*y)))
+        assert all(torch.equal(a, b) for a, b in zip(x, y))
