@@ -954,6 +954,13 @@ std::tuple<Tensor, Tensor> clip_factor_autograd(at::TensorList grads, double max
 
 Tensor clip_grad_norm_autograd(at::TensorList grads, double max_norm, double eps) {
   refuse_tangents("clip_grad_norm", grads);
+  // as torch's operators in place: what stands there is a parameter, where
+  // torch.nn.utils' function would have taken one for its gradient
+  if (at::GradMode::is_enabled())
+    for (size_t i = 0; i < grads.size(); ++i)
+      TORCH_CHECK(!grads[i].requires_grad() || !grads[i].is_leaf(), "grads[", i,
+                  "] is a leaf that requires grad: clip_grad_norm takes the gradients, not the "
+                  "parameters (under torch.no_grad() any tensor)");
   at::AutoDispatchBelowADInplaceOrView guard;
   return MAXSIM_CALL(maxsim_clip_grad_norm, grads, max_norm, eps);
 }

@@ -75,3 +75,26 @@ def test_compiled(dynamic):
                 [torch.ones(1, dtype=torch.int64, device="cuda")] for _ in range(2))
         assert all(torch.equal(a, b) for a, b in zip(fast_step(*x), step(*y)))
         assert all(torch.equal(a, b) for a, b in zip(x, y))
+
+
+def test_parameters_are_not_clipped_in_place_of_gradients():
+    # torch.nn.utils.clip_grad_norm_ takes parameters: the same call here would
+    # have scaled the weights themselves
+    p = torch.nn.Parameter(rand(torch.Generator().manual_seed(7), 50))
+    q = torch.nn.Parameter(rand(torch.Generator().manual_seed(8), 70, dtype=torch.bfloat16))
+    kept = [p.detach().clone(), q.detach().clone()]
+    for call in (lambda: maxsim_amd.clip_grad_norm([p, q], 1e-3),
+                 lambda: maxsim_amd.clip_grad_norm([kept[0].clone(), q], 1e-3),
+                 lambda: maxsim_amd.clip_grad_norm(p, 1e-3)):
+        with pytest.raises(RuntimeError, match="leaf that requires grad"):
+            call()
+    assert torch.equal(p.detach(), kept[0]) and torch.equal(q.detach(), kept[1])
+    (p.sum() + q.sum()).backward()
+    grads = [p.grad, q.grad]  # what is meant
+    maxsim_amd.clip_grad_norm(grads, 1e-3)
+    assert float(maxsim_amd.grad_norm(grads)) < 1.1e-3
+    with torch.no_grad():
+        maxsim_amd.clip_grad_norm([p], 0.5)
+    assert float(maxsim_amd.grad_norm([p])) <= 0.5 * (1 + 2.0 ** -22)
+    # their norm is nothing that writes
+    assert float(maxsim_amd.grad_norm([q])) > 0
