@@ -153,3 +153,16 @@ def test_captured():
         torch.cuda.synchronize()
         assert torch.equal(y.detach(), maxsim_amd.embed_tokens(weight.detach(), ids, lens, scale=2.0))
         assert torch.equal(dw, _grad(weight, ids, lens, dy, scale=2.0)), turn
+
+
+def test_one_id_by_itself():
+    # ids without axes: a row of the table, and a gradient of one axis
+    gen = torch.Generator().manual_seed(20)
+    weight = rand(gen, 40, 24, dtype=torch.float16).requires_grad_(True)
+    y = maxsim_amd.embed_tokens(weight, torch.tensor(7, device="cuda"), scale=0.5)
+    assert y.shape == (24,) and torch.equal(y.detach(), weight.detach()[7] * 0.5)
+    for dy in (rand(gen, 24, dtype=torch.float16), rand(gen, 48, dtype=torch.float16)[::2]):
+        (dw,) = torch.autograd.grad(y, weight, dy, retain_graph=True)
+        assert torch.equal(dw[7], dy * 0.5)
+        dw[7] = 0
+        assert not dw.any()
