@@ -44,8 +44,8 @@ size_t maxsim_amd_embed_backward_workspace_size(maxsim_dtype dtype, int64_t toke
 /* dweight [vocab, dim] (in weight_dtype: dtype or float32): row v is scale
  * times the sum of the rows of dy [tokens, dim], `dy_stride` apart, whose
  * entry in `rows` is v, and 0 where there is none.  Entries outside
- * [0, vocab) belong to no row.  Sums are fp32, in an order that `rows` alone
- * decides, rounded once. */
+ * [0, vocab) belong to no row.  Sums are fp32, in an order that `rows` and the
+ * sizes alone decide, rounded once.  No tokens: dweight becomes 0. */
 int maxsim_amd_embed_backward(maxsim_dtype weight_dtype, maxsim_dtype dtype, const void* dy,
                               int64_t dy_stride, const int32_t* rows, int64_t tokens,
                               int64_t vocab, int64_t dim, float scale, void* dweight,

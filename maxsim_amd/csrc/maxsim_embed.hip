@@ -8,7 +8,7 @@
 // frequent token and none for most others of a large table.  Floating-point
 // atomics would do that in an order of their own every time, and one by one
 // for a frequent token; here the tokens are sorted by row first, stably, so
-// that the ids alone decide every order:
+// that the ids and the sizes alone decide every order:
 //   embed_few_kernel   few tokens: one launch does all of it in LDS;
 //   embed_count_kernel, embed_place_kernel   a pass of the sort of many;
 //   embed_sum_kernel   groups of lanes add up the tokens of one row each, of
@@ -25,8 +25,11 @@ namespace maxsim {
 // ---- forward -----------------------------------------------------------------
 
 // A result of more bytes than this goes past the caches, which then keep the
-// table (524288 tokens x 768, fp32 table, bf16 result: 217 us against 305, and
-// 579 against 617 with the layer norm that reads the result).  A smaller one is
+// table (524288 tokens x 768, fp32 table of 32000 rows, bf16 result, one launch
+// after the other: 217 us against 310, or 157 against 284 where 229376 of the
+// tokens are padding; with a table that other work has pushed out of the caches
+// 289 against 309 and 268 against 276; and 579 against 617 with the layer norm
+// that reads the result).  A smaller one is
 // mostly still there for its reader (40000 tokens: 18.7 against 20.1 us, but
 // 42.4 against 41.5 with the layer norm; 80000, 123 MB: 79 against 90).  Rows
 // that share lines with their neighbours leave pieces of lines behind, which

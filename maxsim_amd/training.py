@@ -16,8 +16,9 @@ both.
 
 The reference leaves these to torch (its training example, README.md:160-205).
 Here they are hand-written HIP kernels behind ``include/maxsim_amd_training.h``
-and ``include/maxsim_amd_encoder.h``: one pass over memory each, sums in fp32
-(the gradients' norm in 64 bits), 16-bit results rounded once.
+and ``include/maxsim_amd_encoder.h``: one pass over memory each (clipping in
+place has one for the norm and another where it clips), sums in fp32 (the
+gradients' norm in 64 bits), 16-bit results rounded once.
 Differentiable means first derivatives in reverse mode: the gradients have no
 derivatives of their own and forward-mode tangents are not carried (both raise).
 The gradients' norm, the factor and clipping record nothing in reverse mode, as
@@ -69,8 +70,8 @@ def embed_tokens(weight, ids, lengths=None, *, scale: float = 1.0, padding_idx=N
     Returns:
         ``[*ids.shape, dim]``, differentiable with respect to weight.  The
         gradient is dense, in weight's dtype: fp32 sums over the tokens of a
-        row, in an order that the ids alone decide, rounded once.  It takes up
-        to 2^31 - 1 tokens."""
+        row, in an order that the ids and the sizes alone decide, rounded once.
+        It takes up to 2^31 - 1 tokens."""
     _require_hip("weight", weight)
     if padding_idx is not None:
         rows = weight.shape[0]
