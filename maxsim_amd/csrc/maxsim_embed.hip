@@ -29,10 +29,9 @@ namespace maxsim {
 // after the other: 217 us against 310, or 157 against 284 where 229376 of the
 // tokens are padding; with a table that other work has pushed out of the caches
 // 289 against 309 and 268 against 276; and 579 against 617 with the layer norm
-// that reads the result).  A smaller one is
-// mostly still there for its reader (40000 tokens: 18.7 against 20.1 us, but
-// 42.4 against 41.5 with the layer norm; 80000, 123 MB: 79 against 90).  Rows
-// that share lines with their neighbours leave pieces of lines behind, which
+// that reads the result).  A smaller one is mostly still there for its reader
+// (40000 tokens: 18.7 against 20.1 us, but 42.4 against 41.5 with the layer
+// norm; 80000, 123 MB: 79 against 90).  Rows that share lines with their neighbours leave pieces of lines behind, which
 // costs short ones more than it gives (256000 x 304 bf16: 44 us against 35, x 301
 // fp32 99 and 99, x 1038 bf16 137 against 199).
 constexpr int64_t kCacheBytes = (int64_t)96 << 20, kCacheRow = 2048;

@@ -23,8 +23,9 @@ constexpr int kGradThreads = 256;
 // A workgroup's share: 16-byte loads that a thread has in flight.  One turn of
 // them (two: 64.5 us against 62.3 for 91 M fp32 gradients, multiplying them 134
 // against 127, launches of either kind in a row; where the norm has just read
-// them the multiplying takes 107), and shorter ones where there are few bytes, for more CUs
-// (100000 bf16 gradients: the squares 3.5 us against 5.4, clipping 3.1 against 5.3).
+// them the multiplying takes 107), and shorter ones where there are few bytes,
+// for more CUs (100000 bf16 gradients: the squares 3.5 us against 5.4, clipping
+// 3.1 against 5.3).
 template <int UNROLL_> struct Share {
   static constexpr int UNROLL = UNROLL_;
   static constexpr int64_t bytes = (int64_t)kGradThreads * 16 * UNROLL_;

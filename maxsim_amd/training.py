@@ -213,9 +213,10 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6) -> torch.Tensor
     The gradients (``[p.grad for p in parameters if p.grad is not None]``) are
     each dense in memory, in any order of their axes, and share none of it
     (ValueError).  A parameter in their place is refused, as by torch's own
-    operators in place, unless under ``torch.no_grad()``.  Products are rounded once.  Nothing is written where the
-    norm is within the limit.  No graph records it: gradients made with
-    ``create_graph`` are differentiated as if they had not been clipped."""
+    operators in place, unless under ``torch.no_grad()``.  Products are rounded
+    once.  Nothing is written where the norm is within the limit.  No graph
+    records it: gradients made with ``create_graph`` are differentiated as if
+    they had not been clipped."""
     grads = _grad_list(grads)
     if not grads:
         return _scalar_of_none(0.0)

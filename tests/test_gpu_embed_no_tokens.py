@@ -31,9 +31,10 @@ def test_empty_batches_of_every_width(dim, kind):
         assert dw.shape == weight.shape and dw.dtype == kind[0] and not dw.any()
 
 
-@pytest.mark.parametrize("vocab,dim", [(1, 16384), (5000, 4099), (300007, 1030)])
+@pytest.mark.parametrize("vocab,dim", [(1, 16384), (5000, 4099), (300007, 1030), (2 ** 29 + 5, 1)])
 def test_the_zeros_of_wide_tables(vocab, dim):
-    # several rows to a workgroup, and rows off every boundary
+    # several rows to a workgroup, rows off every boundary, and more rows than
+    # the launch takes tokens of
     rows = torch.empty(0, dtype=torch.int32, device="cuda")
     for dtype in (torch.float32, torch.bfloat16):
         junk = torch.full((vocab, dim), float("nan"), dtype=dtype, device="cuda")
